@@ -328,6 +328,93 @@ KANB200_API int kanb200_allreduce_sum_f32_ranges(const void* const* peer_bases, 
                                                  size_t pad_offset, int rank, int world, int local_ranks,
                                                  int blocks, int threads, float scale, int* status, void* stream);
 
+/* ---- around a layer: norms, gated residual connections, 8-bit checkpoints -------------------------------
+ * (no counterpart in the reference, whose networks are plain chains of layers; deep chains need the inputs of
+ * every layer inside its knots, a residual path around it, and less memory for what the backward reads)
+ *
+ * Rows of `width` columns.  The stream (x, out and their gradients) may be float32, float64, float16 or
+ * bfloat16; the branch (y, gate, h, parameters, statistics and their gradients) is what the layers compute in:
+ * float64 next to a float64 stream, float32 otherwise.  All arithmetic is done in the branch's type.
+ *
+ *   norm(v) = (v - m) r w + b     RMS:   m = 0,       r = (mean(v^2) + eps)^(-1/2)
+ *                                 LAYER: m = mean(v), r = (mean((v - m)^2) + eps)^(-1/2)
+ *
+ * kanb200_block_forward
+ *   y == NULL:  h = next(x)                                     the norm in front of a layer
+ *   otherwise:  out = x + scale * act(gate) * post(y)           the connection behind it, and, with
+ *               h = next(out)                                   next_norm, the norm of the next block in the same pass
+ *   (out is rounded to the stream's type first; h is the norm of what is stored.)  A NULL gate / scale / weight /
+ *   bias is left out (factor 1, summand 0).  gate_rows consecutive rows share one row of gate (1 = a gate per row).
+ *   post_stats / next_stats [rows, 2] = (m, r) of each row, for the backward (NULL = not wanted).
+ *   checkpoint != NONE also writes 8-bit codes of what the backward reads (each pair may be NULL = not wanted):
+ *   x_* of the norm's input (x, or out with y), y_* of y, gate_* of a gate per row.
+ *
+ * kanb200_block_backward
+ *   gradients for dout (of out; NULL = 0) and dh (of h; NULL = no norm to go through).  `x` is the norm's input (x
+ *   when y is absent in the forward, else out), needed with dh.  has_branch = 1 when the forward had y.  Where codes are
+ *   given the kernels restore x / y / gate from them and the tensor's own pointer is not read; the statistics are those
+ *   of the forward.  NULL output = not needed.  dgate [rows / gate_rows, width] is summed over the rows that share a
+ *   gate row.  The sums over rows go through slabs in the workspace that a second kernel adds in a fixed order: no
+ *   atomics, the same bits on every run.
+ * Row strides are in elements; a row's columns are contiguous.  out, h, dx, codes and scales are dense. */
+#define KANB200_F16  2   /* stream types of these operators only */
+#define KANB200_BF16 3
+
+#define KANB200_NORM_NONE  0
+#define KANB200_NORM_RMS   1
+#define KANB200_NORM_LAYER 2
+
+#define KANB200_ACT_NONE    0
+#define KANB200_ACT_SIGMOID 1
+#define KANB200_ACT_SILU    2
+
+#define KANB200_PACK_NONE 0
+#define KANB200_PACK_INT8 1
+#define KANB200_PACK_E4M3 2
+#define KANB200_PACK_GROUP 128   /* columns of a row that share one scale */
+
+typedef struct kanb200_block_args {
+    int dtype;                       /* of the stream: KANB200_F32 / F64 / F16 / BF16 */
+    int gate_act;                    /* KANB200_ACT_* */
+    int post_norm, next_norm;        /* KANB200_NORM_* */
+    int checkpoint;                  /* KANB200_PACK_* */
+    int has_branch;                  /* backward: the forward had y */
+    double eps;
+    int64_t rows, width;
+    const void* x;      int64_t x_stride;
+    const void* y;      int64_t y_stride;
+    const void* gate;   int64_t gate_stride;   int64_t gate_rows;
+    const void* scale;                                     /* [width] */
+    const void* post_weight; const void* post_bias;        /* [width] */
+    const void* next_weight; const void* next_bias;        /* [width] */
+    void* post_stats;   void* next_stats;                  /* [rows, 2]: written by the forward, read by the backward */
+    void* x_codes;      void* x_scales;                    /* [rows, width], [rows, ceil(width / 128)] */
+    void* y_codes;      void* y_scales;
+    void* gate_codes;   void* gate_scales;
+    void* out;          void* h;                           /* forward */
+    const void* dout;   int64_t dout_stride;               /* backward from here on */
+    const void* dh;     int64_t dh_stride;
+    void* dx;
+    void* dy;           int64_t dy_stride;
+    void* dgate;        int64_t dgate_stride;
+    void* dscale;       void* dpost_weight;  void* dpost_bias;  void* dnext_weight;  void* dnext_bias;   /* [width] */
+} kanb200_block_args;
+
+KANB200_API int kanb200_block_forward(const kanb200_block_args* args, void* stream);
+/* scratch of kanb200_block_backward for these arguments (plain scratch, no status header; 0 = none) */
+KANB200_API size_t kanb200_block_backward_workspace_bytes(const kanb200_block_args* args);
+KANB200_API int kanb200_block_backward(const kanb200_block_args* args, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* 8-bit checkpoint of an activation [rows, width]: per group of 128 columns of a row, A = max|x|,
+ *   scale = max(A * (1 / 127), smallest normal) (E4M3: 1 / 448),  code = round-to-nearest-even(x * (1 / scale)),
+ * and back: x = code * scale.  Codes are int8 or e4m3 bytes, scales float32 (float64 for float64 x).  A group that holds
+ * a NaN or an infinity comes back as NaN. */
+KANB200_API int kanb200_pack_activation(int dtype, int format, const void* x, int64_t x_stride, void* codes,
+                                        void* scales, int64_t rows, int64_t width, void* stream);
+KANB200_API int kanb200_unpack_activation(int dtype, int format, const void* codes, const void* scales, void* x,
+                                          int64_t rows, int64_t width, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,15 +16,18 @@ them are identical, not copies.
 import sys as _sys
 
 import torchsplinekan_b200 as _impl
-from torchsplinekan_b200 import _C, dense_backend, fused, kan, kan_linear, pruning
+from torchsplinekan_b200 import _C, block, dense_backend, fused, kan, kan_linear, pruning
 from torchsplinekan_b200 import KAN, KANLinear, __version__
+from torchsplinekan_b200.block import block_norm, gated_residual, pack_activation, unpack_activation
 from torchsplinekan_b200.pruning import PruneResult, prune_nodes
 
 reference_backend = dense_backend
 
-for _name, _mod in (("_C", _C), ("reference_backend", dense_backend), ("fused", fused), ("kan", kan),
+for _name, _mod in (("_C", _C), ("reference_backend", dense_backend), ("block", block), ("fused", fused),
+                    ("kan", kan),
                     ("kan_linear", kan_linear), ("pruning", pruning)):
     _sys.modules[f"{__name__}.{_name}"] = _mod
 del _name, _mod
 
-__all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "__version__"]
+__all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "block_norm", "gated_residual",
+           "pack_activation", "unpack_activation", "__version__"]

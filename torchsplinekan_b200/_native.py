@@ -26,6 +26,28 @@ MAX_IN_FEATURES = 65535
 
 _c_void_p, _c_int, _c_i64, _c_size = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 
+# Stream types of the operators around a layer, besides F32 and F64, and their settings.
+F16, BF16 = 2, 3
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+ACT_NONE, ACT_SIGMOID, ACT_SILU = 0, 1, 2
+PACK_NONE, PACK_INT8, PACK_E4M3, PACK_GROUP = 0, 1, 2, 128
+
+
+class BlockArgs(ctypes.Structure):
+    """``kanb200_block_args`` (fields and their meaning: include/kan_b200.h); everything starts as 0 / NULL."""
+    _fields_ = (
+        [(n, _c_int) for n in ("dtype", "gate_act", "post_norm", "next_norm", "checkpoint", "has_branch")]
+        + [("eps", ctypes.c_double), ("rows", _c_i64), ("width", _c_i64)]
+        + [("x", _c_void_p), ("x_stride", _c_i64), ("y", _c_void_p), ("y_stride", _c_i64),
+           ("gate", _c_void_p), ("gate_stride", _c_i64), ("gate_rows", _c_i64)]
+        + [(n, _c_void_p) for n in ("scale", "post_weight", "post_bias", "next_weight", "next_bias", "post_stats",
+                                    "next_stats", "x_codes", "x_scales", "y_codes", "y_scales", "gate_codes",
+                                    "gate_scales", "out", "h")]
+        + [("dout", _c_void_p), ("dout_stride", _c_i64), ("dh", _c_void_p), ("dh_stride", _c_i64), ("dx", _c_void_p),
+           ("dy", _c_void_p), ("dy_stride", _c_i64), ("dgate", _c_void_p), ("dgate_stride", _c_i64)]
+        + [(n, _c_void_p) for n in ("dscale", "dpost_weight", "dpost_bias", "dnext_weight", "dnext_bias")])
+
+
 # name -> (restype, argtypes); must list every symbol of include/kan_b200.h
 SIGNATURES = {
     "kanb200_last_error": (ctypes.c_char_p, []),
@@ -74,6 +96,13 @@ SIGNATURES = {
     "kanb200_backward_param_rows": (_c_int, [_c_int] + [_c_void_p] * 9 + [_c_i64, _c_i64, _c_i64, _c_int, _c_int,
                                                                           _c_i64, _c_i64, _c_void_p, _c_size,
                                                                           _c_void_p]),
+    "kanb200_block_forward": (_c_int, [_c_void_p, _c_void_p]),
+    "kanb200_block_backward_workspace_bytes": (_c_size, [_c_void_p]),
+    "kanb200_block_backward": (_c_int, [_c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "kanb200_pack_activation": (_c_int, [_c_int, _c_int, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_i64,
+                                         _c_void_p]),
+    "kanb200_unpack_activation": (_c_int, [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64,
+                                           _c_void_p]),
     "kanb200_allreduce_pad_bytes": (_c_size, [_c_int, _c_int]),
     "kanb200_allreduce_set_wait_limit_ms": (_c_int, [_c_int]),
     "kanb200_allreduce_sum_f32_ranges": (_c_int, [ctypes.POINTER(_c_void_p), _c_void_p, ctypes.POINTER(_c_size),

@@ -1,0 +1,95 @@
+"""
+Operators around a KAN layer: the norm in front of it, the gated residual connection behind it, and 8-bit checkpoints of
+what a training step keeps for its backward.  The reference has no counterpart (its networks are plain chains of
+layers); deep chains need the inputs of every layer inside that layer's knots, a residual path around it, and less memory
+per layer.
+
+Rows are the leading dimensions, columns the last one.  The *stream* (``x``, the result of :func:`gated_residual`) may
+be float32, float64, bfloat16 or float16; the *branch* (``y``, gates, parameters, the norm's result) is what
+:class:`KANLinear` computes in: float64 next to a float64 stream, float32 otherwise.
+
+CUDA tensors run on the native kernels (one kernel forward; backward one kernel plus the fixed-order sum of the
+parameter gradients), CPU tensors on dense PyTorch formulas.  ``create_graph=True`` is exact without a checkpoint and
+raises with one.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _C
+
+NORMS = {None: 0, "rms": 1, "layer": 2}
+GATE_ACTIVATIONS = {None: 0, "sigmoid": 1, "silu": 2}
+CHECKPOINTS = {None: 0, "int8": 1, "e4m3": 2}
+PACK_GROUP = int(_C.PACK_GROUP)
+
+
+def _code(table: dict, name: str, value) -> int:
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        raise ValueError(f"{name} must be one of {list(table)}, got {value!r}") from None
+
+
+def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+               kind: str = "rms", eps: float = 1e-6, checkpoint: Optional[str] = None) -> torch.Tensor:
+    """``(x - m) r * weight + bias`` over the last dimension, in the branch's type: the norm in front of a layer.
+
+    ``kind``: "rms" (``m = 0``, ``r = (mean(x^2) + eps)^-1/2``) or "layer" (``m = mean(x)``,
+    ``r = (mean((x - m)^2) + eps)^-1/2``).
+
+    ``checkpoint``: None keeps ``x`` for the backward; "int8" / "e4m3" keep 8-bit codes of it instead (see
+    :func:`pack_activation`), written by the same kernel.  The result is the same; the gradients are those of the
+    formulas with the restored ``x`` next to the exact ``m`` and ``r``."""
+    kind_code = _code(NORMS, "kind", kind)
+    if kind_code == 0:
+        raise ValueError("kind must be 'rms' or 'layer', got None")
+    return _C.block_norm(x, weight, bias, kind_code, eps, _code(CHECKPOINTS, "checkpoint", checkpoint))
+
+
+def gated_residual(x: torch.Tensor, y: torch.Tensor, *, gate: Union[torch.Tensor, str, None] = None,
+                   gate_activation: Optional[str] = None, scale: Optional[torch.Tensor] = None,
+                   post_norm: Optional[str] = None, post_weight: Optional[torch.Tensor] = None,
+                   post_bias: Optional[torch.Tensor] = None, next_norm: Optional[str] = None,
+                   next_weight: Optional[torch.Tensor] = None, next_bias: Optional[torch.Tensor] = None,
+                   eps: float = 1e-6, checkpoint: Optional[str] = None
+                   ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """The connection behind a layer, ``out = x + scale * act(gate) * post(y)``, in one pass.
+
+    ``gate``: None; a tensor of ``x``'s shape; one of size 1 in trailing row dimensions (``[B, 1, D]`` next to an ``x`` of
+    ``[B, T, D]``: one gate per sequence; ``[D]``: one for all rows); or "packed": ``y`` is ``[..., 2 D]`` and holds value
+    and gate side by side.  ``gate_activation``: None, "sigmoid" or "silu".  ``scale``: ``[D]``.
+    ``post_norm`` / ``next_norm``: None, "rms" or "layer", as in :func:`block_norm`.
+
+    With ``next_norm`` the result is ``(out, h)`` where ``h`` is the norm of ``out`` (as stored, in ``x``'s type) for the
+    next block.  ``checkpoint``: what the backward reads of ``y``, of a gate per row and of ``out`` is kept as 8-bit codes;
+    a shared gate is kept as it is."""
+    packed = isinstance(gate, str)
+    if packed:
+        if gate != "packed":
+            raise ValueError(f"gate must be a tensor, None or 'packed', got {gate!r}")
+        gate = None
+    return _C.gated_residual(x, y, gate, packed, _code(GATE_ACTIVATIONS, "gate_activation", gate_activation), scale,
+                             _code(NORMS, "post_norm", post_norm), post_weight, post_bias,
+                             _code(NORMS, "next_norm", next_norm), next_weight, next_bias, eps,
+                             _code(CHECKPOINTS, "checkpoint", checkpoint))
+
+
+def pack_activation(x: torch.Tensor, format: str = "int8") -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)``: ``x`` in 8 bits with one scale per 128 columns of a row.
+
+    Per group, with ``A = max|x|``: ``scale = max(A / 127, smallest normal)`` ("e4m3": ``A / 448``) and
+    ``codes = round(x / scale)``, int8 or float8_e4m3fn.  "int8" has the smaller error on inputs of about one size
+    (at most ``A / 254``), "e4m3" keeps relative precision (``2^-4``) over a wide range.  A group that holds a NaN or an
+    infinity comes back as NaN, so an overflow stays visible.  CUDA tensors only; no gradient flows through it."""
+    code = _code(CHECKPOINTS, "format", format)
+    if code == 0:
+        raise ValueError("format must be 'int8' or 'e4m3', got None")
+    return _C.pack_activation(x, code)
+
+
+def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``codes * scales`` in ``dtype`` (default: the type of the scales)."""
+    return _C.unpack_activation(codes, scales, scales.dtype if dtype is None else dtype)

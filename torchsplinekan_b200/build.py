@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import concurrent.futures
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -17,13 +18,14 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libkan_b200.so")
-SOURCES = ["kan_capi.cu", "kan_simt.cu", "kan_reg.cu", "kan_dense64.cu", "kan_tc.cu", "kan_tc_edge.cu", "kan_refit.cu", "kan_collective.cu"]
+SOURCES = ["kan_capi.cu", "kan_simt.cu", "kan_reg.cu", "kan_dense64.cu", "kan_tc.cu", "kan_tc_edge.cu", "kan_refit.cu", "kan_collective.cu", "kan_block.cu", "kan_pack.cu"]
 # test-only library (operand-layout self-test); never loaded by the package
 SELFTEST_SOURCE = "kan_selftest.cu"
 SELFTEST_PATH = os.path.join(LIB_DIR, "libkan_b200_selftest.so")
 # PyTorch operator layer (TORCH_LIBRARY + pybind + autograd node), host C++ only
-EXT_SOURCE = "kan_torch_ext.cpp"
-HEADERS = ["kan_device.cuh", "kan_dmma.cuh", "kan_internal.h", "kan_table.cuh", "kan_tc_ptx.cuh", "kan_tc_common.cuh", os.path.join("..", "..", "include", "kan_b200.h")]
+EXT_SOURCES = ["kan_torch_ext.cpp", "kan_block_ext.cpp"]
+EXT_HEADERS = ["kan_ext_util.h", os.path.join("..", "..", "include", "kan_b200.h")]
+HEADERS = ["kan_block.h", "kan_block.cuh", "kan_device.cuh", "kan_dmma.cuh", "kan_internal.h", "kan_table.cuh", "kan_tc_ptx.cuh", "kan_tc_common.cuh", os.path.join("..", "..", "include", "kan_b200.h")]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=hidden"]
@@ -41,6 +43,20 @@ def _older_than(target: str, deps) -> bool:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _includes(src: str) -> set:
+    """The repository's headers that a source includes, directly or through another one."""
+    found, todo = set(), [os.path.join(CSRC, src)]
+    while todo:
+        at = todo.pop()
+        with open(at) as f:
+            names = re.findall(r'^#include "([^"]+)"', f.read(), re.M)
+        for path in (os.path.normpath(os.path.join(os.path.dirname(at), n)) for n in names):
+            if path not in found:
+                found.add(path)
+                todo.append(path)
+    return found
 
 
 def _stale() -> bool:
@@ -67,12 +83,12 @@ def build_selftest(force: bool = False) -> str:
 
 
 def build_extension(force: bool = False) -> str:
-    """Compiles the PyTorch operator layer (csrc/kan_torch_ext.cpp) into ``_C.<abi>.so`` beside the
+    """Compiles the PyTorch operator layer (csrc/kan_torch_ext.cpp, csrc/kan_block_ext.cpp) into ``_C.<abi>.so`` beside the
     package's Python files; it links libkan_b200.so (found at run time through ``$ORIGIN/lib``)."""
     import sysconfig
     target = ext_path()
-    src = os.path.join(CSRC, EXT_SOURCE)
-    if not force and not _older_than(target, [src, os.path.join(PKG, "..", "include", "kan_b200.h"), LIB_PATH]):
+    deps = [os.path.join(CSRC, s) for s in EXT_SOURCES + EXT_HEADERS]
+    if not force and not _older_than(target, deps + [LIB_PATH]):
         return target
     import torch
     from torch.utils import cpp_extension as ce
@@ -85,16 +101,30 @@ def build_extension(force: bool = False) -> str:
     # interpreter's other extension modules (a toolchain that links its own copy statically breaks
     # stream formatting inside the module).
     cxx = shutil.which("g++", path="/usr/bin:/usr/local/bin:/bin") or shutil.which("g++") or "g++"
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *["-I" + p for p in ce.include_paths()], "-I" + sysconfig.get_paths()["include"],
-           "-I" + os.path.join(cuda_home, "include"), src, "-o", target + ".tmp",
-           "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
-           "-L" + LIB_DIR, "-lkan_b200", "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib, *cudart]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {EXT_SOURCE}:\n{r.stdout}\n{r.stderr[-6000:]}")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+             "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *["-I" + p for p in ce.include_paths()], "-I" + sysconfig.get_paths()["include"],
+             "-I" + os.path.join(cuda_home, "include")]
+    obj_dir = os.path.join(PKG, "build")
+    os.makedirs(obj_dir, exist_ok=True)
+
+    def run(cmd, what: str) -> None:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed for {what}:\n{r.stdout}\n{r.stderr[-6000:]}")
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(obj_dir, src.replace(".cpp", ".ext.o"))
+        if force or _older_than(obj, [os.path.join(CSRC, src), *_includes(src)]):
+            run([cxx, *flags, "-c", os.path.join(CSRC, src), "-o", obj], src)
+        return obj
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(EXT_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, EXT_SOURCES))
+    run([cxx, "-shared", *objs, "-o", target + ".tmp",
+         "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+         "-L" + LIB_DIR, "-lkan_b200", "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib, *cudart], "the operator layer")
     os.replace(target + ".tmp", target)
     return target
 
@@ -118,6 +148,8 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
 
     def compile_one(src: str) -> str:
         obj = os.path.join(obj_dir, src.replace(".cu", ".o"))
+        if not force and not verbose and not _older_than(obj, [os.path.join(CSRC, src), *_includes(src)]):
+            return obj
         cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             cmd.insert(1, "-Xptxas")

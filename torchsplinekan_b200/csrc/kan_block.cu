@@ -1,0 +1,426 @@
+// The norm in front of a KAN layer and the gated residual connection behind it, forward and backward.
+//
+//   forward   [out = x + scale act(gate) post(y)],  h = next(out or x)
+//   backward  g = dout + next'(dh),  dx = g,  dz = g scale act(gate),  dy = post'(dz),
+//             dgate = g scale act'(gate) z,  and the sums over rows of the five parameters
+//   norm'(d)  = r (v - mean(v) - xhat mean(v xhat)),  v = d w        (mean(v) for LAYER only)
+//
+// One pass over memory is the floor: 5 floats per element forward and 8 backward with everything on, a few dozen
+// operations each, so bandwidth bounds the large calls and latency the small ones.
+#include "kan_block.cuh"
+
+#include <algorithm>
+
+namespace kanb200 {
+namespace {
+
+constexpr int kLoopThreads = 256;
+constexpr int kMaxColumnSums = 5;
+
+template <typename B, int K> __device__ __forceinline__ void warp_sum(B (&v)[K]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+}
+
+// Sums of K values over the block, the same bits in every thread (fixed order over the warps).
+template <typename B, int K> __device__ __forceinline__ void block_sum(B (&v)[K], B* buf) {
+    warp_sum<B, K>(v);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    __syncthreads();                                        // buf may still be read from the sum before
+    if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) buf[k * 32 + warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        B s = B(0);
+        for (int w = 0; w < nw; ++w) s += buf[k * 32 + w];
+        v[k] = s;
+    }
+}
+
+// Calls body(c) for the columns of this thread: a warp owns blocks of 128 columns (the groups of a checkpoint).
+template <typename F> __device__ __forceinline__ void for_columns(int64_t width, F body) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    for (int64_t b = warp; b * kPackGroup < width; b += nw)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t c = b * kPackGroup + e * 32 + lane;
+            if (c < width) body(c);
+        }
+}
+
+// Codes and scales of one row; value(c) gives its elements.
+template <typename B, typename F>
+__device__ __forceinline__ void pack_row(int format, uint8_t* codes, B* scales, int64_t width, F value) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    for (int64_t b = warp; b * kPackGroup < width; b += nw) {
+        B v[4];
+        typename AbsBits<B>::type top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t c = b * kPackGroup + e * 32 + lane;
+            v[e] = c < width ? value(c) : B(0);
+            top = max(top, AbsBits<B>::of(v[e]));
+        }
+        const B scale = pack_scale<B>(format, AbsBits<B>::back(lanes_max<32>(top))), inv = pack_inverse<B>(scale);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t c = b * kPackGroup + e * 32 + lane;
+            if (c < width) codes[c] = (uint8_t)to_code(format, v[e], inv);
+        }
+        if (lane == 0) scales[b] = scale;
+    }
+}
+
+template <typename B> struct Moments {
+    B mean, rstd;
+};
+
+// m and r of a row whose elements are value(c): two passes, so that the variance has no cancellation.
+template <typename B, typename F>
+__device__ __forceinline__ Moments<B> row_moments(int kind, int64_t width, B eps, B* buf, F value) {
+    B m = B(0);
+    if (kind == kNormLayer) {
+        B s[1] = {B(0)};
+        for_columns(width, [&](int64_t c) { s[0] += value(c); });
+        block_sum<B, 1>(s, buf);
+        m = s[0] / B(width);
+    }
+    B s[1] = {B(0)};
+    for_columns(width, [&](int64_t c) {
+        const B d = value(c) - m;
+        s[0] += d * d;
+    });
+    block_sum<B, 1>(s, buf);
+    return {m, inv_sqrt(s[0] / B(width) + eps)};
+}
+
+// ---- rows of any width: a block per row, passes over the row in the caches ------------------------------------------
+template <typename S> __global__ void __launch_bounds__(kLoopThreads) loop_forward_kernel(const kanb200_block_args a) {
+    using B = Br<S>;
+    __shared__ B buf[32];
+    const int64_t D = a.width, groups = (D + kPackGroup - 1) / kPackGroup;
+    const B eps = B(a.eps);
+    const B *scale = static_cast<const B*>(a.scale), *pw = static_cast<const B*>(a.post_weight),
+            *pb = static_cast<const B*>(a.post_bias), *nw = static_cast<const B*>(a.next_weight),
+            *nb = static_cast<const B*>(a.next_bias);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const S* x = static_cast<const S*>(a.x) + row * a.x_stride;
+        if (a.y) {
+            const B* y = static_cast<const B*>(a.y) + row * a.y_stride;
+            const B* gate = a.gate ? static_cast<const B*>(a.gate) + row / a.gate_rows * a.gate_stride : nullptr;
+            S* out = static_cast<S*>(a.out) + row * D;
+            Moments<B> p{B(0), B(1)};
+            if (a.post_norm != kNormNone) {
+                p = row_moments<B>(a.post_norm, D, eps, buf, [&](int64_t c) { return y[c]; });
+                if (a.post_stats && threadIdx.x == 0) {
+                    static_cast<B*>(a.post_stats)[2 * row] = p.mean;
+                    static_cast<B*>(a.post_stats)[2 * row + 1] = p.rstd;
+                }
+            }
+            for_columns(D, [&](int64_t c) {
+                B z = (y[c] - p.mean) * p.rstd;
+                if (pw) z *= pw[c];
+                if (pb) z += pb[c];
+                B t = gate ? gate_value<B>(a.gate_act, gate[c]) : B(1);
+                if (scale) t *= scale[c];
+                out[c] = narrow<S>(widen(x[c]) + t * z);
+            });
+            if (a.y_codes)
+                pack_row<B>(a.checkpoint, static_cast<uint8_t*>(a.y_codes) + row * D,
+                            static_cast<B*>(a.y_scales) + row * groups, D, [&](int64_t c) { return y[c]; });
+            if (a.gate_codes)
+                pack_row<B>(a.checkpoint, static_cast<uint8_t*>(a.gate_codes) + row * D,
+                            static_cast<B*>(a.gate_scales) + row * groups, D, [&](int64_t c) { return gate[c]; });
+            x = out;                                        // each thread reads back only what it wrote
+        }
+        if (a.next_norm != kNormNone) {
+            const Moments<B> n = row_moments<B>(a.next_norm, D, eps, buf, [&](int64_t c) { return widen(x[c]); });
+            if (a.next_stats && threadIdx.x == 0) {
+                static_cast<B*>(a.next_stats)[2 * row] = n.mean;
+                static_cast<B*>(a.next_stats)[2 * row + 1] = n.rstd;
+            }
+            B* h = static_cast<B*>(a.h) + row * D;
+            for_columns(D, [&](int64_t c) {
+                B v = (widen(x[c]) - n.mean) * n.rstd;
+                if (nw) v *= nw[c];
+                if (nb) v += nb[c];
+                h[c] = v;
+            });
+        }
+        if (a.x_codes)
+            pack_row<B>(a.checkpoint, static_cast<uint8_t*>(a.x_codes) + row * D,
+                        static_cast<B*>(a.x_scales) + row * groups, D, [&](int64_t c) { return widen(x[c]); });
+    }
+}
+
+// Work of the backward: items of `chunk` consecutive rows that share a gate row, dealt to the blocks in turn.
+struct Split {
+    int64_t span;        // rows per gate row (all rows when no gate is shared)
+    int64_t chunk;       // rows per item
+    int64_t per_span;    // items per span
+    int64_t items;
+    int blocks;
+};
+
+enum { kSumScale, kSumPostWeight, kSumPostBias, kSumNextWeight, kSumNextBias };
+
+struct BackwardSlabs {
+    void* column[kMaxColumnSums];    // [blocks, width] each; NULL = not needed
+    void* gate;                      // [items, width]: per-item sums of dgate (the output itself with one item per span)
+};
+
+template <typename S>
+__global__ void __launch_bounds__(kLoopThreads) loop_backward_kernel(const kanb200_block_args a, const Split sp,
+                                                                    const BackwardSlabs slabs) {
+    using B = Br<S>;
+    __shared__ B buf[64];
+    const int64_t D = a.width, groups = (D + kPackGroup - 1) / kPackGroup;
+    const B *scale = static_cast<const B*>(a.scale), *pw = static_cast<const B*>(a.post_weight),
+            *pb = static_cast<const B*>(a.post_bias), *nw = static_cast<const B*>(a.next_weight);
+    B* sum[kMaxColumnSums];
+#pragma unroll
+    for (int k = 0; k < kMaxColumnSums; ++k)
+        sum[k] = slabs.column[k] ? static_cast<B*>(slabs.column[k]) + (int64_t)blockIdx.x * D : nullptr;
+    for_columns(D, [&](int64_t c) {
+#pragma unroll
+        for (int k = 0; k < kMaxColumnSums; ++k)
+            if (sum[k]) sum[k][c] = B(0);
+    });
+    const bool shared_gate = a.gate && a.gate_rows > 1;
+    for (int64_t item = blockIdx.x; item < sp.items; item += gridDim.x) {
+        const int64_t span = item / sp.per_span, first = span * sp.span + item % sp.per_span * sp.chunk;
+        const int64_t last = min(min(first + sp.chunk, (span + 1) * sp.span), a.rows);
+        B* gate_sum = shared_gate && slabs.gate ? static_cast<B*>(slabs.gate) + item * D : nullptr;
+        for (int64_t row = first; row < last; ++row) {
+            const S* dout = a.dout ? static_cast<const S*>(a.dout) + row * a.dout_stride : nullptr;
+            const B* dh = a.dh ? static_cast<const B*>(a.dh) + row * a.dh_stride : nullptr;
+            B n_mean = B(0), n_rstd = B(0), n_flat = B(0), n_along = B(0);
+            auto nhat = [&](int64_t c) {
+                const B v = a.x_codes ? from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.x_codes)[row * D + c],
+                                                     static_cast<const B*>(a.x_scales)[row * groups + c / kPackGroup])
+                                      : widen(static_cast<const S*>(a.x)[row * a.x_stride + c]);
+                return (v - n_mean) * n_rstd;
+            };
+            if (dh) {
+                n_mean = static_cast<const B*>(a.next_stats)[2 * row];
+                n_rstd = static_cast<const B*>(a.next_stats)[2 * row + 1];
+                B s[2] = {B(0), B(0)};
+                for_columns(D, [&](int64_t c) {
+                    const B v = nw ? dh[c] * nw[c] : dh[c], xh = nhat(c);
+                    s[0] += v;
+                    s[1] += v * xh;
+                    if (sum[kSumNextWeight]) sum[kSumNextWeight][c] += dh[c] * xh;
+                    if (sum[kSumNextBias]) sum[kSumNextBias][c] += dh[c];
+                });
+                block_sum<B, 2>(s, buf);
+                n_flat = a.next_norm == kNormLayer ? s[0] / B(D) : B(0);
+                n_along = s[1] / B(D);
+            }
+            auto grad = [&](int64_t c) {
+                B g = dout ? widen(dout[c]) : B(0);
+                if (dh) g += n_rstd * ((nw ? dh[c] * nw[c] : dh[c]) - n_flat - nhat(c) * n_along);
+                return g;
+            };
+            if (a.dx) for_columns(D, [&](int64_t c) { static_cast<S*>(a.dx)[row * D + c] = narrow<S>(grad(c)); });
+            if (!a.has_branch) continue;
+            B p_mean = B(0), p_rstd = B(1);
+            if (a.post_norm != kNormNone) {
+                p_mean = static_cast<const B*>(a.post_stats)[2 * row];
+                p_rstd = static_cast<const B*>(a.post_stats)[2 * row + 1];
+            }
+            auto yhat = [&](int64_t c) {
+                const B v = a.y_codes ? from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.y_codes)[row * D + c],
+                                                     static_cast<const B*>(a.y_scales)[row * groups + c / kPackGroup])
+                                      : static_cast<const B*>(a.y)[row * a.y_stride + c];
+                return (v - p_mean) * p_rstd;
+            };
+            auto gate = [&](int64_t c, B& act, B& dact) {
+                act = B(1);
+                dact = B(0);
+                if (a.gate_codes)
+                    gate_value_grad<B>(a.gate_act,
+                                       from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.gate_codes)[row * D + c],
+                                                    static_cast<const B*>(a.gate_scales)[row * groups + c / kPackGroup]),
+                                       act, dact);
+                else if (a.gate)
+                    gate_value_grad<B>(a.gate_act,
+                                       static_cast<const B*>(a.gate)[row / a.gate_rows * a.gate_stride + c], act, dact);
+            };
+            B s[2] = {B(0), B(0)};
+            for_columns(D, [&](int64_t c) {
+                const B g = grad(c), yh = yhat(c);
+                B z = pw ? yh * pw[c] : yh, act, dact;
+                if (pb) z += pb[c];
+                gate(c, act, dact);
+                const B gs = scale ? g * scale[c] : g, dz = gs * act;
+                if (sum[kSumScale]) sum[kSumScale][c] += g * act * z;
+                if (a.dgate && !shared_gate) static_cast<B*>(a.dgate)[row * a.dgate_stride + c] = gs * dact * z;
+                if (gate_sum) gate_sum[c] = (row == first ? B(0) : gate_sum[c]) + gs * dact * z;
+                if (sum[kSumPostWeight]) sum[kSumPostWeight][c] += dz * yh;
+                if (sum[kSumPostBias]) sum[kSumPostBias][c] += dz;
+                const B u = pw ? dz * pw[c] : dz;
+                s[0] += u;
+                s[1] += u * yh;
+            });
+            if (!a.dy) continue;
+            B p_flat = B(0), p_along = B(0);
+            if (a.post_norm != kNormNone) {
+                block_sum<B, 2>(s, buf);
+                p_flat = a.post_norm == kNormLayer ? s[0] / B(D) : B(0);
+                p_along = s[1] / B(D);
+            }
+            for_columns(D, [&](int64_t c) {
+                B act, dact;
+                gate(c, act, dact);
+                B u = grad(c) * act;
+                if (scale) u *= scale[c];
+                if (pw) u *= pw[c];
+                static_cast<B*>(a.dy)[row * a.dy_stride + c] =
+                    a.post_norm != kNormNone ? p_rstd * (u - p_flat - yhat(c) * p_along) : u;
+            });
+        }
+    }
+}
+
+// dst[g][c] = sum over i < n of slab[(g n + i)][c], in that order within 8 interleaved partial sums that are then added
+// in order: the same bits on every run.  A block sums 32 columns of one g; blockIdx.y deals out the g.
+struct SlabSum {
+    const void* slab;
+    void* dst;
+    int64_t dst_stride;
+};
+struct SlabSums {
+    SlabSum part[kMaxColumnSums];
+};
+template <typename B>
+__global__ void __launch_bounds__(256) sum_slabs_kernel(const SlabSums sums, int64_t width, int64_t n, int64_t spans) {
+    __shared__ B buf[8][33];
+    const SlabSum p = sums.part[blockIdx.z];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    for (int64_t g = blockIdx.y; g < spans; g += gridDim.y) {
+        const B* slab = static_cast<const B*>(p.slab) + g * n * width;
+        B s = B(0);
+        if (c < width)
+            for (int64_t i = warp; i < n; i += 8) s += slab[i * width + c];
+        __syncthreads();
+        buf[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0 && c < width) {
+#pragma unroll
+            for (int w = 1; w < 8; ++w) s += buf[w][lane];
+            static_cast<B*>(p.dst)[g * p.dst_stride + c] = s;
+        }
+    }
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+size_t branch_bytes(int dtype) { return dtype == KANB200_F64 ? 8 : 4; }
+
+Split split_rows(const kanb200_block_args& a) {
+    Split s;
+    const bool shared = a.dgate && a.gate_rows > 1;
+    s.span = shared ? a.gate_rows : a.rows;
+    s.chunk = shared ? std::min<int64_t>(a.gate_rows, std::max<int64_t>(1, a.rows / 592)) : 1;
+    s.per_span = div_up(s.span, s.chunk);
+    s.items = div_up(a.rows, s.span) * s.per_span;
+    s.blocks = (int)std::min<int64_t>(s.items, 592);
+    return s;
+}
+
+void column_outputs(const kanb200_block_args& a, void* (&out)[kMaxColumnSums]) {
+    out[kSumScale] = a.dscale;
+    out[kSumPostWeight] = a.dpost_weight;
+    out[kSumPostBias] = a.dpost_bias;
+    out[kSumNextWeight] = a.dnext_weight;
+    out[kSumNextBias] = a.dnext_bias;
+}
+
+// slabs of the column sums first, then those of a shared gate
+size_t lay_out_slabs(const kanb200_block_args& a, const Split& s, void* ws, BackwardSlabs& slabs) {
+    const size_t row = (size_t)a.width * branch_bytes(a.dtype);
+    void* outs[kMaxColumnSums];
+    column_outputs(a, outs);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        void* p = static_cast<char*>(ws) + at;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    };
+    for (int k = 0; k < kMaxColumnSums; ++k)
+        slabs.column[k] = !outs[k] ? nullptr : s.blocks == 1 ? outs[k] : take(row * s.blocks);
+    slabs.gate = nullptr;
+    if (a.dgate && a.gate_rows > 1)
+        slabs.gate = s.per_span == 1 && a.dgate_stride == a.width ? a.dgate : take(row * s.items);
+    return at;
+}
+
+template <typename S> cudaError_t launch_forward(const kanb200_block_args& a, cudaStream_t st) {
+    const int blocks = (int)std::min<int64_t>(a.rows, 148 * 8);
+    loop_forward_kernel<S><<<blocks, kLoopThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename S>
+cudaError_t launch_backward(const kanb200_block_args& a, void* ws, cudaStream_t st) {
+    using B = Br<S>;
+    const Split s = split_rows(a);
+    BackwardSlabs slabs;
+    lay_out_slabs(a, s, ws, slabs);
+    loop_backward_kernel<S><<<s.blocks, kLoopThreads, 0, st>>>(a, s, slabs);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    void* outs[kMaxColumnSums];
+    column_outputs(a, outs);
+    SlabSums sums;
+    int n = 0;
+    for (int k = 0; k < kMaxColumnSums; ++k)
+        if (outs[k] && slabs.column[k] != outs[k]) sums.part[n++] = {slabs.column[k], outs[k], a.width};
+    const unsigned cols = (unsigned)div_up(a.width, 32);
+    if (n > 0) {
+        sum_slabs_kernel<B><<<dim3(cols, 1, n), 256, 0, st>>>(sums, a.width, s.blocks, 1);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    if (slabs.gate && slabs.gate != a.dgate) {
+        const int64_t spans = s.items / s.per_span;
+        sums.part[0] = {slabs.gate, a.dgate, a.dgate_stride};
+        sum_slabs_kernel<B><<<dim3(cols, (unsigned)std::min<int64_t>(spans, 65535), 1), 256, 0, st>>>(sums, a.width,
+                                                                                                     s.per_span, spans);
+        e = cudaGetLastError();
+    }
+    return e;
+}
+
+}  // namespace
+
+cudaError_t block_forward(const kanb200_block_args& a, cudaStream_t st) {
+    switch (a.dtype) {
+        case KANB200_F32: return launch_forward<float>(a, st);
+        case KANB200_F64: return launch_forward<double>(a, st);
+        case KANB200_F16: return launch_forward<__half>(a, st);
+        default: return launch_forward<__nv_bfloat16>(a, st);
+    }
+}
+
+size_t block_backward_workspace(const kanb200_block_args& a) {
+    if (a.rows < 1) return 0;
+    BackwardSlabs slabs;
+    return lay_out_slabs(a, split_rows(a), nullptr, slabs);
+}
+
+cudaError_t block_backward(const kanb200_block_args& a, void* ws, size_t ws_bytes, cudaStream_t st) {
+    if (block_backward_workspace(a) > ws_bytes) return cudaErrorMemoryAllocation;
+    switch (a.dtype) {
+        case KANB200_F32: return launch_backward<float>(a, ws, st);
+        case KANB200_F64: return launch_backward<double>(a, ws, st);
+        case KANB200_F16: return launch_backward<__half>(a, ws, st);
+        default: return launch_backward<__nv_bfloat16>(a, ws, st);
+    }
+}
+
+}  // namespace kanb200

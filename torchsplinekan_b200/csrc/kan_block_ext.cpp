@@ -1,0 +1,687 @@
+// PyTorch operators around a KAN layer: the norm in front of it, the gated residual connection behind it, and 8-bit
+// checkpoints (kanb200_block_forward / _backward, kanb200_pack_activation / _unpack_activation).
+//
+// As in kan_torch_ext.cpp everything numerical of the native path happens behind the C ABI; this file validates,
+// allocates outputs and scratch from the caching allocator (per call, so that calls on several streams and captured
+// graphs share nothing), passes raw pointers and the current stream, and keeps the autograd bookkeeping.  The
+// composite formulas serve CPU tensors and backward passes that are themselves recorded (create_graph=True).
+#include <ATen/TensorUtils.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "kan_ext_util.h"
+
+namespace kan_ext {
+namespace {
+
+namespace py = pybind11;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int stream_code(const Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return KANB200_F32;
+        case at::kDouble: return KANB200_F64;
+        case at::kHalf: return KANB200_F16;
+        case at::kBFloat16: return KANB200_BF16;
+        default:
+            TORCH_CHECK(false, what, ": x must be float32, float64, float16 or bfloat16, got ", t.scalar_type());
+    }
+}
+at::ScalarType branch_type(const Tensor& x) { return x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
+
+// A tensor as rows with one stride: its own memory where the layout allows, a contiguous copy otherwise.
+struct Rows {
+    Tensor keep;
+    int64_t stride = 0;
+    const void* ptr() const { return keep.defined() ? keep.data_ptr() : nullptr; }
+};
+Rows as_rows(const Tensor& t, int64_t rows, int64_t width) {
+    if (!t.defined()) return {};
+    const int64_t shape[2] = {rows, width};
+    const auto strides = at::detail::computeStride(t.sizes(), t.strides(), at::IntArrayRef(shape, 2));
+    if (strides && ((*strides)[1] == 1 || width == 1) && ((*strides)[0] >= 0)) return {t, (*strides)[0]};
+    return {t.contiguous(), width};
+}
+
+void check_vector(const Tensor& t, const char* what, const char* name, int64_t width, at::ScalarType type,
+                  const Tensor& x) {
+    if (!t.defined()) return;
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == width, what, ": ", name, " must have shape [", width, "], got ", t.sizes());
+    TORCH_CHECK(t.scalar_type() == type, what, ": ", name, " must be ", type, " next to ", x.scalar_type(), " x, got ",
+                t.scalar_type());
+    TORCH_CHECK(t.device() == x.device(), what, ": ", name, " must be on x's device");
+}
+
+void check_settings(const char* what, double eps, int64_t checkpoint) {
+    TORCH_CHECK(eps > 0.0 && std::isfinite(eps), what, ": eps must be positive, got ", eps);
+    TORCH_CHECK(checkpoint >= KANB200_PACK_NONE && checkpoint <= KANB200_PACK_E4M3, what, ": unknown checkpoint format");
+}
+
+int64_t row_count(const Tensor& x) {
+    int64_t n = 1;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) n *= x.size(d);
+    return n;
+}
+
+Packed new_codes(int64_t rows, int64_t width, int format, const Tensor& like, at::ScalarType scale_type) {
+    const int64_t groups = (width + KANB200_PACK_GROUP - 1) / KANB200_PACK_GROUP;
+    return {at::empty({rows, width}, like.options().dtype(format == KANB200_PACK_INT8 ? at::kChar : at::kFloat8_e4m3fn)),
+            at::empty({rows, groups}, like.options().dtype(scale_type))};
+}
+
+void run_backward(kanb200_block_args& a, const Tensor& like, cudaStream_t st) {
+    const size_t bytes = kanb200_block_backward_workspace_bytes(&a);
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    check_rc(kanb200_block_backward(&a, mptr(ws), bytes, st));
+}
+
+// ------------------------------------------------------------------------------------------------
+// composite formulas
+// ------------------------------------------------------------------------------------------------
+Tensor standardise(const Tensor& v, int64_t kind, double eps, Tensor* rstd = nullptr) {
+    const Tensor c = kind == KANB200_NORM_LAYER ? v - v.mean(-1, true) : v;
+    const Tensor r = (c.square().mean(-1, true) + eps).rsqrt();
+    if (rstd) *rstd = r;
+    return c * r;
+}
+Tensor affine(Tensor v, const Tensor& w, const Tensor& b) {
+    if (w.defined()) v = v * w;
+    if (b.defined()) v = v + b;
+    return v;
+}
+Tensor over_rows(const Tensor& t) { return t.reshape({-1, t.size(-1)}).sum(0); }
+Tensor activate(const Tensor& g, int64_t act) {
+    return act == KANB200_ACT_NONE ? g : act == KANB200_ACT_SIGMOID ? at::sigmoid(g) : at::silu(g);
+}
+Tensor activate_grad(const Tensor& g, int64_t act) {
+    if (act == KANB200_ACT_NONE) return at::ones_like(g);
+    const Tensor s = at::sigmoid(g);
+    return act == KANB200_ACT_SIGMOID ? s * (1.0 - s) : s * (1.0 + g * (1.0 - s));
+}
+// (d input, d weight, d bias) of affine(standardise(v)) for the gradient d of its value
+std::tuple<Tensor, Tensor, Tensor> norm_gradient(const Tensor& v, const Tensor& w, const Tensor& d, int64_t kind,
+                                                 double eps) {
+    Tensor rstd;
+    const Tensor vhat = standardise(v, kind, eps, &rstd), u = w.defined() ? d * w : d;
+    Tensor inner = u - vhat * (u * vhat).mean(-1, true);
+    if (kind == KANB200_NORM_LAYER) inner = inner - u.mean(-1, true);
+    return std::make_tuple(rstd * inner, over_rows(d * vhat), over_rows(d));
+}
+
+Tensor norm_composite(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind, double eps) {
+    return affine(standardise(x.to(branch_type(x)), kind, eps), w, b);
+}
+
+// ------------------------------------------------------------------------------------------------
+// h = norm(x)
+// ------------------------------------------------------------------------------------------------
+void check_norm(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind, double eps, int64_t checkpoint) {
+    const char* what = "block_norm";
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must have at least one column, got ", x.sizes());
+    stream_code(x, what);
+    TORCH_CHECK(kind == KANB200_NORM_RMS || kind == KANB200_NORM_LAYER, what, ": unknown norm");
+    check_settings(what, eps, checkpoint);
+    check_vector(w, what, "weight", x.size(-1), branch_type(x), x);
+    check_vector(b, what, "bias", x.size(-1), branch_type(x), x);
+}
+
+struct NormSaved {
+    Tensor stats;
+    Packed packed;
+};
+
+Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind, double eps, int64_t checkpoint,
+                    NormSaved* saved) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+    const at::ScalarType type = branch_type(x);
+    Tensor h = at::empty(x.sizes(), x.options().dtype(type));
+    kanb200_block_args a{};
+    a.dtype = stream_code(x, "block_norm");
+    a.rows = row_count(x);
+    a.width = x.size(-1);
+    a.next_norm = (int)kind;
+    a.eps = eps;
+    if (saved) {
+        saved->stats = at::empty({a.rows, 2}, h.options());
+        a.next_stats = mptr(saved->stats);
+        if (checkpoint != KANB200_PACK_NONE) {
+            saved->packed = new_codes(a.rows, a.width, (int)checkpoint, x, type);
+            a.checkpoint = (int)checkpoint;
+            a.x_codes = mptr(saved->packed.codes);
+            a.x_scales = mptr(saved->packed.scales);
+        }
+    }
+    const Rows xr = as_rows(x, a.rows, a.width);
+    const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+    a.x = xr.ptr();
+    a.x_stride = xr.stride;
+    a.next_weight = cptr(wc);
+    a.next_bias = cptr(bc);
+    a.h = h.data_ptr();
+    check_rc(kanb200_block_forward(&a, st));
+    return h;
+}
+
+bool wants_grad(std::initializer_list<Tensor> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor& t : ts)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+
+// The autograd node's inputs must be defined tensors: an absent one is an empty tensor there.
+const Tensor& or_absent(const Tensor& t) {
+    static const Tensor& absent = *new Tensor(at::empty({0}));
+    return t.defined() ? t : absent;
+}
+Tensor present(const Tensor& t) { return has(t) ? t : Tensor(); }
+
+Tensor or_undefined(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+
+struct BlockNorm : public torch::autograd::Function<BlockNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind,
+                          double eps, int64_t checkpoint) {
+        NormSaved s;
+        const Tensor weight = present(w);
+        Tensor h = norm_forward(x, weight, present(b), kind, eps, checkpoint, &s);
+        ctx->saved_data["kind"] = kind;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["checkpoint"] = checkpoint;
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
+        ctx->save_for_backward({checkpoint != KANB200_PACK_NONE ? Tensor() : x, weight, s.stats, s.packed.codes, s.packed.scales});
+        return h;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &stats = saved[2], &codes = saved[3], &scales = saved[4];
+        const int64_t kind = ctx->saved_data["kind"].toInt(), checkpoint = ctx->saved_data["checkpoint"].toInt();
+        const double eps = ctx->saved_data["eps"].toDouble();
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+        Tensor dx, dw, db;
+        if (at::GradMode::is_enabled()) {
+            TORCH_CHECK(checkpoint == KANB200_PACK_NONE,
+                        "block_norm: create_graph=True needs the input itself, not its 8-bit checkpoint");
+            std::tie(dx, dw, db) = norm_gradient(x.to(branch_type(x)), w, grads[0], kind, eps);
+            return {dx.to(x.scalar_type()), dw, db, Tensor(), Tensor(), Tensor()};
+        }
+        c10::cuda::CUDAGuard guard(stats.device());
+        const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+        kanb200_block_args a{};
+        a.width = shape.back();
+        a.rows = stats.size(0);
+        const Rows xr = as_rows(x, a.rows, a.width), dr = as_rows(grads[0], a.rows, a.width);
+        if (ctx->needs_input_grad(0)) dx = at::empty(shape, stats.options().dtype(type));
+        if (ctx->needs_input_grad(1)) dw = at::empty({a.width}, stats.options());
+        if (ctx->needs_input_grad(2)) db = at::empty({a.width}, stats.options());
+        a.dtype = type == at::kFloat ? KANB200_F32 : type == at::kDouble ? KANB200_F64
+                  : type == at::kHalf ? KANB200_F16 : KANB200_BF16;
+        a.next_norm = (int)kind;
+        a.checkpoint = (int)checkpoint;
+        a.eps = eps;
+        a.x = xr.ptr();
+        a.x_stride = xr.stride;
+        const Tensor wc = w.defined() ? w.contiguous() : w;
+        a.next_weight = cptr(wc);
+        a.next_stats = const_cast<void*>(cptr(stats));
+        a.x_codes = const_cast<void*>(cptr(codes));
+        a.x_scales = const_cast<void*>(cptr(scales));
+        a.dh = dr.ptr();
+        a.dh_stride = dr.stride;
+        a.dx = mptr(dx);
+        a.dnext_weight = mptr(dw);
+        a.dnext_bias = mptr(db);
+        run_backward(a, stats, st);
+        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor block_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, int64_t kind,
+                  double eps, int64_t checkpoint) {
+    const Tensor w = or_undefined(weight), b = or_undefined(bias);
+    check_norm(x, w, b, kind, eps, checkpoint);
+    TORCH_CHECK(x.is_cuda() || checkpoint == KANB200_PACK_NONE, "block_norm: 8-bit checkpoints need CUDA tensors");
+    if (!x.is_cuda() || x.numel() == 0) return norm_composite(x, w, b, kind, eps);
+    if (!wants_grad({x, w, b})) return norm_forward(x, w, b, kind, eps, checkpoint, nullptr);
+    return BlockNorm::apply(x, or_absent(w), or_absent(b), kind, eps, checkpoint);
+}
+
+// ------------------------------------------------------------------------------------------------
+// out = x + scale act(gate) post(y),  h = next(out)
+// ------------------------------------------------------------------------------------------------
+struct Gated {
+    Tensor x, y, gate, scale, pw, pb, nw, nb;
+    bool packed = false;               // y holds [value | gate] side by side
+    int64_t act = 0, post = 0, next = 0, checkpoint = 0;
+    double eps = 0;
+    int64_t rows = 0, width = 0, gate_rows = 1;
+
+    bool gated() const { return packed || gate.defined(); }
+};
+
+void check_gated(Gated& g) {
+    const char* what = "gated_residual";
+    const Tensor &x = g.x, &y = g.y;
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must have at least one column, got ", x.sizes());
+    stream_code(x, what);
+    check_settings(what, g.eps, g.checkpoint);
+    TORCH_CHECK(g.act >= KANB200_ACT_NONE && g.act <= KANB200_ACT_SILU, what, ": unknown gate activation");
+    for (int64_t n : {g.post, g.next})
+        TORCH_CHECK(n >= KANB200_NORM_NONE && n <= KANB200_NORM_LAYER, what, ": unknown norm");
+    const at::ScalarType type = branch_type(x);
+    g.width = x.size(-1);
+    g.rows = row_count(x);
+    auto shape = x.sizes().vec();
+    if (g.packed) shape.back() *= 2;
+    TORCH_CHECK(y.sizes() == at::IntArrayRef(shape), what, ": y must have shape ", at::IntArrayRef(shape),
+                g.packed ? " (value and gate side by side)" : "", ", got ", y.sizes());
+    TORCH_CHECK(y.scalar_type() == type, what, ": y must be ", type, " next to ", x.scalar_type(), " x, got ",
+                y.scalar_type());
+    TORCH_CHECK(y.device() == x.device(), what, ": y must be on x's device");
+    TORCH_CHECK(g.gated() || g.act == KANB200_ACT_NONE, what, ": a gate activation needs a gate");
+    if (g.gate.defined()) {
+        const Tensor& t = g.gate;
+        TORCH_CHECK(t.scalar_type() == type, what, ": gate must be ", type, " next to ", x.scalar_type(), " x, got ",
+                    t.scalar_type());
+        TORCH_CHECK(t.device() == x.device(), what, ": gate must be on x's device");
+        // a gate per row, or one for all rows of the trailing dimensions in which it has size 1
+        bool ok = t.dim() >= 1 && t.size(-1) == g.width && (t.dim() == x.dim() || t.dim() == 1);
+        int64_t own = 1;
+        if (ok && t.dim() == x.dim()) {
+            int64_t d = 0;
+            while (d + 1 < x.dim() && t.size(d) == x.size(d)) own *= t.size(d++);
+            for (; d + 1 < x.dim(); ++d) ok = ok && t.size(d) == 1;
+        }
+        TORCH_CHECK(ok, what, ": gate must have x's shape ", x.sizes(), " or size 1 in trailing row dimensions, got ",
+                    t.sizes());
+        g.gate_rows = own > 0 ? std::max<int64_t>(g.rows / own, 1) : 1;
+    }
+    check_vector(g.scale, what, "scale", g.width, type, x);
+    check_vector(g.pw, what, "post_weight", g.width, type, x);
+    check_vector(g.pb, what, "post_bias", g.width, type, x);
+    check_vector(g.nw, what, "next_weight", g.width, type, x);
+    check_vector(g.nb, what, "next_bias", g.width, type, x);
+    TORCH_CHECK(g.post != KANB200_NORM_NONE || !(g.pw.defined() || g.pb.defined()), what,
+                ": post_weight and post_bias need post_norm");
+    TORCH_CHECK(g.next != KANB200_NORM_NONE || !(g.nw.defined() || g.nb.defined()), what,
+                ": next_weight and next_bias need next_norm");
+}
+
+// value and gate of the branch as differentiable tensors
+std::pair<Tensor, Tensor> halves(const Gated& g) {
+    if (!g.packed) return {g.y, g.gate};
+    return {g.y.narrow(-1, 0, g.width), g.y.narrow(-1, g.width, g.width)};
+}
+
+variable_list gated_composite(const Gated& g) {
+    const auto [y, gate] = halves(g);
+    Tensor t = affine(g.post != KANB200_NORM_NONE ? standardise(y, g.post, g.eps) : y, g.pw, g.pb);
+    if (gate.defined()) t = t * activate(gate, g.act);
+    if (g.scale.defined()) t = t * g.scale;
+    const Tensor out = (g.x.to(branch_type(g.x)) + t).to(g.x.scalar_type());
+    if (g.next == KANB200_NORM_NONE) return {out};
+    return {out, norm_composite(out, g.nw, g.nb, g.next, g.eps)};
+}
+
+struct GatedSaved {
+    Tensor post_stats, next_stats;
+    Packed y, gate, out;
+};
+
+void fill(kanb200_block_args& a, const Gated& g) {
+    a.gate_act = (int)g.act;
+    a.post_norm = (int)g.post;
+    a.next_norm = (int)g.next;
+    a.eps = g.eps;
+    a.rows = g.rows;
+    a.width = g.width;
+    a.gate_rows = g.gate_rows;
+}
+
+// y and gate as rows of the branch's memory: two tensors, or the two halves of one
+void branch_rows(const Gated& g, Rows& y, const void*& gate, int64_t& gate_stride, Rows& gate_keep) {
+    y = as_rows(g.y, g.rows, g.packed ? 2 * g.width : g.width);
+    if (g.packed) {
+        gate = static_cast<const char*>(y.ptr()) + g.width * g.y.element_size();
+        gate_stride = y.stride;
+    } else if (g.gate.defined()) {
+        gate_keep = as_rows(g.gate, g.rows / g.gate_rows, g.width);
+        gate = gate_keep.ptr();
+        gate_stride = gate_keep.stride;
+    }
+}
+
+variable_list gated_forward(const Gated& g, GatedSaved* saved) {
+    c10::cuda::CUDAGuard guard(g.x.device());
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+    const at::ScalarType type = branch_type(g.x);
+    const auto branch = g.x.options().dtype(type);
+    Tensor out = at::empty(g.x.sizes(), g.x.options()), h;
+    if (g.next != KANB200_NORM_NONE) h = at::empty(g.x.sizes(), branch);
+    kanb200_block_args a{};
+    fill(a, g);
+    a.dtype = stream_code(g.x, "gated_residual");
+    if (saved) {
+        if (g.post != KANB200_NORM_NONE) saved->post_stats = at::empty({g.rows, 2}, branch);
+        if (h.defined()) saved->next_stats = at::empty({g.rows, 2}, branch);
+        a.post_stats = mptr(saved->post_stats);
+        a.next_stats = mptr(saved->next_stats);
+        if (g.checkpoint != KANB200_PACK_NONE) {
+            a.checkpoint = (int)g.checkpoint;
+            saved->y = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
+            a.y_codes = mptr(saved->y.codes);
+            a.y_scales = mptr(saved->y.scales);
+            if (g.gated() && g.gate_rows == 1) {
+                saved->gate = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
+                a.gate_codes = mptr(saved->gate.codes);
+                a.gate_scales = mptr(saved->gate.scales);
+            }
+            if (h.defined()) {
+                saved->out = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
+                a.x_codes = mptr(saved->out.codes);
+                a.x_scales = mptr(saved->out.scales);
+            }
+        }
+    }
+    const Rows xr = as_rows(g.x, g.rows, g.width);
+    Rows yr, gr;
+    branch_rows(g, yr, a.gate, a.gate_stride, gr);
+    const auto vec = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
+    const Tensor scale = vec(g.scale), pw = vec(g.pw), pb = vec(g.pb), nw = vec(g.nw), nb = vec(g.nb);
+    a.x = xr.ptr();
+    a.x_stride = xr.stride;
+    a.y = yr.ptr();
+    a.y_stride = yr.stride;
+    a.scale = cptr(scale);
+    a.post_weight = cptr(pw);
+    a.post_bias = cptr(pb);
+    a.next_weight = cptr(nw);
+    a.next_bias = cptr(nb);
+    a.out = out.data_ptr();
+    a.h = mptr(h);
+    check_rc(kanb200_block_forward(&a, st));
+    if (h.defined()) return {out, h};
+    return {out};
+}
+
+// needs_input_grad / result slots
+enum { kX, kY, kGate, kScale, kPostWeight, kPostBias, kNextWeight, kNextBias, kGatedInputs };
+
+struct GatedResidual : public torch::autograd::Function<GatedResidual> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& y, const Tensor& gate,
+                                 const Tensor& scale, const Tensor& pw, const Tensor& pb, const Tensor& nw,
+                                 const Tensor& nb, bool packed, int64_t act, int64_t post, int64_t next, double eps,
+                                 int64_t checkpoint) {
+        Gated g{x, y, present(gate), present(scale), present(pw), present(pb), present(nw), present(nb),
+                packed, act, post, next, checkpoint, eps};
+        check_gated(g);
+        GatedSaved s;
+        variable_list outs = gated_forward(g, &s);
+        ctx->set_materialize_grads(false);
+        auto& d = ctx->saved_data;
+        d["packed"] = packed;
+        d["act"] = act;
+        d["post"] = post;
+        d["next"] = next;
+        d["eps"] = eps;
+        d["checkpoint"] = checkpoint;
+        d["gate_rows"] = g.gate_rows;
+        d["shape"] = x.sizes().vec();
+        d["dtype"] = (int64_t)x.scalar_type();
+        d["gate_shape"] = gate.sizes().vec();
+        const bool codes = checkpoint != KANB200_PACK_NONE;
+        const bool keep_gate = !codes || g.gate_rows > 1;
+        ctx->save_for_backward({next != KANB200_NORM_NONE && !codes ? outs[0] : Tensor(), codes ? Tensor() : y,
+                                keep_gate ? g.gate : Tensor(), g.scale, g.pw, g.pb, g.nw, s.post_stats, s.next_stats,
+                                s.out.codes, s.out.scales, s.y.codes, s.y.scales, s.gate.codes, s.gate.scales});
+        return outs;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->get_saved_variables();
+        auto& d = ctx->saved_data;
+        Gated g;
+        g.packed = d["packed"].toBool();
+        g.act = d["act"].toInt();
+        g.post = d["post"].toInt();
+        g.next = d["next"].toInt();
+        g.eps = d["eps"].toDouble();
+        g.checkpoint = d["checkpoint"].toInt();
+        g.gate_rows = d["gate_rows"].toInt();
+        const auto shape = d["shape"].toIntVector(), gate_shape = d["gate_shape"].toIntVector();
+        const auto type = (at::ScalarType)d["dtype"].toInt();
+        g.width = shape.back();
+        g.rows = 1;
+        for (size_t i = 0; i + 1 < shape.size(); ++i) g.rows *= shape[i];
+        g.y = v[1];
+        g.gate = v[2];
+        g.scale = v[3];
+        g.pw = v[4];
+        g.pb = v[5];
+        g.nw = v[6];
+        const Tensor dout = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
+        variable_list result(kGatedInputs + 6);
+        if (!dout.defined() && !dh.defined()) return result;
+        if (at::GradMode::is_enabled()) {
+            TORCH_CHECK(g.checkpoint == KANB200_PACK_NONE,
+                        "gated_residual: create_graph=True needs the inputs themselves, not their 8-bit checkpoints");
+            composite_backward(g, v[0], dout, dh, type, result);
+            return result;
+        }
+        const Tensor& like = dout.defined() ? dout : dh;
+        c10::cuda::CUDAGuard guard(like.device());
+        const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+        const auto branch = like.options().dtype(type == at::kDouble ? at::kDouble : at::kFloat);
+        kanb200_block_args a{};
+        fill(a, g);
+        if (!dh.defined()) a.next_norm = KANB200_NORM_NONE;
+        a.dtype = type == at::kFloat ? KANB200_F32 : type == at::kDouble ? KANB200_F64
+                  : type == at::kHalf ? KANB200_F16 : KANB200_BF16;
+        a.has_branch = 1;
+        a.checkpoint = (int)g.checkpoint;
+        const auto need = [&](int i) { return ctx->needs_input_grad(i); };
+        Tensor dx, dy, dgate;
+        if (need(kX)) {
+            // without a norm behind, the stream's gradient passes through unchanged
+            if (dh.defined()) dx = at::empty(shape, like.options().dtype(type));
+            else result[kX] = dout;
+        }
+        const bool want_gate = g.packed ? need(kY) : need(kGate);
+        if (need(kY)) {
+            auto s = shape;
+            if (g.packed) s.back() *= 2;
+            dy = at::empty(s, branch);
+            a.dy_stride = s.back();
+        }
+        if (want_gate && !g.packed) dgate = at::empty(gate_shape, branch);
+        const auto vec = [&](int i) {
+            if (need(i)) result[i] = at::empty({g.width}, branch);
+            return mptr(result[i]);
+        };
+        a.dscale = vec(kScale);
+        a.dpost_weight = vec(kPostWeight);
+        a.dpost_bias = vec(kPostBias);
+        if (dh.defined()) {
+            a.dnext_weight = vec(kNextWeight);
+            a.dnext_bias = vec(kNextBias);
+        }
+        const Rows xr = as_rows(dh.defined() ? v[0] : Tensor(), g.rows, g.width), dor = as_rows(dout, g.rows, g.width),
+                   dhr = as_rows(dh, g.rows, g.width);
+        Rows yr, gr;
+        if (g.y.defined()) branch_rows(g, yr, a.gate, a.gate_stride, gr);
+        else if (g.gate.defined()) {
+            gr = as_rows(g.gate, g.rows / g.gate_rows, g.width);
+            a.gate = gr.ptr();
+            a.gate_stride = gr.stride;
+        }
+        const auto dense = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
+        const Tensor scale = dense(g.scale), pw = dense(g.pw), pb = dense(g.pb), nw = dense(g.nw);
+        a.x = xr.ptr();
+        a.x_stride = xr.stride;
+        a.y = yr.ptr();
+        a.y_stride = yr.stride;
+        a.scale = cptr(scale);
+        a.post_weight = cptr(pw);
+        a.post_bias = cptr(pb);
+        if (dh.defined()) a.next_weight = cptr(nw);
+        a.post_stats = const_cast<void*>(cptr(v[7]));
+        a.next_stats = const_cast<void*>(cptr(v[8]));
+        if (dh.defined()) {
+            a.x_codes = const_cast<void*>(cptr(v[9]));
+            a.x_scales = const_cast<void*>(cptr(v[10]));
+        }
+        a.y_codes = const_cast<void*>(cptr(v[11]));
+        a.y_scales = const_cast<void*>(cptr(v[12]));
+        a.gate_codes = const_cast<void*>(cptr(v[13]));
+        a.gate_scales = const_cast<void*>(cptr(v[14]));
+        a.dout = dor.ptr();
+        a.dout_stride = dor.stride;
+        a.dh = dhr.ptr();
+        a.dh_stride = dhr.stride;
+        a.dx = mptr(dx);
+        a.dy = mptr(dy);
+        if (want_gate && g.packed) {
+            a.dgate = has(dy) ? static_cast<char*>(dy.data_ptr()) + g.width * dy.element_size() : nullptr;
+            a.dgate_stride = 2 * g.width;
+        } else {
+            a.dgate = mptr(dgate);
+            a.dgate_stride = g.width;
+        }
+        if (a.dx || a.dy || a.dgate || a.dscale || a.dpost_weight || a.dpost_bias || a.dnext_weight || a.dnext_bias)
+            run_backward(a, like, st);
+        if (dx.defined()) result[kX] = dx;
+        result[kY] = dy;
+        result[kGate] = dgate;
+        return result;
+    }
+
+    static void composite_backward(const Gated& g, const Tensor& out, const Tensor& dout, const Tensor& dh,
+                                   at::ScalarType type, variable_list& result) {
+        const auto btype = type == at::kDouble ? at::kDouble : at::kFloat;
+        const auto [y, gate] = halves(g);
+        Tensor grad = dout.defined() ? dout.to(btype) : Tensor();
+        if (dh.defined()) {
+            Tensor through;
+            std::tie(through, result[kNextWeight], result[kNextBias]) = norm_gradient(out.to(btype), g.nw, dh, g.next, g.eps);
+            grad = grad.defined() ? grad + through : through;
+        }
+        result[kX] = grad.to(type);
+        const Tensor z = affine(g.post != KANB200_NORM_NONE ? standardise(y, g.post, g.eps) : y, g.pw, g.pb);
+        const Tensor gs = g.scale.defined() ? grad * g.scale : grad;
+        Tensor dz = gs, dgate;
+        if (gate.defined()) {
+            const Tensor act = activate(gate, g.act);
+            dz = gs * act;
+            dgate = (gs * activate_grad(gate, g.act) * z).sum_to_size(gate.sizes());
+            result[kScale] = over_rows(grad * act * z);
+        } else {
+            result[kScale] = over_rows(grad * z);
+        }
+        if (g.post != KANB200_NORM_NONE)
+            std::tie(result[kY], result[kPostWeight], result[kPostBias]) = norm_gradient(y, g.pw, dz, g.post, g.eps);
+        else
+            result[kY] = dz;
+        if (g.packed) result[kY] = at::cat({result[kY], dgate}, -1);
+        else result[kGate] = dgate;
+        if (!g.scale.defined()) result[kScale] = Tensor();
+    }
+};
+
+py::object gated_residual(const Tensor& x, const Tensor& y, const std::optional<Tensor>& gate, bool packed, int64_t act,
+                          const std::optional<Tensor>& scale, int64_t post, const std::optional<Tensor>& pw,
+                          const std::optional<Tensor>& pb, int64_t next, const std::optional<Tensor>& nw,
+                          const std::optional<Tensor>& nb, double eps, int64_t checkpoint) {
+    Gated g{x, y, or_undefined(gate), or_undefined(scale), or_undefined(pw), or_undefined(pb), or_undefined(nw),
+            or_undefined(nb), packed, act, post, next, checkpoint, eps};
+    check_gated(g);
+    TORCH_CHECK(x.is_cuda() || checkpoint == KANB200_PACK_NONE, "gated_residual: 8-bit checkpoints need CUDA tensors");
+    variable_list outs;
+    if (!x.is_cuda() || x.numel() == 0) {
+        outs = gated_composite(g);
+    } else if (!wants_grad({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb})) {
+        outs = gated_forward(g, nullptr);
+    } else {
+        outs = GatedResidual::apply(g.x, g.y, or_absent(g.gate), or_absent(g.scale), or_absent(g.pw), or_absent(g.pb),
+                                    or_absent(g.nw), or_absent(g.nb), packed, act, post, next, eps, checkpoint);
+    }
+    if (outs.size() == 1) return py::cast(outs[0]);
+    return py::make_tuple(outs[0], outs[1]);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------------------
+// 8-bit checkpoints
+// ------------------------------------------------------------------------------------------------
+Packed pack_rows(const Tensor& x, int format) {
+    const char* what = "pack_activation";
+    const int code = stream_code(x, what);
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must have at least one column, got ", x.sizes());
+    TORCH_CHECK(x.is_cuda(), what, ": x must be a CUDA tensor (this backend has no CPU kernels)");
+    c10::cuda::CUDAGuard guard(x.device());
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+    const int64_t rows = row_count(x), width = x.size(-1);
+    auto shape = x.sizes().vec();
+    Packed p = new_codes(rows, width, format, x, branch_type(x));
+    const Rows xr = as_rows(x, rows, width);
+    check_rc(kanb200_pack_activation(code, format, xr.ptr(), xr.stride, mptr(p.codes), mptr(p.scales), rows, width, st));
+    if (x.dim() != 2) {
+        p.codes = p.codes.view(shape);
+        shape.back() = p.scales.size(1);
+        p.scales = p.scales.view(shape);
+    }
+    return p;
+}
+
+Tensor unpack_rows(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+    const char* what = "unpack_activation";
+    TORCH_CHECK(codes.scalar_type() == at::kChar || codes.scalar_type() == at::kFloat8_e4m3fn, what,
+                ": codes must be int8 or float8_e4m3fn, got ", codes.scalar_type());
+    TORCH_CHECK(codes.dim() >= 1 && codes.size(-1) >= 1, what, ": codes must have at least one column, got ", codes.sizes());
+    auto shape = codes.sizes().vec();
+    shape.back() = (shape.back() + KANB200_PACK_GROUP - 1) / KANB200_PACK_GROUP;
+    TORCH_CHECK(scales.sizes() == at::IntArrayRef(shape), what, ": scales must have shape ", at::IntArrayRef(shape),
+                ", got ", scales.sizes());
+    TORCH_CHECK(dtype == at::kFloat || dtype == at::kDouble || dtype == at::kHalf || dtype == at::kBFloat16, what,
+                ": dtype must be float32, float64, float16 or bfloat16, got ", dtype);
+    const auto stype = dtype == at::kDouble ? at::kDouble : at::kFloat;
+    TORCH_CHECK(scales.scalar_type() == stype, what, ": scales of ", dtype, " values must be ", stype, ", got ",
+                scales.scalar_type());
+    TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(), what,
+                ": codes and scales must be CUDA tensors on one device");
+    c10::cuda::CUDAGuard guard(codes.device());
+    const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+    const Tensor cc = codes.contiguous(), sc = scales.contiguous();
+    Tensor x = at::empty(codes.sizes(), codes.options().dtype(dtype));
+    check_rc(kanb200_unpack_activation(stream_code(x, what),
+                                       codes.scalar_type() == at::kChar ? KANB200_PACK_INT8 : KANB200_PACK_E4M3, cptr(cc),
+                                       cptr(sc), mptr(x), row_count(codes), codes.size(-1), st));
+    return x;
+}
+
+void bind_block_operators(py::module_& m) {
+    m.attr("PACK_GROUP") = KANB200_PACK_GROUP;
+    m.def("block_norm", &block_norm, "norm(x) weight + bias, autograd-aware");
+    m.def("gated_residual", &gated_residual, "x + scale act(gate) post(y) and, with a next norm, the norm of it");
+    m.def("pack_activation",
+          [](const Tensor& x, int64_t format) {
+              Packed p = pack_rows(x, (int)format);
+              return py::make_tuple(p.codes, p.scales);
+          },
+          "(codes, scales) of an 8-bit checkpoint");
+    m.def("unpack_activation", [](const Tensor& codes, const Tensor& scales, py::object dtype) {
+              return unpack_rows(codes, scales, torch::python::detail::py_object_to_dtype(dtype));
+          },
+          "the values of an 8-bit checkpoint");
+}
+
+}  // namespace kan_ext

@@ -1,8 +1,10 @@
 // C ABI of the library (declared in include/kan_b200.h): argument validation,
 // mode resolution, workspace sizing and dispatch to the kernel launchers.
 #include "../../include/kan_b200.h"
+#include "kan_block.h"
 #include "kan_internal.h"
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -74,6 +76,77 @@ bool edge_x_bwd_uses_tc(int mode, int dtype, const LayerShape& s, bool custom_ba
     if (mode == KANB200_MODE_AUTO)
         return s.N >= 256 && s.O > 16 && s.N * s.I * (int64_t)(s.O > 128 ? s.O : 128) >= ((int64_t)1 << 23);
     return true;
+}
+
+// Arguments of the operators around a layer (kan_block.cu), before any launch.
+int check_stream_dtype(const char* what, int dtype) {
+    if (dtype != KANB200_F32 && dtype != KANB200_F64 && dtype != KANB200_F16 && dtype != KANB200_BF16)
+        return fail(KANB200_EINVAL, "%s: the stream must be float32, float64, float16 or bfloat16", what);
+    return KANB200_OK;
+}
+int check_rows(const char* what, int64_t rows, int64_t width) {
+    if (rows < 0 || width < 1 || width > ((int64_t)1 << 24))
+        return fail(KANB200_EINVAL, "%s: bad sizes rows=%lld width=%lld", what, (long long)rows, (long long)width);
+    if (rows > ((int64_t)1 << 46) / width)
+        return fail(KANB200_EINVAL, "%s: rows * width is too large", what);
+    return KANB200_OK;
+}
+int check_block(const kanb200_block_args* a, bool backward) {
+    const char* what = backward ? "block_backward" : "block_forward";
+    if (!a) return fail(KANB200_EINVAL, "%s: args must not be NULL", what);
+    int rc = check_stream_dtype(what, a->dtype);
+    if (rc == KANB200_OK) rc = check_rows(what, a->rows, a->width);
+    if (rc != KANB200_OK) return rc;
+    auto norm_ok = [](int n) { return n >= KANB200_NORM_NONE && n <= KANB200_NORM_LAYER; };
+    if (!norm_ok(a->post_norm) || !norm_ok(a->next_norm)) return fail(KANB200_EINVAL, "%s: unknown norm", what);
+    if (a->gate_act < KANB200_ACT_NONE || a->gate_act > KANB200_ACT_SILU)
+        return fail(KANB200_EINVAL, "%s: unknown gate activation %d", what, a->gate_act);
+    if (a->checkpoint < KANB200_PACK_NONE || a->checkpoint > KANB200_PACK_E4M3)
+        return fail(KANB200_EINVAL, "%s: unknown checkpoint format %d", what, a->checkpoint);
+    if (!(a->eps > 0.0) || !std::isfinite(a->eps)) return fail(KANB200_EINVAL, "%s: eps must be positive", what);
+    if (a->x_stride < 0 || a->y_stride < 0 || a->gate_stride < 0 || a->dout_stride < 0 || a->dh_stride < 0)
+        return fail(KANB200_EINVAL, "%s: row strides must not be negative", what);
+    if ((a->post_norm == KANB200_NORM_NONE && (a->post_weight || a->post_bias)) ||
+        (a->next_norm == KANB200_NORM_NONE && (a->next_weight || a->next_bias)))
+        return fail(KANB200_EINVAL, "%s: a weight or bias needs its norm", what);
+    if ((a->gate || a->gate_codes) && (a->gate_rows < 1 || a->rows % a->gate_rows != 0))
+        return fail(KANB200_EINVAL, "%s: rows=%lld is not a multiple of gate_rows=%lld", what, (long long)a->rows,
+                    (long long)a->gate_rows);
+    if (a->gate_codes && a->gate_rows != 1)
+        return fail(KANB200_EINVAL, "%s: gate codes exist for a gate per row only", what);
+    if (!a->x_codes != !a->x_scales || !a->y_codes != !a->y_scales || !a->gate_codes != !a->gate_scales)
+        return fail(KANB200_EINVAL, "%s: codes and scales come together", what);
+    if (a->checkpoint == KANB200_PACK_NONE && (a->x_codes || a->y_codes || a->gate_codes))
+        return fail(KANB200_EINVAL, "%s: codes need a checkpoint format", what);
+    if (a->rows == 0) return KANB200_OK;
+    if (!backward) {
+        if (!a->x) return fail(KANB200_EINVAL, "%s: x must not be NULL", what);
+        if (a->next_norm != KANB200_NORM_NONE && !a->h) return fail(KANB200_EINVAL, "%s: h must not be NULL", what);
+        if (a->y ? !a->out : (a->next_norm == KANB200_NORM_NONE))
+            return fail(KANB200_EINVAL, "%s: %s", what, a->y ? "out must not be NULL" : "without y a norm is needed");
+        if (!a->y && (a->gate || a->scale || a->post_norm != KANB200_NORM_NONE || a->y_codes))
+            return fail(KANB200_EINVAL, "%s: gate, scale, post norm and y codes need y", what);
+        if (a->gate_codes && !a->gate) return fail(KANB200_EINVAL, "%s: gate codes need a gate", what);
+        return KANB200_OK;
+    }
+    if (!a->dout && !a->dh) return fail(KANB200_EINVAL, "%s: dout or dh must be given", what);
+    if (a->dh && (a->next_norm == KANB200_NORM_NONE || !a->next_stats || (!a->x && !a->x_codes)))
+        return fail(KANB200_EINVAL, "%s: dh needs the norm, its statistics and its input", what);
+    if (!a->dh && (a->dnext_weight || a->dnext_bias))
+        return fail(KANB200_EINVAL, "%s: the next norm's gradients need dh", what);
+    if (!a->has_branch) {
+        if (!a->dh) return fail(KANB200_EINVAL, "%s: without a branch dh must be given", what);
+        if (a->dy || a->dgate || a->dscale || a->dpost_weight || a->dpost_bias)
+            return fail(KANB200_EINVAL, "%s: gradients of a branch that the forward did not have", what);
+        return KANB200_OK;
+    }
+    if (!a->y && !a->y_codes) return fail(KANB200_EINVAL, "%s: y or its codes must be given", what);
+    if (a->post_norm != KANB200_NORM_NONE ? !a->post_stats : (a->dpost_weight || a->dpost_bias))
+        return fail(KANB200_EINVAL, "%s: the post norm's statistics or the norm itself are missing", what);
+    if (a->dgate && !a->gate && !a->gate_codes) return fail(KANB200_EINVAL, "%s: dgate needs the gate", what);
+    if ((a->dy && a->dy_stride < a->width) || (a->dgate && a->dgate_stride < a->width))
+        return fail(KANB200_EINVAL, "%s: rows of dy or dgate overlap", what);
+    return KANB200_OK;
 }
 
 }  // namespace
@@ -704,6 +777,62 @@ KANB200_API int kanb200_allreduce_sum_f32(const void* const* peer_bases, void* m
                                           int* status, void* stream) {
     return kanb200_allreduce_sum_f32_ranges(peer_bases, multicast_base, &payload_offset, &n_floats, 1, pad_offset,
                                             rank, world, local_ranks, blocks, 512, scale, status, stream);
+}
+
+KANB200_API int kanb200_block_forward(const kanb200_block_args* args, void* stream) {
+    const int rc = check_block(args, false);
+    if (rc != KANB200_OK || args->rows == 0) return rc;
+    const cudaError_t e = block_forward(*args, (cudaStream_t)stream);
+    return e == cudaSuccess ? KANB200_OK : cuda_fail(e, "block_forward");
+}
+
+KANB200_API size_t kanb200_block_backward_workspace_bytes(const kanb200_block_args* args) {
+    return check_block(args, true) == KANB200_OK ? block_backward_workspace(*args) : 0;
+}
+
+KANB200_API int kanb200_block_backward(const kanb200_block_args* args, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+    const int rc = check_block(args, true);
+    if (rc != KANB200_OK) return rc;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (args->rows == 0) {                                   // sums over no rows
+        void* sums[] = {args->dscale, args->dpost_weight, args->dpost_bias, args->dnext_weight, args->dnext_bias};
+        for (void* p : sums) {
+            if (!p) continue;
+            const cudaError_t e = cudaMemsetAsync(p, 0, (size_t)args->width * (args->dtype == KANB200_F64 ? 8 : 4), st);
+            if (e != cudaSuccess) return cuda_fail(e, "block_backward");
+        }
+        return KANB200_OK;
+    }
+    const cudaError_t e = block_backward(*args, workspace, workspace ? workspace_bytes : 0, st);
+    return e == cudaSuccess ? KANB200_OK : cuda_fail(e, "block_backward");
+}
+
+KANB200_API int kanb200_pack_activation(int dtype, int format, const void* x, int64_t x_stride, void* codes,
+                                        void* scales, int64_t rows, int64_t width, void* stream) {
+    int rc = check_stream_dtype("pack_activation", dtype);
+    if (rc == KANB200_OK) rc = check_rows("pack_activation", rows, width);
+    if (rc != KANB200_OK) return rc;
+    if (format != KANB200_PACK_INT8 && format != KANB200_PACK_E4M3)
+        return fail(KANB200_EINVAL, "pack_activation: unknown format %d", format);
+    if (x_stride < 0) return fail(KANB200_EINVAL, "pack_activation: the row stride must not be negative");
+    if (rows == 0) return KANB200_OK;
+    if (!x || !codes || !scales) return fail(KANB200_EINVAL, "pack_activation: x, codes and scales must not be NULL");
+    const cudaError_t e = pack_activation(dtype, format, x, x_stride, codes, scales, rows, width, (cudaStream_t)stream);
+    return e == cudaSuccess ? KANB200_OK : cuda_fail(e, "pack_activation");
+}
+
+KANB200_API int kanb200_unpack_activation(int dtype, int format, const void* codes, const void* scales, void* x,
+                                          int64_t rows, int64_t width, void* stream) {
+    int rc = check_stream_dtype("unpack_activation", dtype);
+    if (rc == KANB200_OK) rc = check_rows("unpack_activation", rows, width);
+    if (rc != KANB200_OK) return rc;
+    if (format != KANB200_PACK_INT8 && format != KANB200_PACK_E4M3)
+        return fail(KANB200_EINVAL, "unpack_activation: unknown format %d", format);
+    if (rows == 0) return KANB200_OK;
+    if (!x || !codes || !scales) return fail(KANB200_EINVAL, "unpack_activation: x, codes and scales must not be NULL");
+    const cudaError_t e = unpack_activation(dtype, format, codes, scales, x, rows, width, (cudaStream_t)stream);
+    return e == cudaSuccess ? KANB200_OK : cuda_fail(e, "unpack_activation");
 }
 
 }  // extern "C"

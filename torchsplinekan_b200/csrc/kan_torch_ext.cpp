@@ -27,7 +27,7 @@
 #include <unordered_map>
 #include <vector>
 
-#include "../../include/kan_b200.h"
+#include "kan_ext_util.h"
 
 namespace {
 
@@ -37,21 +37,15 @@ namespace py = pybind11;
 // ------------------------------------------------------------------------------------------------
 // small helpers
 // ------------------------------------------------------------------------------------------------
-inline bool has(const Tensor& t) { return t.defined() && t.numel() > 0; }
-inline const void* cptr(const Tensor& t) { return has(t) ? t.data_ptr() : nullptr; }
-inline void* mptr(Tensor& t) { return has(t) ? t.data_ptr() : nullptr; }
+using kan_ext::check_rc;
+using kan_ext::cptr;
+using kan_ext::has;
+using kan_ext::mptr;
 
 inline int dtype_code(const Tensor& t) {
     if (t.scalar_type() == at::kFloat) return KANB200_F32;
     if (t.scalar_type() == at::kDouble) return KANB200_F64;
     TORCH_CHECK(false, "only FP32 and FP64 inputs are supported, got ", t.scalar_type());
-}
-
-void check_rc(int rc) {
-    if (rc == KANB200_OK) return;
-    const std::string msg = kanb200_last_error();
-    if (rc == KANB200_EINVAL) TORCH_CHECK(false, msg);
-    TORCH_CHECK(false, "kan_b200 error ", rc, ": ", msg);
 }
 
 std::atomic<int> g_mode{KANB200_MODE_AUTO};
@@ -1007,4 +1001,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("_poke_status", &poke_status, py::arg("purpose"), py::arg("code"), py::arg("as_kernel") = true);
     m.def("set_event_log", &set_event_log);
     m.def("take_event_log", &take_event_log);
+    kan_ext::bind_block_operators(m);
 }
