@@ -18,14 +18,15 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libkan_b200.so")
-SOURCES = ["kan_capi.cu", "kan_simt.cu", "kan_reg.cu", "kan_dense64.cu", "kan_tc.cu", "kan_tc_edge.cu", "kan_refit.cu", "kan_collective.cu", "kan_block.cu", "kan_pack.cu"]
+SOURCES = ["kan_capi.cu", "kan_simt.cu", "kan_reg.cu", "kan_dense64.cu", "kan_tc.cu", "kan_tc_edge.cu", "kan_refit.cu", "kan_collective.cu", "kan_block.cu",
+           "kan_block_f32.cu", "kan_block_f64.cu", "kan_block_f16.cu", "kan_block_bf16.cu", "kan_pack.cu"]
 # test-only library (operand-layout self-test); never loaded by the package
 SELFTEST_SOURCE = "kan_selftest.cu"
 SELFTEST_PATH = os.path.join(LIB_DIR, "libkan_b200_selftest.so")
 # PyTorch operator layer (TORCH_LIBRARY + pybind + autograd node), host C++ only
 EXT_SOURCES = ["kan_torch_ext.cpp", "kan_block_ext.cpp"]
 EXT_HEADERS = ["kan_ext_util.h", os.path.join("..", "..", "include", "kan_b200.h")]
-HEADERS = ["kan_block.h", "kan_block.cuh", "kan_device.cuh", "kan_dmma.cuh", "kan_internal.h", "kan_table.cuh", "kan_tc_ptx.cuh", "kan_tc_common.cuh", os.path.join("..", "..", "include", "kan_b200.h")]
+HEADERS = ["kan_block.h", "kan_block.cuh", "kan_block_plan.h", "kan_block_ring.cuh", "kan_device.cuh", "kan_dmma.cuh", "kan_internal.h", "kan_table.cuh", "kan_tc_ptx.cuh", "kan_tc_common.cuh", os.path.join("..", "..", "include", "kan_b200.h")]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=hidden"]

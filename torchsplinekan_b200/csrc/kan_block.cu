@@ -8,6 +8,7 @@
 // One pass over memory is the floor: 5 floats per element forward and 8 backward with everything on, a few dozen
 // operations each, so bandwidth bounds the large calls and latency the small ones.
 #include "kan_block.cuh"
+#include "kan_block_plan.h"
 
 #include <algorithm>
 
@@ -15,7 +16,6 @@ namespace kanb200 {
 namespace {
 
 constexpr int kLoopThreads = 256;
-constexpr int kMaxColumnSums = 5;
 
 template <typename B, int K> __device__ __forceinline__ void warp_sum(B (&v)[K]) {
 #pragma unroll
@@ -157,37 +157,21 @@ template <typename S> __global__ void __launch_bounds__(kLoopThreads) loop_forwa
     }
 }
 
-// Work of the backward: items of `chunk` consecutive rows that share a gate row, dealt to the blocks in turn.
-struct Split {
-    int64_t span;        // rows per gate row (all rows when no gate is shared)
-    int64_t chunk;       // rows per item
-    int64_t per_span;    // items per span
-    int64_t items;
-    int blocks;
-};
-
-enum { kSumScale, kSumPostWeight, kSumPostBias, kSumNextWeight, kSumNextBias };
-
-struct BackwardSlabs {
-    void* column[kMaxColumnSums];    // [blocks, width] each; NULL = not needed
-    void* gate;                      // [items, width]: per-item sums of dgate (the output itself with one item per span)
-};
-
 template <typename S>
-__global__ void __launch_bounds__(kLoopThreads) loop_backward_kernel(const kanb200_block_args a, const Split sp,
+__global__ void __launch_bounds__(kLoopThreads) loop_backward_kernel(const kanb200_block_args a, const RowSplit sp,
                                                                     const BackwardSlabs slabs) {
     using B = Br<S>;
     __shared__ B buf[64];
     const int64_t D = a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const B *scale = static_cast<const B*>(a.scale), *pw = static_cast<const B*>(a.post_weight),
             *pb = static_cast<const B*>(a.post_bias), *nw = static_cast<const B*>(a.next_weight);
-    B* sum[kMaxColumnSums];
+    B* sum[kColumnSums];
 #pragma unroll
-    for (int k = 0; k < kMaxColumnSums; ++k)
+    for (int k = 0; k < kColumnSums; ++k)
         sum[k] = slabs.column[k] ? static_cast<B*>(slabs.column[k]) + (int64_t)blockIdx.x * D : nullptr;
     for_columns(D, [&](int64_t c) {
 #pragma unroll
-        for (int k = 0; k < kMaxColumnSums; ++k)
+        for (int k = 0; k < kColumnSums; ++k)
             if (sum[k]) sum[k][c] = B(0);
     });
     const bool shared_gate = a.gate && a.gate_rows > 1;
@@ -294,7 +278,7 @@ struct SlabSum {
     int64_t dst_stride;
 };
 struct SlabSums {
-    SlabSum part[kMaxColumnSums];
+    SlabSum part[kColumnSums];
 };
 template <typename B>
 __global__ void __launch_bounds__(256) sum_slabs_kernel(const SlabSums sums, int64_t width, int64_t n, int64_t spans) {
@@ -322,18 +306,98 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 size_t branch_bytes(int dtype) { return dtype == KANB200_F64 ? 8 : 4; }
 
-Split split_rows(const kanb200_block_args& a) {
-    Split s;
-    const bool shared = a.dgate && a.gate_rows > 1;
-    s.span = shared ? a.gate_rows : a.rows;
-    s.chunk = shared ? std::min<int64_t>(a.gate_rows, std::max<int64_t>(1, a.rows / 592)) : 1;
+// Items for about `teams` workers: with a shared gate long enough that what leaves per item is little next to what its rows
+// read (a slab row per chunk rows), short enough that every worker has some.
+RowSplit split_rows(const kanb200_block_args& a, int64_t teams) {
+    RowSplit s;
+    s.shared = a.gate && a.gate_rows > 1;
+    s.span = s.shared ? a.gate_rows : a.rows;
+    s.chunk = s.shared ? (int)std::min<int64_t>({a.gate_rows, std::max<int64_t>(1, a.rows / (2 * teams)), 64}) : 1;
     s.per_span = div_up(s.span, s.chunk);
     s.items = div_up(a.rows, s.span) * s.per_span;
-    s.blocks = (int)std::min<int64_t>(s.items, 592);
     return s;
 }
 
-void column_outputs(const kanb200_block_args& a, void* (&out)[kMaxColumnSums]) {
+constexpr int kLoopBlocks = kSms * 4;
+
+// ---- the ring kernels' plan ---------------------------------------------------------------------------------------------
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Four elements at once everywhere: width and strides multiples of four, pointers aligned to four elements.
+bool four_at_once(const kanb200_block_args& a) {
+    const size_t s = 4 * (a.dtype == KANB200_F64 ? 4 : a.dtype == KANB200_F32 ? 4 : 2), b = 16;
+    for (int64_t n : {a.width, a.x_stride, a.y ? a.y_stride : 0, a.gate ? a.gate_stride : 0, a.dout ? a.dout_stride : 0,
+                      a.dh ? a.dh_stride : 0, a.dy ? a.dy_stride : 0, a.dgate ? a.dgate_stride : 0})
+        if (n % 4) return false;
+    for (const void* p : {a.x, (const void*)a.out, a.dout, (const void*)a.dx})
+        if (!aligned(p, s)) return false;
+    for (const void* p : {a.y, a.gate, (const void*)a.h, a.dh, (const void*)a.dy, (const void*)a.dgate})
+        if (!aligned(p, b)) return false;
+    for (const void* p : {a.x_codes, a.y_codes, a.gate_codes})
+        if (!aligned(p, 4)) return false;
+    return true;
+}
+
+// Largest width of the ring kernels: 8 blocks of 32 warps (float64: 16), a warp per 128 columns.
+int64_t ring_width(int dtype) { return (int64_t)8 * (dtype == KANB200_F64 ? 16 : 32) * kPackGroup; }
+
+RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
+    RingPlan p{};
+    const int B = (int)branch_bytes(a.dtype), S = a.dtype == KANB200_F64 ? 8 : a.dtype == KANB200_F32 ? 4 : 2;
+    p.vec = four_at_once(a);
+    p.lanes = a.width <= 32 ? 8 : a.width <= 64 ? 16 : 32;
+    const int all = (int)div_up(a.width, kPackGroup), most = a.dtype == KANB200_F64 ? 16 : 32;
+    p.cluster = 1;
+    while (div_up(all, p.cluster) > most) p.cluster *= 2;
+    p.warps = p.lanes == 32 ? (int)div_up(all, p.cluster) : 1;
+    p.big = p.warps > 8;
+    p.teams_per_block = p.big || p.cluster > 1 ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
+    p.threads = p.lanes == 32 ? 32 * p.warps * p.teams_per_block : 256;
+    const int T = p.threads;
+
+    // a stage of the ring
+    const auto feed = [&](int size) { return p.vec || size >= 4 ? 4 * size * T : 0; };
+    const auto kept = [&](const void* codes, int size) { return codes ? (4 + B) * T : feed(size); };
+    int at = 0;
+    const auto take = [&](bool there, int bytes) {
+        const int here = at;
+        if (there) at += bytes;
+        return here;
+    };
+    const bool branch = backward ? a.has_branch : a.y != nullptr;
+    if (backward) {
+        p.at_dout = take(a.dout, feed(S));
+        p.at_dh = take(a.dh, feed(B));
+        p.at_x = take(a.dh, kept(a.x_codes, S));
+        p.at_next_stats = take(a.dh, 2 * B * T);
+        p.at_y = take(branch, kept(a.y_codes, B));
+        p.at_gate = take(branch && (a.gate || a.gate_codes), kept(a.gate_codes, B));
+        p.at_post_stats = take(branch && a.post_norm != kNormNone, 2 * B * T);
+    } else {
+        at = feed(S) + (branch ? feed(B) : 0) + (branch && a.gate ? feed(B) : 0);
+    }
+    p.stage_bytes = std::max(at, 4 * B * T);             // the blocks' column sums meet in the ring at the end
+
+    // blocks to an SM by registers (the kernels' launch bounds), then as many stages as keep about 96 KB on their way
+    const int registers = B == 8 ? 128 : p.big || !backward ? 64 : 128;
+    int per_sm = std::max(1, 65536 / (registers * T));
+    const int room = 220 * 1024;
+    while (per_sm > 1 && (2 * p.stage_bytes + 2048) * per_sm > room) --per_sm;
+    p.stages = 2;
+    for (int n : {3, 4, 6, 8}) {
+        if ((n * p.stage_bytes + 2048) * per_sm > room || (p.stages - 1) * p.stage_bytes * per_sm >= 96 * 1024) break;
+        p.stages = n;
+    }
+    const int64_t most_teams = (int64_t)kSms * per_sm / p.cluster * p.teams_per_block;
+    static_cast<RowSplit&>(p) = split_rows(a, most_teams);
+    const int64_t groups = std::min<int64_t>(div_up(p.items, p.teams_per_block), most_teams / p.teams_per_block);
+    p.blocks = (int)groups * p.cluster;
+    p.teams = groups * p.teams_per_block;
+    return p;
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+void column_outputs(const kanb200_block_args& a, void* (&out)[kColumnSums]) {
     out[kSumScale] = a.dscale;
     out[kSumPostWeight] = a.dpost_weight;
     out[kSumPostBias] = a.dpost_bias;
@@ -341,56 +405,76 @@ void column_outputs(const kanb200_block_args& a, void* (&out)[kMaxColumnSums]) {
     out[kSumNextBias] = a.dnext_bias;
 }
 
+struct BackwardPlan {
+    bool use_ring;
+    RingPlan ring;
+    RowSplit split;
+    int slab_rows;
+    BackwardSlabs slabs;
+    size_t bytes;
+};
+
 // slabs of the column sums first, then those of a shared gate
-size_t lay_out_slabs(const kanb200_block_args& a, const Split& s, void* ws, BackwardSlabs& slabs) {
+BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
+    BackwardPlan p{};
+    p.use_ring = a.width <= ring_width(a.dtype);
+    if (p.use_ring) {
+        p.ring = plan_ring(a, true);
+        p.split = p.ring;
+        p.slab_rows = p.ring.blocks / p.ring.cluster;
+    } else {
+        p.split = split_rows(a, kLoopBlocks);
+        p.slab_rows = (int)std::min<int64_t>(p.split.items, kLoopBlocks);
+    }
     const size_t row = (size_t)a.width * branch_bytes(a.dtype);
-    void* outs[kMaxColumnSums];
-    column_outputs(a, outs);
-    size_t at = 0;
-    auto take = [&](size_t bytes) {
-        void* p = static_cast<char*>(ws) + at;
-        at += (bytes + 255) / 256 * 256;
-        return p;
+    const auto take = [&](size_t bytes) {
+        void* at = static_cast<char*>(ws) + p.bytes;
+        p.bytes += (bytes + 255) / 256 * 256;
+        return at;
     };
-    for (int k = 0; k < kMaxColumnSums; ++k)
-        slabs.column[k] = !outs[k] ? nullptr : s.blocks == 1 ? outs[k] : take(row * s.blocks);
-    slabs.gate = nullptr;
-    if (a.dgate && a.gate_rows > 1)
-        slabs.gate = s.per_span == 1 && a.dgate_stride == a.width ? a.dgate : take(row * s.items);
-    return at;
+    void* outs[kColumnSums];
+    column_outputs(a, outs);
+    for (int k = 0; k < kColumnSums; ++k)
+        p.slabs.column[k] = !outs[k] ? nullptr : p.slab_rows == 1 ? outs[k] : take(row * p.slab_rows);
+    if (a.dgate && p.split.shared)
+        p.slabs.gate = p.split.per_span == 1 && a.dgate_stride == a.width ? a.dgate : take(row * p.split.items);
+    return p;
 }
 
 template <typename S> cudaError_t launch_forward(const kanb200_block_args& a, cudaStream_t st) {
-    const int blocks = (int)std::min<int64_t>(a.rows, 148 * 8);
+    if (a.width <= ring_width(a.dtype)) return ring_forward<S>(a, plan_ring(a, false), st);
+    const int blocks = (int)std::min<int64_t>(a.rows, kLoopBlocks * 2);
     loop_forward_kernel<S><<<blocks, kLoopThreads, 0, st>>>(a);
     return cudaGetLastError();
 }
 
 template <typename S>
-cudaError_t launch_backward(const kanb200_block_args& a, void* ws, cudaStream_t st) {
+cudaError_t launch_backward(const kanb200_block_args& a, const BackwardPlan& p, cudaStream_t st) {
     using B = Br<S>;
-    const Split s = split_rows(a);
-    BackwardSlabs slabs;
-    lay_out_slabs(a, s, ws, slabs);
-    loop_backward_kernel<S><<<s.blocks, kLoopThreads, 0, st>>>(a, s, slabs);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e;
+    if (p.use_ring) {
+        e = ring_backward<S>(a, p.ring, p.slabs, st);
+    } else {
+        loop_backward_kernel<S><<<p.slab_rows, kLoopThreads, 0, st>>>(a, p.split, p.slabs);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
-    void* outs[kMaxColumnSums];
+    void* outs[kColumnSums];
     column_outputs(a, outs);
     SlabSums sums;
     int n = 0;
-    for (int k = 0; k < kMaxColumnSums; ++k)
-        if (outs[k] && slabs.column[k] != outs[k]) sums.part[n++] = {slabs.column[k], outs[k], a.width};
+    for (int k = 0; k < kColumnSums; ++k)
+        if (outs[k] && p.slabs.column[k] != outs[k]) sums.part[n++] = {p.slabs.column[k], outs[k], a.width};
     const unsigned cols = (unsigned)div_up(a.width, 32);
     if (n > 0) {
-        sum_slabs_kernel<B><<<dim3(cols, 1, n), 256, 0, st>>>(sums, a.width, s.blocks, 1);
+        sum_slabs_kernel<B><<<dim3(cols, 1, n), 256, 0, st>>>(sums, a.width, p.slab_rows, 1);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
-    if (slabs.gate && slabs.gate != a.dgate) {
-        const int64_t spans = s.items / s.per_span;
-        sums.part[0] = {slabs.gate, a.dgate, a.dgate_stride};
-        sum_slabs_kernel<B><<<dim3(cols, (unsigned)std::min<int64_t>(spans, 65535), 1), 256, 0, st>>>(sums, a.width,
-                                                                                                     s.per_span, spans);
+    if (p.slabs.gate && p.slabs.gate != a.dgate) {
+        const int64_t spans = p.split.items / p.split.per_span;
+        sums.part[0] = {p.slabs.gate, a.dgate, a.dgate_stride};
+        sum_slabs_kernel<B><<<dim3(cols, (unsigned)std::min<int64_t>(spans, 65535), 1), 256, 0, st>>>(
+            sums, a.width, p.split.per_span, spans);
         e = cudaGetLastError();
     }
     return e;
@@ -408,18 +492,17 @@ cudaError_t block_forward(const kanb200_block_args& a, cudaStream_t st) {
 }
 
 size_t block_backward_workspace(const kanb200_block_args& a) {
-    if (a.rows < 1) return 0;
-    BackwardSlabs slabs;
-    return lay_out_slabs(a, split_rows(a), nullptr, slabs);
+    return a.rows < 1 ? 0 : plan_backward(a, nullptr).bytes;
 }
 
 cudaError_t block_backward(const kanb200_block_args& a, void* ws, size_t ws_bytes, cudaStream_t st) {
-    if (block_backward_workspace(a) > ws_bytes) return cudaErrorMemoryAllocation;
+    const BackwardPlan p = plan_backward(a, ws);
+    if (p.bytes > ws_bytes) return cudaErrorMemoryAllocation;
     switch (a.dtype) {
-        case KANB200_F32: return launch_backward<float>(a, ws, st);
-        case KANB200_F64: return launch_backward<double>(a, ws, st);
-        case KANB200_F16: return launch_backward<__half>(a, ws, st);
-        default: return launch_backward<__nv_bfloat16>(a, ws, st);
+        case KANB200_F32: return launch_backward<float>(a, p, st);
+        case KANB200_F64: return launch_backward<double>(a, p, st);
+        case KANB200_F16: return launch_backward<__half>(a, p, st);
+        default: return launch_backward<__nv_bfloat16>(a, p, st);
     }
 }
 

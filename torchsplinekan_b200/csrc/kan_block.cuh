@@ -76,10 +76,13 @@ template <> struct AbsBits<double> {
 };
 // maximum over the W lanes (a power of two, aligned) that share a group
 template <int W> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-    if (W == 32) return __reduce_max_sync(0xffffffffu, v);
+    if constexpr (W == 32) {
+        return __reduce_max_sync(0xffffffffu, v);
+    } else {
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+        for (int o = W / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
 }
 template <int W> __device__ __forceinline__ unsigned long long lanes_max(unsigned long long v) {
 #pragma unroll
