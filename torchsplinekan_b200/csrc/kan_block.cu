@@ -338,33 +338,43 @@ bool four_at_once(const kanb200_block_args& a) {
     return true;
 }
 
-// Largest width of the ring kernels: 8 blocks of 32 warps (float64: 16), a warp per 128 columns.
-int64_t ring_width(int dtype) { return (int64_t)8 * (dtype == KANB200_F64 ? 16 : 32) * kPackGroup; }
+// Columns that a warp of the ring kernels covers.
+int warp_columns(const kanb200_block_args& a, bool backward) {
+    return kPackGroup * ring_chunks(backward, backward ? a.has_branch : a.y != nullptr, a.dtype == KANB200_F64);
+}
+// The ring kernels take rows of up to 8 blocks of 16 warps, and 32-bit row numbers and strides.
+bool ring_fits(const kanb200_block_args& a, bool backward) {
+    for (int64_t n : {a.rows, a.x_stride, a.y_stride, a.gate_stride, a.dout_stride, a.dh_stride, a.dy_stride, a.dgate_stride})
+        if (n >= ((int64_t)1 << 31) - 4096) return false;
+    return a.width <= (int64_t)8 * 16 * warp_columns(a, backward);
+}
 
 RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     RingPlan p{};
     const int B = (int)branch_bytes(a.dtype), S = a.dtype == KANB200_F64 ? 8 : a.dtype == KANB200_F32 ? 4 : 2;
+    const bool branch = backward ? a.has_branch : a.y != nullptr;
+    const int per_warp = warp_columns(a, backward), V = per_warp / kPackGroup;
     p.vec = four_at_once(a);
-    p.lanes = a.width <= 32 ? 8 : a.width <= 64 ? 16 : 32;
-    const int all = (int)div_up(a.width, kPackGroup), most = a.dtype == KANB200_F64 ? 16 : 32;
+    p.lanes = 4;
+    while (p.lanes < 32 && p.lanes * 4 * V < a.width) p.lanes *= 2;
+    const int all = (int)div_up(a.width, per_warp);
     p.cluster = 1;
-    while (div_up(all, p.cluster) > most) p.cluster *= 2;
+    while (div_up(all, p.cluster) > 16) p.cluster *= 2;
     p.warps = p.lanes == 32 ? (int)div_up(all, p.cluster) : 1;
-    p.big = p.warps > 8;
-    p.teams_per_block = p.big || p.cluster > 1 ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
+    p.big = p.warps > 8 || p.cluster > 1;
+    p.teams_per_block = p.big ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
     p.threads = p.lanes == 32 ? 32 * p.warps * p.teams_per_block : 256;
     const int T = p.threads;
 
     // a stage of the ring
-    const auto feed = [&](int size) { return p.vec || size >= 4 ? 4 * size * T : 0; };
-    const auto kept = [&](const void* codes, int size) { return codes ? (4 + B) * T : feed(size); };
+    const auto feed = [&](int size) { return p.vec || size >= 4 ? 4 * size * V * T : 0; };
+    const auto kept = [&](const void* codes, int size) { return codes ? (4 + B) * V * T : feed(size); };
     int at = 0;
     const auto take = [&](bool there, int bytes) {
         const int here = at;
         if (there) at += bytes;
         return here;
     };
-    const bool branch = backward ? a.has_branch : a.y != nullptr;
     if (backward) {
         p.at_dout = take(a.dout, feed(S));
         p.at_dh = take(a.dh, feed(B));
@@ -374,12 +384,12 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
         p.at_gate = take(branch && (a.gate || a.gate_codes), kept(a.gate_codes, B));
         p.at_post_stats = take(branch && a.post_norm != kNormNone, 2 * B * T);
     } else {
-        at = feed(S) + (branch ? feed(B) : 0) + (branch && a.gate ? feed(B) : 0);
+        at = feed(S) + (branch ? feed(B) : 0) + (branch && a.gate && a.gate_rows == 1 ? feed(B) : 0);
     }
     p.stage_bytes = std::max(at, 4 * B * T);             // the blocks' column sums meet in the ring at the end
 
     // blocks to an SM by registers (the kernels' launch bounds), then as many stages as keep about 96 KB on their way
-    const int registers = B == 8 ? 128 : p.big || !backward ? 64 : 128;
+    const int registers = 65536 / (ring_threads(p.big) * ring_blocks(backward, branch, p.big, B == 8));
     int per_sm = std::max(1, 65536 / (registers * T));
     const int room = 220 * 1024;
     while (per_sm > 1 && (2 * p.stage_bytes + 2048) * per_sm > room) --per_sm;
@@ -417,7 +427,7 @@ struct BackwardPlan {
 // slabs of the column sums first, then those of a shared gate
 BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
     BackwardPlan p{};
-    p.use_ring = a.width <= ring_width(a.dtype);
+    p.use_ring = ring_fits(a, true);
     if (p.use_ring) {
         p.ring = plan_ring(a, true);
         p.split = p.ring;
@@ -442,7 +452,7 @@ BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
 }
 
 template <typename S> cudaError_t launch_forward(const kanb200_block_args& a, cudaStream_t st) {
-    if (a.width <= ring_width(a.dtype)) return ring_forward<S>(a, plan_ring(a, false), st);
+    if (ring_fits(a, false)) return ring_forward<S>(a, plan_ring(a, false), st);
     const int blocks = (int)std::min<int64_t>(a.rows, kLoopBlocks * 2);
     loop_forward_kernel<S><<<blocks, kLoopThreads, 0, st>>>(a);
     return cudaGetLastError();

@@ -5,8 +5,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "kan_block.h"
 
 namespace kanb200 {
@@ -31,7 +29,7 @@ struct RowSplit {
 
 struct RingPlan : RowSplit {
     int64_t teams;                   // of the launch
-    int lanes;                       // 8, 16 or 32
+    int lanes;                       // 4, 8, 16 or 32
     int warps;                       // of a team, in one block (lanes == 32)
     int teams_per_block, cluster;
     int threads, blocks, stages, stage_bytes;
@@ -39,9 +37,13 @@ struct RingPlan : RowSplit {
     bool vec, big;
 };
 
-// Registers: 256-thread blocks may use 128 (two to an SM), larger ones 64 (float64: 128, half as many threads).
-template <typename S> constexpr int ring_max_threads(bool big) {
-    return !big ? 256 : std::is_same<S, double>::value ? 512 : 1024;
+// Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers for the sums
+// that are parameter gradients (20 V floats behind a branch, 8 V behind a norm alone).
+constexpr int ring_chunks(bool backward, bool branch, bool f64) { return backward && branch ? (f64 ? 1 : 2) : f64 ? 2 : 4; }
+// Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.
+constexpr int ring_threads(bool big) { return big ? 512 : 256; }
+constexpr int ring_blocks(bool backward, bool branch, bool big, bool f64) {
+    return big ? 1 : backward || branch || f64 ? 2 : 3;
 }
 
 template <typename S> cudaError_t ring_forward(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st);
