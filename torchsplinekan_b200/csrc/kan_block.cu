@@ -366,27 +366,20 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.threads = p.lanes == 32 ? 32 * p.warps * p.teams_per_block : 256;
     const int T = p.threads;
 
-    // a stage of the ring
-    const auto feed = [&](int size) { return p.vec || size >= 4 ? 4 * size * V * T : 0; };
-    const auto kept = [&](const void* codes, int size) { return codes ? (4 + B) * V * T : feed(size); };
-    int at = 0;
-    const auto take = [&](bool there, int bytes) {
-        const int here = at;
-        if (there) at += bytes;
-        return here;
-    };
+    // a stage of the ring: BackwardStage, or x, y and a gate per row
+    const int most = ring_threads(p.big);
+    const bool row_gate = branch && (a.gate || a.gate_codes) && !(a.gate && a.gate_rows > 1);
     if (backward) {
-        p.at_dout = take(a.dout, feed(S));
-        p.at_dh = take(a.dh, feed(B));
-        p.at_x = take(a.dh, kept(a.x_codes, S));
-        p.at_next_stats = take(a.dh, 2 * B * T);
-        p.at_y = take(branch, kept(a.y_codes, B));
-        p.at_gate = take(branch && (a.gate || a.gate_codes), kept(a.gate_codes, B));
-        p.at_post_stats = take(branch && a.post_norm != kNormNone, 2 * B * T);
+        const auto take = [&](bool there, int bytes) { p.stage_bytes += there ? bytes : 0; };
+        take(a.dh, ring_bytes(B, p.vec, V, most) + ring_kept_bytes(S, p.vec, V, most, B) + 2 * B * most);
+        take(branch, ring_kept_bytes(B, p.vec, V, most, B) + 2 * B * most);
+        take(a.dout || row_gate, ring_bytes(S, p.vec, V, most));
+        take(row_gate, ring_kept_bytes(B, p.vec, V, most, B));
     } else {
-        at = feed(S) + (branch ? feed(B) : 0) + (branch && a.gate && a.gate_rows == 1 ? feed(B) : 0);
+        p.stage_bytes = ring_bytes(S, p.vec, V, most) + (branch ? ring_bytes(B, p.vec, V, most) : 0) +
+                        (row_gate ? ring_bytes(B, p.vec, V, most) : 0);
     }
-    p.stage_bytes = std::max(at, 4 * B * T);             // the blocks' column sums meet in the ring at the end
+    p.stage_bytes = std::max(p.stage_bytes, 4 * B * most);      // the blocks' column sums meet in the ring at the end
 
     // blocks to an SM by registers (the kernels' launch bounds), then as many stages as keep about 96 KB on their way
     const int registers = 65536 / (ring_threads(p.big) * ring_blocks(backward, branch, p.big, B == 8));

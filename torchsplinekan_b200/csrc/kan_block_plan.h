@@ -33,7 +33,6 @@ struct RingPlan : RowSplit {
     int warps;                       // of a team, in one block (lanes == 32)
     int teams_per_block, cluster;
     int threads, blocks, stages, stage_bytes;
-    int at_dout, at_dh, at_x, at_next_stats, at_y, at_gate, at_post_stats;      // backward: tensors within a stage
     bool vec, big;
 };
 
@@ -45,6 +44,27 @@ constexpr int ring_threads(bool big) { return big ? 512 : 256; }
 constexpr int ring_blocks(bool backward, bool branch, bool big, bool f64) {
     return big ? 1 : backward || branch || f64 ? 2 : 3;
 }
+
+// Bytes of one tensor in a stage of the ring: elements of less than 4 bytes that cannot be copied four at a time are not
+// there.  Values that may come as codes need room for either.
+constexpr int ring_bytes(int element, bool vec, int chunks, int threads) {
+    return vec || element >= 4 ? 4 * element * chunks * threads : 0;
+}
+constexpr int ring_kept_bytes(int element, bool vec, int chunks, int threads, int branch) {
+    return ring_bytes(element, vec, chunks, threads) > (4 + branch) * chunks * threads
+               ? ring_bytes(element, vec, chunks, threads) : (4 + branch) * chunks * threads;
+}
+// A stage of the backward; what is not part of every call comes last.
+template <bool NEXT, bool BRANCH, int V, int T, bool VEC, int S, int B> struct BackwardStage {
+    static constexpr int dh = 0;
+    static constexpr int x = dh + (NEXT ? ring_bytes(B, VEC, V, T) : 0);
+    static constexpr int next_stats = x + (NEXT ? ring_kept_bytes(S, VEC, V, T, B) : 0);
+    static constexpr int y = next_stats + (NEXT ? 2 * B * T : 0);
+    static constexpr int post_stats = y + (BRANCH ? ring_kept_bytes(B, VEC, V, T, B) : 0);
+    static constexpr int dout = post_stats + (BRANCH ? 2 * B * T : 0);
+    static constexpr int gate = dout + ring_bytes(S, VEC, V, T);
+    static constexpr int end = gate + ring_kept_bytes(B, VEC, V, T, B);
+};
 
 template <typename S> cudaError_t ring_forward(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st);
 template <typename S>

@@ -42,12 +42,14 @@ __device__ __forceinline__ void copies_wait_oldest(int stages) {
     }
 }
 
-// Which columns a thread owns.  Chunk j of a warp covers the 4 LANES columns from col + j * step on; a thread has four of
-// them, side by side (VEC: rows, strides and pointers allow four elements at once) or LANES apart.
+// Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other; a thread has four of each,
+// side by side (VEC: rows, strides and pointers allow four elements at once) or LANES apart.  Distances between a thread's
+// elements are constants, so a row costs one address per tensor.
 template <int LANES, int V, bool VEC> struct Columns {
-    int col, step, width;
-    __device__ __forceinline__ int at(int j, int e) const { return col + j * step + (VEC ? e : LANES * e); }
-    __device__ __forceinline__ bool ok(int j, int e) const { return VEC ? col + j * step < width : at(j, e) < width; }
+    int col, width;
+    static __device__ __forceinline__ constexpr int apart(int j, int e) { return j * 4 * LANES + (VEC ? e : LANES * e); }
+    __device__ __forceinline__ int at(int j, int e) const { return col + apart(j, e); }
+    __device__ __forceinline__ bool ok(int j, int e) const { return at(j, VEC ? 0 : e) < width; }
 };
 
 template <typename T> struct alignas(4 * sizeof(T) > 16 ? 16 : 4 * sizeof(T)) Quad {
@@ -73,43 +75,44 @@ template <typename T> __device__ __forceinline__ void store_quad(T* p, const Qua
 }
 
 // A thread's elements of one tensor on their way from a row in memory to registers.  Types of less than 4 bytes that
-// cannot be copied four at a time have no ring slot: they are loaded where they are used.
-template <typename T, int LANES, int V, bool VEC> struct Feed {
+// cannot be copied four at a time have no ring slot: they are loaded where they are used.  T is the block's most threads:
+// a slot's pieces are arrays over T threads, so that all distances in a stage are constants too.  `row` and `slot` point to
+// the thread's own first element and place.
+template <typename E, int LANES, int V, bool VEC, int T> struct Feed {
     using Cols = Columns<LANES, V, VEC>;
-    static constexpr bool kRing = VEC || sizeof(T) >= 4;
-    static constexpr int kPiece = VEC ? (4 * sizeof(T) > 16 ? 16 : 4 * (int)sizeof(T)) : (int)sizeof(T);
-    static constexpr int kPieces = 4 * (int)sizeof(T) / kPiece;         // per chunk
-    static constexpr int kBytes = kRing ? 4 * (int)sizeof(T) * V : 0;   // per thread and stage
+    static constexpr bool kRing = VEC || sizeof(E) >= 4;
+    static constexpr int kPiece = VEC ? (4 * sizeof(E) > 16 ? 16 : 4 * (int)sizeof(E)) : (int)sizeof(E);
+    static constexpr int kPieces = 4 * (int)sizeof(E) / kPiece;             // per chunk
+    static constexpr int kBytes = kRing ? 4 * (int)sizeof(E) * V * T : 0;   // of a stage
 
-    // `slot`: this tensor's part of the stage; its pieces are arrays over the block's threads
-    static __device__ __forceinline__ void issue(uint32_t slot, const T* row, const Cols& c) {
+    static __device__ __forceinline__ void issue(uint32_t stage, const E* row, const Cols& c) {
         if constexpr (!kRing) return;
-        const uint32_t dst = slot + threadIdx.x * kPiece, step = blockDim.x * kPiece;
+        const uint32_t dst = stage + threadIdx.x * kPiece;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             if constexpr (VEC) {
                 if (c.ok(j, 0))
 #pragma unroll
                     for (int p = 0; p < kPieces; ++p)
-                        copy_async<kPiece>(dst + (j * kPieces + p) * step,
-                                           reinterpret_cast<const char*>(row + c.at(j, 0)) + p * kPiece);
+                        copy_async<kPiece>(dst + (j * kPieces + p) * T * kPiece,
+                                           reinterpret_cast<const char*>(row + Cols::apart(j, 0)) + p * kPiece);
             } else if constexpr (kRing) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (c.ok(j, e)) copy_async<kPiece>(dst + (4 * j + e) * step, row + c.at(j, e));
+                    if (c.ok(j, e)) copy_async<kPiece>(dst + (4 * j + e) * T * kPiece, row + Cols::apart(j, e));
             }
         }
     }
-    static __device__ __forceinline__ void take(const char* slot, const T* row, const Cols& c, int j, T (&v)[4]) {
+    static __device__ __forceinline__ void take(const char* stage, const E* row, const Cols& c, int j, E (&v)[4]) {
+        const char* src = stage + threadIdx.x * kPiece;
         if constexpr (VEC) {
-            Quad<T> q{};
+            Quad<E> q{};
             if (c.ok(j, 0)) {
-                const char* src = slot + (j * kPieces * blockDim.x + threadIdx.x) * kPiece;
                 if constexpr (kPieces == 2) {
-                    reinterpret_cast<float4*>(&q)[0] = *reinterpret_cast<const float4*>(src);
-                    reinterpret_cast<float4*>(&q)[1] = *reinterpret_cast<const float4*>(src + blockDim.x * kPiece);
+                    reinterpret_cast<float4*>(&q)[0] = *reinterpret_cast<const float4*>(src + (2 * j) * T * kPiece);
+                    reinterpret_cast<float4*>(&q)[1] = *reinterpret_cast<const float4*>(src + (2 * j + 1) * T * kPiece);
                 } else {
-                    q = *reinterpret_cast<const Quad<T>*>(src);
+                    q = *reinterpret_cast<const Quad<E>*>(src + j * T * kPiece);
                 }
             }
 #pragma unroll
@@ -117,15 +120,16 @@ template <typename T, int LANES, int V, bool VEC> struct Feed {
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = T{};
+                v[e] = E{};
                 if (!c.ok(j, e)) continue;
-                if constexpr (kRing) v[e] = *reinterpret_cast<const T*>(slot + ((4 * j + e) * blockDim.x + threadIdx.x) * kPiece);
-                else v[e] = row[c.at(j, e)];
+                if constexpr (kRing) v[e] = *reinterpret_cast<const E*>(src + (4 * j + e) * T * kPiece);
+                else v[e] = row[Cols::apart(j, e)];
             }
         }
     }
 };
 
+// `row`: the thread's own first element, here and below
 template <typename T, int LANES, int V, bool VEC>
 __device__ __forceinline__ void put(T* row, const Columns<LANES, V, VEC>& c, int j, const T (&v)[4]) {
     if constexpr (VEC) {
@@ -133,25 +137,38 @@ __device__ __forceinline__ void put(T* row, const Columns<LANES, V, VEC>& c, int
         Quad<T> q;
 #pragma unroll
         for (int e = 0; e < 4; ++e) q.v[e] = v[e];
-        store_quad(row + c.at(j, 0), q);
+        store_quad(row + c.apart(j, 0), q);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (c.ok(j, e)) row[c.at(j, e)] = v[e];
+            if (c.ok(j, e)) row[c.apart(j, e)] = v[e];
     }
 }
 
 // Four values of a parameter (or a shared gate row); 0 beyond the row.
 template <typename T, int LANES, int V, bool VEC>
-__device__ __forceinline__ void get(const T* p, const Columns<LANES, V, VEC>& c, int j, T (&v)[4]) {
+__device__ __forceinline__ void get(const T* row, const Columns<LANES, V, VEC>& c, int j, T (&v)[4]) {
     if constexpr (VEC) {
         Quad<T> q{};
-        if (c.ok(j, 0)) q = load_quad(p + c.at(j, 0));
+        if (c.ok(j, 0)) q = load_quad(row + c.apart(j, 0));
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = q.v[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c.ok(j, e) ? p[c.at(j, e)] : T(0);
+        for (int e = 0; e < 4; ++e) v[e] = c.ok(j, e) ? row[c.apart(j, e)] : T(0);
+    }
+}
+
+// v = (v - mean) * rstd for the row's own columns, 0 beyond them
+template <typename B, int LANES, int V, bool VEC>
+__device__ __forceinline__ void normalise(const Columns<LANES, V, VEC>& c, int j, B mean, B rstd, B (&v)[4]) {
+    if constexpr (VEC) {                                   // beyond the row v is 0 and so are both moments taken
+        const B m = c.ok(j, 0) ? mean : B(0), r = c.ok(j, 0) ? rstd : B(0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (v[e] - m) * r;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c.ok(j, e) ? (v[e] - mean) * rstd : B(0);
     }
 }
 
@@ -255,8 +272,7 @@ __device__ __forceinline__ void set_up(const RingPlan& p, int width, TeamScratch
         team.team = p.teams_per_block == 1 ? 0 : warp / p.warps;
         team.warp = warp - team.team * p.warps;
         team.lane = lane;
-        c.col = (team.rank * p.warps * V + team.warp) * kPackGroup + (VEC ? 4 * lane : lane);
-        c.step = p.warps * kPackGroup;
+        c.col = (team.rank * p.warps + team.warp) * V * kPackGroup + (VEC ? 4 * lane : lane);
         team_id = group * p.teams_per_block + team.team;
         first_of_warp = team_id;
     } else {
@@ -265,7 +281,6 @@ __device__ __forceinline__ void set_up(const RingPlan& p, int width, TeamScratch
         team.warp = 0;
         team.lane = lane & (LANES - 1);
         c.col = VEC ? 4 * team.lane : team.lane;
-        c.step = 4 * LANES;
         team_id = group * p.teams_per_block + threadIdx.x / LANES;
         first_of_warp = group * p.teams_per_block + warp * (32 / LANES);
     }
@@ -305,10 +320,12 @@ __device__ __forceinline__ void put_codes(int format, const B (&v)[V][4], const 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, bool VEC, bool BRANCH, bool BIG>
 __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, BIG, sizeof(S) == 8))
-    ring_forward_kernel(const kanb200_block_args a, const RingPlan p) {
+    ring_forward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p) {
     using B = Br<S>;
-    using FS = Feed<S, LANES, V, VEC>;
-    using FB = Feed<B, LANES, V, VEC>;
+    constexpr int T = ring_threads(BIG);
+    using FS = Feed<S, LANES, V, VEC, T>;
+    using FB = Feed<B, LANES, V, VEC, T>;
+    constexpr int at_y = FS::kBytes, at_gate = at_y + FB::kBytes;
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
@@ -316,16 +333,15 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
     uint32_t team_id, first_of_warp;
     set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c, team_id, first_of_warp);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    const int at_y = FS::kBytes * blockDim.x, at_gate = at_y + FB::kBytes * blockDim.x;
     const bool row_gate = BRANCH && a.gate && !p.shared;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const B eps = B(a.eps), per = B(1) / B(D);
 
-    const S* x = static_cast<const S*>(a.x);
-    const B *y = static_cast<const B*>(a.y), *gate = static_cast<const B*>(a.gate),
-            *scale = static_cast<const B*>(a.scale), *pw = static_cast<const B*>(a.post_weight),
-            *pb = static_cast<const B*>(a.post_bias), *nw = static_cast<const B*>(a.next_weight),
-            *nb = static_cast<const B*>(a.next_bias);
+    const S* x = static_cast<const S*>(a.x) + c.col;
+    const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col,
+            *scale = static_cast<const B*>(a.scale) + c.col, *pw = static_cast<const B*>(a.post_weight) + c.col,
+            *pb = static_cast<const B*>(a.post_bias) + c.col, *nw = static_cast<const B*>(a.next_weight) + c.col,
+            *nb = static_cast<const B*>(a.next_bias) + c.col;
 
     const auto issue = [&](const RowCursor& r, int stage) {
         if (r.active()) {
@@ -378,7 +394,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
         const bool live = now.active();
         const char* at = ring + stage * p.stage_bytes;
         const uint32_t row = now.row;
-        const uint64_t dense = (uint64_t)row * (uint32_t)D;
+        const uint64_t dense = (uint64_t)row * (uint32_t)D + (uint32_t)c.col;      // of dense tensors
         B o[V][4] = {};
         if (BRANCH) {
             B v[V][4] = {};
@@ -406,14 +422,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 B w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[j][e] = (v[j][e] - mean) * rstd;
-                if (pw) {
+                normalise<B>(c, j, mean, rstd, v[j]);
+                if (a.post_weight) {
                     get<B, LANES, V, VEC>(pw, c, j, w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[j][e] *= w[e];
                 }
-                if (pb) {
+                if (a.post_bias) {
                     get<B, LANES, V, VEC>(pb, c, j, w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[j][e] += w[e];
@@ -421,7 +436,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
                 if (p.shared)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[j][e] *= t[j][e];
-                if (scale) {
+                if (a.scale) {
                     get<B, LANES, V, VEC>(scale, c, j, w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[j][e] *= w[e];
@@ -469,14 +484,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     B w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] = (o[j][e] - mean) * rstd;
-                    if (nw) {
+                    normalise<B>(c, j, mean, rstd, o[j]);
+                    if (a.next_weight) {
                         get<B, LANES, V, VEC>(nw, c, j, w);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[j][e] *= w[e];
                     }
-                    if (nb) {
+                    if (a.next_bias) {
                         get<B, LANES, V, VEC>(nb, c, j, w);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[j][e] += w[e];
@@ -494,11 +508,14 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, bool VEC, bool BRANCH, bool NEXT, bool BIG>
 __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, BIG, sizeof(S) == 8))
-    ring_backward_kernel(const kanb200_block_args a, const RingPlan p, const BackwardSlabs slabs) {
+    ring_backward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p,
+                         const __grid_constant__ BackwardSlabs slabs) {
     using B = Br<S>;
-    using FS = Feed<S, LANES, V, VEC>;
-    using FB = Feed<B, LANES, V, VEC>;
-    using FQ = Feed<uint8_t, LANES, V, VEC>;
+    constexpr int T = ring_threads(BIG);
+    using FS = Feed<S, LANES, V, VEC, T>;
+    using FB = Feed<B, LANES, V, VEC, T>;
+    using FQ = Feed<uint8_t, LANES, V, VEC, T>;
+    using At = BackwardStage<NEXT, BRANCH, V, T, VEC, (int)sizeof(S), (int)sizeof(B)>;
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
@@ -510,37 +527,38 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
     const bool row_gate = BRANCH && (a.gate || a.gate_codes) && !p.shared;
     const B per = B(1) / B(D);
 
-    const S *x = static_cast<const S*>(a.x), *dout = static_cast<const S*>(a.dout);
-    const B *y = static_cast<const B*>(a.y), *gate = static_cast<const B*>(a.gate), *dh = static_cast<const B*>(a.dh),
-            *scale = static_cast<const B*>(a.scale), *pw = static_cast<const B*>(a.post_weight),
-            *pb = static_cast<const B*>(a.post_bias), *nw = static_cast<const B*>(a.next_weight);
+    const S *x = static_cast<const S*>(a.x) + c.col, *dout = static_cast<const S*>(a.dout) + c.col;
+    const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col,
+            *dh = static_cast<const B*>(a.dh) + c.col, *scale = static_cast<const B*>(a.scale) + c.col,
+            *pw = static_cast<const B*>(a.post_weight) + c.col, *pb = static_cast<const B*>(a.post_bias) + c.col,
+            *nw = static_cast<const B*>(a.next_weight) + c.col;
     B sum_scale[V][4] = {}, sum_pw[V][4] = {}, sum_pb[V][4] = {}, sum_nw[V][4] = {}, sum_nb[V][4] = {}, sum_gate[V][4] = {};
 
     // a tensor that may be there as codes: codes and their groups' scales, or the values themselves
     const auto issue_kept = [&](uint32_t at, const void* codes, const void* scales, auto* values, int64_t stride, uint32_t row) {
-        using T = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
+        using E = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
         if (codes) {
-            FQ::issue(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D, c);
-            const B* from = static_cast<const B*>(scales) + (uint64_t)row * (uint32_t)groups;
-            const uint32_t dst = at + blockDim.x * 4 * V + threadIdx.x * (uint32_t)sizeof(B);
+            FQ::issue(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c);
+            const B* from = static_cast<const B*>(scales) + (uint64_t)row * (uint32_t)groups + c.col / kPackGroup;
+            const uint32_t dst = at + 4 * V * T + threadIdx.x * (uint32_t)sizeof(B);
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (c.at(j, 0) < D) copy_async<sizeof(B)>(dst + j * blockDim.x * (uint32_t)sizeof(B), from + c.at(j, 0) / kPackGroup);
+                if (c.at(j, 0) < D) copy_async<sizeof(B)>(dst + j * T * (uint32_t)sizeof(B), from + j * 4 * LANES / kPackGroup);
         } else {
-            Feed<T, LANES, V, VEC>::issue(at, row_at(values, row, stride), c);
+            Feed<E, LANES, V, VEC, T>::issue(at, row_at(values, row, stride), c);
         }
     };
     const auto take_kept = [&](const char* at, const void* codes, auto* values, int64_t stride, uint32_t row, int j, B (&v)[4]) {
-        using T = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
+        using E = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
         if (codes) {
             uint8_t q[4];
-            FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D, c, j, q);
-            const B s = *reinterpret_cast<const B*>(at + blockDim.x * 4 * V + (j * blockDim.x + threadIdx.x) * sizeof(B));
+            FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c, j, q);
+            const B s = c.at(j, 0) < D ? *reinterpret_cast<const B*>(at + 4 * V * T + (j * T + threadIdx.x) * sizeof(B)) : B(0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = c.ok(j, e) ? from_code<B>(a.checkpoint, q[e], s) : B(0);
+            for (int e = 0; e < 4; ++e) v[e] = from_code<B>(a.checkpoint, q[e], s);
         } else {
-            T raw[4];
-            Feed<T, LANES, V, VEC>::take(at, row_at(values, row, stride), c, j, raw);
+            E raw[4];
+            Feed<E, LANES, V, VEC, T>::take(at, row_at(values, row, stride), c, j, raw);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = widen(raw[e]);
         }
@@ -548,18 +566,18 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
     const auto issue = [&](const RowCursor& r, int stage) {
         if (r.active()) {
             const uint32_t at = ring_at + stage * p.stage_bytes;
-            if (dout) FS::issue(at + p.at_dout, row_at(dout, r.row, a.dout_stride), c);
+            if (a.dout) FS::issue(at + At::dout, row_at(dout, r.row, a.dout_stride), c);
             if (NEXT) {
-                FB::issue(at + p.at_dh, row_at(dh, r.row, a.dh_stride), c);
-                issue_kept(at + p.at_x, a.x_codes, a.x_scales, x, a.x_stride, r.row);
-                copy_async<2 * sizeof(B)>(at + p.at_next_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
+                FB::issue(at + At::dh, row_at(dh, r.row, a.dh_stride), c);
+                issue_kept(at + At::x, a.x_codes, a.x_scales, x, a.x_stride, r.row);
+                copy_async<2 * sizeof(B)>(at + At::next_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
                                           static_cast<const B*>(a.next_stats) + 2 * (uint64_t)r.row);
             }
             if (BRANCH) {
-                issue_kept(at + p.at_y, a.y_codes, a.y_scales, y, a.y_stride, r.row);
-                if (row_gate) issue_kept(at + p.at_gate, a.gate_codes, a.gate_scales, gate, a.gate_stride, r.row);
+                issue_kept(at + At::y, a.y_codes, a.y_scales, y, a.y_stride, r.row);
+                if (row_gate) issue_kept(at + At::gate, a.gate_codes, a.gate_scales, gate, a.gate_stride, r.row);
                 if (a.post_norm != kNormNone)
-                    copy_async<2 * sizeof(B)>(at + p.at_post_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
+                    copy_async<2 * sizeof(B)>(at + At::post_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
                                               static_cast<const B*>(a.post_stats) + 2 * (uint64_t)r.row);
             }
         }
@@ -582,33 +600,33 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
         const bool live = now.active();
         const char* at = ring + stage * p.stage_bytes;
         const uint32_t row = now.row;
-        const uint64_t dense = (uint64_t)row * (uint32_t)D;
+        const uint64_t dense = (uint64_t)row * (uint32_t)D + (uint32_t)c.col;      // of dense tensors
         B g[V][4] = {};                                     // gradient of the norm's input, then of y
-        if (dout && live)
+        if (a.dout && live)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 S raw[4];
-                FS::take(at + p.at_dout, row_at(dout, row, a.dout_stride), c, j, raw);
+                FS::take(at + At::dout, row_at(dout, row, a.dout_stride), c, j, raw);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) g[j][e] = widen(raw[e]);
             }
         if (NEXT) {
             B v[V][4] = {}, d[V][4] = {}, mean = B(0), rstd = B(0), s[2] = {B(0), B(0)};
             if (live) {
-                const B* stats = reinterpret_cast<const B*>(at + p.at_next_stats + threadIdx.x * 2 * sizeof(B));
+                const B* stats = reinterpret_cast<const B*>(at + At::next_stats + threadIdx.x * 2 * sizeof(B));
                 mean = stats[0];
                 rstd = stats[1];
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    FB::take(at + p.at_dh, row_at(dh, row, a.dh_stride), c, j, d[j]);
-                    take_kept(at + p.at_x, a.x_codes, x, a.x_stride, row, j, v[j]);
+                    FB::take(at + At::dh, row_at(dh, row, a.dh_stride), c, j, d[j]);
+                    take_kept(at + At::x, a.x_codes, x, a.x_stride, row, j, v[j]);
+                    normalise<B>(c, j, mean, rstd, v[j]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[j][e] = c.ok(j, e) ? (v[j][e] - mean) * rstd : B(0);     // the normalised row
                         sum_nw[j][e] += d[j][e] * v[j][e];
                         sum_nb[j][e] += d[j][e];
                     }
-                    if (nw) {
+                    if (a.next_weight) {
                         B w[4];
                         get<B, LANES, V, VEC>(nw, c, j, w);
 #pragma unroll
@@ -637,7 +655,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
             B v[V][4] = {}, mean = B(0), rstd = B(1), s[2] = {B(0), B(0)};
             if (live) {
                 if (a.post_norm != kNormNone) {
-                    const B* stats = reinterpret_cast<const B*>(at + p.at_post_stats + threadIdx.x * 2 * sizeof(B));
+                    const B* stats = reinterpret_cast<const B*>(at + At::post_stats + threadIdx.x * 2 * sizeof(B));
                     mean = stats[0];
                     rstd = stats[1];
                 }
@@ -645,20 +663,20 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     B w[4], act[4], dact[4], z[4];
-                    take_kept(at + p.at_y, a.y_codes, y, a.y_stride, row, j, v[j]);
+                    take_kept(at + At::y, a.y_codes, y, a.y_stride, row, j, v[j]);
+                    normalise<B>(c, j, mean, rstd, v[j]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[j][e] = c.ok(j, e) ? (v[j][e] - mean) * rstd : B(0);
                         z[e] = v[j][e];
                         act[e] = B(1);
                         dact[e] = B(0);
                     }
-                    if (pw) {
+                    if (a.post_weight) {
                         get<B, LANES, V, VEC>(pw, c, j, w);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) z[e] *= w[e];
                     }
-                    if (pb) {
+                    if (a.post_bias) {
                         B b[4];
                         get<B, LANES, V, VEC>(pb, c, j, b);
 #pragma unroll
@@ -667,13 +685,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
                     if (p.shared || row_gate) {
                         B gv[4];
                         if (p.shared) get<B, LANES, V, VEC>(shared, c, j, gv);
-                        else take_kept(at + p.at_gate, a.gate_codes, gate, a.gate_stride, row, j, gv);
+                        else take_kept(at + At::gate, a.gate_codes, gate, a.gate_stride, row, j, gv);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) gate_value_grad<B>(a.gate_act, gv[e], act[e], dact[e]);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum_scale[j][e] += g[j][e] * act[e] * z[e];
-                    if (scale) {
+                    if (a.scale) {
                         B sc[4];
                         get<B, LANES, V, VEC>(scale, c, j, sc);
 #pragma unroll
@@ -690,9 +708,9 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
 #pragma unroll
                         for (int e = 0; e < 4; ++e) sum_gate[j][e] += z[e];
                     } else if (a.dgate) {
-                        put<B, LANES, V, VEC>(row_at(static_cast<B*>(a.dgate), row, a.dgate_stride), c, j, z);
+                        put<B, LANES, V, VEC>(row_at(static_cast<B*>(a.dgate) + c.col, row, a.dgate_stride), c, j, z);
                     }
-                    if (pw)
+                    if (a.post_weight)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) g[j][e] *= w[e];
 #pragma unroll
@@ -711,13 +729,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
                 if (live)
 #pragma unroll
                     for (int j = 0; j < V; ++j)
-                        put<B, LANES, V, VEC>(row_at(static_cast<B*>(a.dy), row, a.dy_stride), c, j, g[j]);
+                        put<B, LANES, V, VEC>(row_at(static_cast<B*>(a.dy) + c.col, row, a.dy_stride), c, j, g[j]);
             }
             if (slabs.gate && now.pos + 1 == p.chunk) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     if (now.item < (uint32_t)p.items)
-                        put<B, LANES, V, VEC>(static_cast<B*>(slabs.gate) + (uint64_t)now.item * (uint32_t)D, c, j, sum_gate[j]);
+                        put<B, LANES, V, VEC>(static_cast<B*>(slabs.gate) + (uint64_t)now.item * (uint32_t)D + c.col, c, j, sum_gate[j]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum_gate[j][e] = B(0);
                 }
@@ -735,7 +753,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
     const int per_team = blockDim.x / p.teams_per_block;
     const auto leave = [&](int which, B (&v)[V][4]) {
         if (!slabs.column[which]) return;
-        B* row = static_cast<B*>(slabs.column[which]) + (uint64_t)block * (uint32_t)D;
+        B* row = static_cast<B*>(slabs.column[which]) + (uint64_t)block * (uint32_t)D + c.col;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             if (p.teams_per_block > 1) {
