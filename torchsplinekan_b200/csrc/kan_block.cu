@@ -174,131 +174,151 @@ __global__ void __launch_bounds__(kLoopThreads) loop_backward_kernel(const kanb2
         for (int k = 0; k < kColumnSums; ++k)
             if (sum[k]) sum[k][c] = B(0);
     });
-    const bool shared_gate = a.gate && a.gate_rows > 1;
-    for (int64_t item = blockIdx.x; item < sp.items; item += gridDim.x) {
-        const int64_t span = item / sp.per_span, first = span * sp.span + item % sp.per_span * sp.chunk;
-        const int64_t last = min(min(first + sp.chunk, (span + 1) * sp.span), a.rows);
-        B* gate_sum = shared_gate && slabs.gate ? static_cast<B*>(slabs.gate) + item * D : nullptr;
-        for (int64_t row = first; row < last; ++row) {
-            const S* dout = a.dout ? static_cast<const S*>(a.dout) + row * a.dout_stride : nullptr;
-            const B* dh = a.dh ? static_cast<const B*>(a.dh) + row * a.dh_stride : nullptr;
-            B n_mean = B(0), n_rstd = B(0), n_flat = B(0), n_along = B(0);
-            auto nhat = [&](int64_t c) {
-                const B v = a.x_codes ? from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.x_codes)[row * D + c],
-                                                     static_cast<const B*>(a.x_scales)[row * groups + c / kPackGroup])
-                                      : widen(static_cast<const S*>(a.x)[row * a.x_stride + c]);
-                return (v - n_mean) * n_rstd;
-            };
-            if (dh) {
-                n_mean = static_cast<const B*>(a.next_stats)[2 * row];
-                n_rstd = static_cast<const B*>(a.next_stats)[2 * row + 1];
-                B s[2] = {B(0), B(0)};
-                for_columns(D, [&](int64_t c) {
-                    const B v = nw ? dh[c] * nw[c] : dh[c], xh = nhat(c);
-                    s[0] += v;
-                    s[1] += v * xh;
-                    if (sum[kSumNextWeight]) sum[kSumNextWeight][c] += dh[c] * xh;
-                    if (sum[kSumNextBias]) sum[kSumNextBias][c] += dh[c];
-                });
-                block_sum<B, 2>(s, buf);
-                n_flat = a.next_norm == kNormLayer ? s[0] / B(D) : B(0);
-                n_along = s[1] / B(D);
-            }
-            auto grad = [&](int64_t c) {
-                B g = dout ? widen(dout[c]) : B(0);
-                if (dh) g += n_rstd * ((nw ? dh[c] * nw[c] : dh[c]) - n_flat - nhat(c) * n_along);
-                return g;
-            };
-            if (a.dx) for_columns(D, [&](int64_t c) { static_cast<S*>(a.dx)[row * D + c] = narrow<S>(grad(c)); });
-            if (!a.has_branch) continue;
-            B p_mean = B(0), p_rstd = B(1);
-            if (a.post_norm != kNormNone) {
-                p_mean = static_cast<const B*>(a.post_stats)[2 * row];
-                p_rstd = static_cast<const B*>(a.post_stats)[2 * row + 1];
-            }
-            auto yhat = [&](int64_t c) {
-                const B v = a.y_codes ? from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.y_codes)[row * D + c],
-                                                     static_cast<const B*>(a.y_scales)[row * groups + c / kPackGroup])
-                                      : static_cast<const B*>(a.y)[row * a.y_stride + c];
-                return (v - p_mean) * p_rstd;
-            };
-            auto gate = [&](int64_t c, B& act, B& dact) {
-                act = B(1);
-                dact = B(0);
-                if (a.gate_codes)
-                    gate_value_grad<B>(a.gate_act,
-                                       from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.gate_codes)[row * D + c],
-                                                    static_cast<const B*>(a.gate_scales)[row * groups + c / kPackGroup]),
-                                       act, dact);
-                else if (a.gate)
-                    gate_value_grad<B>(a.gate_act,
-                                       static_cast<const B*>(a.gate)[row / a.gate_rows * a.gate_stride + c], act, dact);
-            };
+    const int64_t first = (int64_t)blockIdx.x * sp.rows_per_team;
+    const int64_t last = min(first + (int64_t)sp.rows_per_team, a.rows);
+    for (int64_t row = first; row < last; ++row) {
+        const int64_t span = sp.shared ? row / a.gate_rows : 0, span_first = span * a.gate_rows;
+        B* gate_sum = nullptr;                       // where the row's share of a shared gate's gradient adds up
+        if (slabs.gate)
+            gate_sum = first <= span_first && span_first + a.gate_rows <= last
+                           ? static_cast<B*>(a.dgate) + span * a.dgate_stride
+                           : static_cast<B*>(slabs.gate) + (blockIdx.x + span) * D;
+        const bool opens = row == first || row == span_first;
+        const S* dout = a.dout ? static_cast<const S*>(a.dout) + row * a.dout_stride : nullptr;
+        const B* dh = a.dh ? static_cast<const B*>(a.dh) + row * a.dh_stride : nullptr;
+        B n_mean = B(0), n_rstd = B(0), n_flat = B(0), n_along = B(0);
+        auto nhat = [&](int64_t c) {
+            const B v = a.x_codes ? from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.x_codes)[row * D + c],
+                                                 static_cast<const B*>(a.x_scales)[row * groups + c / kPackGroup])
+                                  : widen(static_cast<const S*>(a.x)[row * a.x_stride + c]);
+            return (v - n_mean) * n_rstd;
+        };
+        if (dh) {
+            n_mean = static_cast<const B*>(a.next_stats)[2 * row];
+            n_rstd = static_cast<const B*>(a.next_stats)[2 * row + 1];
             B s[2] = {B(0), B(0)};
             for_columns(D, [&](int64_t c) {
-                const B g = grad(c), yh = yhat(c);
-                B z = pw ? yh * pw[c] : yh, act, dact;
-                if (pb) z += pb[c];
-                gate(c, act, dact);
-                const B gs = scale ? g * scale[c] : g, dz = gs * act;
-                if (sum[kSumScale]) sum[kSumScale][c] += g * act * z;
-                if (a.dgate && !shared_gate) static_cast<B*>(a.dgate)[row * a.dgate_stride + c] = gs * dact * z;
-                if (gate_sum) gate_sum[c] = (row == first ? B(0) : gate_sum[c]) + gs * dact * z;
-                if (sum[kSumPostWeight]) sum[kSumPostWeight][c] += dz * yh;
-                if (sum[kSumPostBias]) sum[kSumPostBias][c] += dz;
-                const B u = pw ? dz * pw[c] : dz;
-                s[0] += u;
-                s[1] += u * yh;
+                const B v = nw ? dh[c] * nw[c] : dh[c], xh = nhat(c);
+                s[0] += v;
+                s[1] += v * xh;
+                if (sum[kSumNextWeight]) sum[kSumNextWeight][c] += dh[c] * xh;
+                if (sum[kSumNextBias]) sum[kSumNextBias][c] += dh[c];
             });
-            if (!a.dy) continue;
-            B p_flat = B(0), p_along = B(0);
-            if (a.post_norm != kNormNone) {
-                block_sum<B, 2>(s, buf);
-                p_flat = a.post_norm == kNormLayer ? s[0] / B(D) : B(0);
-                p_along = s[1] / B(D);
-            }
-            for_columns(D, [&](int64_t c) {
-                B act, dact;
-                gate(c, act, dact);
-                B u = grad(c) * act;
-                if (scale) u *= scale[c];
-                if (pw) u *= pw[c];
-                static_cast<B*>(a.dy)[row * a.dy_stride + c] =
-                    a.post_norm != kNormNone ? p_rstd * (u - p_flat - yhat(c) * p_along) : u;
-            });
+            block_sum<B, 2>(s, buf);
+            n_flat = a.next_norm == kNormLayer ? s[0] / B(D) : B(0);
+            n_along = s[1] / B(D);
         }
+        auto grad = [&](int64_t c) {
+            B g = dout ? widen(dout[c]) : B(0);
+            if (dh) g += n_rstd * ((nw ? dh[c] * nw[c] : dh[c]) - n_flat - nhat(c) * n_along);
+            return g;
+        };
+        if (a.dx) for_columns(D, [&](int64_t c) { static_cast<S*>(a.dx)[row * D + c] = narrow<S>(grad(c)); });
+        if (!a.has_branch) continue;
+        B p_mean = B(0), p_rstd = B(1);
+        if (a.post_norm != kNormNone) {
+            p_mean = static_cast<const B*>(a.post_stats)[2 * row];
+            p_rstd = static_cast<const B*>(a.post_stats)[2 * row + 1];
+        }
+        auto yhat = [&](int64_t c) {
+            const B v = a.y_codes ? from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.y_codes)[row * D + c],
+                                                 static_cast<const B*>(a.y_scales)[row * groups + c / kPackGroup])
+                                  : static_cast<const B*>(a.y)[row * a.y_stride + c];
+            return (v - p_mean) * p_rstd;
+        };
+        auto gate = [&](int64_t c, B& act, B& dact) {
+            act = B(1);
+            dact = B(0);
+            if (a.gate_codes)
+                gate_value_grad<B>(a.gate_act,
+                                   from_code<B>(a.checkpoint, static_cast<const uint8_t*>(a.gate_codes)[row * D + c],
+                                                static_cast<const B*>(a.gate_scales)[row * groups + c / kPackGroup]),
+                                   act, dact);
+            else if (a.gate)
+                gate_value_grad<B>(a.gate_act,
+                                   static_cast<const B*>(a.gate)[row / a.gate_rows * a.gate_stride + c], act, dact);
+        };
+        B s[2] = {B(0), B(0)};
+        for_columns(D, [&](int64_t c) {
+            const B g = grad(c), yh = yhat(c);
+            B z = pw ? yh * pw[c] : yh, act, dact;
+            if (pb) z += pb[c];
+            gate(c, act, dact);
+            const B gs = scale ? g * scale[c] : g, dz = gs * act;
+            if (sum[kSumScale]) sum[kSumScale][c] += g * act * z;
+            if (a.dgate && !sp.shared) static_cast<B*>(a.dgate)[row * a.dgate_stride + c] = gs * dact * z;
+            if (gate_sum) gate_sum[c] = (opens ? B(0) : gate_sum[c]) + gs * dact * z;
+            if (sum[kSumPostWeight]) sum[kSumPostWeight][c] += dz * yh;
+            if (sum[kSumPostBias]) sum[kSumPostBias][c] += dz;
+            const B u = pw ? dz * pw[c] : dz;
+            s[0] += u;
+            s[1] += u * yh;
+        });
+        if (!a.dy) continue;
+        B p_flat = B(0), p_along = B(0);
+        if (a.post_norm != kNormNone) {
+            block_sum<B, 2>(s, buf);
+            p_flat = a.post_norm == kNormLayer ? s[0] / B(D) : B(0);
+            p_along = s[1] / B(D);
+        }
+        for_columns(D, [&](int64_t c) {
+            B act, dact;
+            gate(c, act, dact);
+            B u = grad(c) * act;
+            if (scale) u *= scale[c];
+            if (pw) u *= pw[c];
+            static_cast<B*>(a.dy)[row * a.dy_stride + c] =
+                a.post_norm != kNormNone ? p_rstd * (u - p_flat - yhat(c) * p_along) : u;
+        });
     }
 }
 
-// dst[g][c] = sum over i < n of slab[(g n + i)][c], in that order within 8 interleaved partial sums that are then added
-// in order: the same bits on every run.  A block sums 32 columns of one g; blockIdx.y deals out the g.
-struct SlabSum {
-    const void* slab;
-    void* dst;
-    int64_t dst_stride;
-};
+// Adds slab rows in a fixed order, 16 interleaved partial sums and then those: the same bits on every run.  A block sums 32
+// columns of one result: a parameter's gradient (all slab rows), or a shared gate row's (those of the teams among which
+// its rows were divided; one that a single team has is already in place).
 struct SlabSums {
-    SlabSum part[kColumnSums];
+    const void* slab[kColumnSums];
+    void* dst[kColumnSums];
+    int parameters;
+    int64_t slab_rows;
+    const void* gate_slab;
+    void* dgate;
+    int64_t dgate_stride, gate_rows, spans, rows_per_team;
 };
-template <typename B>
-__global__ void __launch_bounds__(256) sum_slabs_kernel(const SlabSums sums, int64_t width, int64_t n, int64_t spans) {
-    __shared__ B buf[8][33];
-    const SlabSum p = sums.part[blockIdx.z];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-    for (int64_t g = blockIdx.y; g < spans; g += gridDim.y) {
-        const B* slab = static_cast<const B*>(p.slab) + g * n * width;
-        B s = B(0);
-        if (c < width)
-            for (int64_t i = warp; i < n; i += 8) s += slab[i * width + c];
+constexpr int kSumWarps = 16;
+template <typename B> __global__ void __launch_bounds__(kSumWarps * 32) sum_slabs_kernel(const SlabSums s, int width) {
+    __shared__ B buf[kSumWarps][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    const auto reduce = [&](const B* slab, int n, B* dst) {
+        B sum = B(0);
+        if (c < width) {
+            int i = warp;
+            const B* at = slab + (int64_t)i * width + c;
+            const int64_t next = (int64_t)kSumWarps * width;
+            for (; i + 3 * kSumWarps < n; i += 4 * kSumWarps, at += 4 * next) {      // four loads under way
+                const B p = at[0], q = at[next], r = at[2 * next], t = at[3 * next];
+                sum += (p + q) + (r + t);
+            }
+            for (; i < n; i += kSumWarps, at += next) sum += *at;
+        }
         __syncthreads();
-        buf[warp][lane] = s;
+        buf[warp][lane] = sum;
         __syncthreads();
         if (warp == 0 && c < width) {
 #pragma unroll
-            for (int w = 1; w < 8; ++w) s += buf[w][lane];
-            static_cast<B*>(p.dst)[g * p.dst_stride + c] = s;
+            for (int w = 1; w < kSumWarps; ++w) sum += buf[w][lane];
+            dst[c] = sum;
         }
+    };
+    if ((int)blockIdx.y < s.parameters) {
+        reduce(static_cast<const B*>(s.slab[blockIdx.y]), (int)s.slab_rows, static_cast<B*>(s.dst[blockIdx.y]));
+        return;
+    }
+    for (int64_t g = blockIdx.y - s.parameters; g < s.spans; g += gridDim.y - s.parameters) {
+        const int64_t from = g * s.gate_rows / s.rows_per_team, to = ((g + 1) * s.gate_rows - 1) / s.rows_per_team;
+        if (from != to)
+            reduce(static_cast<const B*>(s.gate_slab) + (from + g) * width, (int)(to - from + 1),
+                   static_cast<B*>(s.dgate) + g * s.dgate_stride);
     }
 }
 
@@ -306,15 +326,11 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 size_t branch_bytes(int dtype) { return dtype == KANB200_F64 ? 8 : 4; }
 
-// Items for about `teams` workers: with a shared gate long enough that what leaves per item is little next to what its rows
-// read (a slab row per chunk rows), short enough that every worker has some.
-RowSplit split_rows(const kanb200_block_args& a, int64_t teams) {
+RowSplit split_rows(const kanb200_block_args& a, int64_t most_teams) {
     RowSplit s;
     s.shared = a.gate && a.gate_rows > 1;
-    s.span = s.shared ? a.gate_rows : a.rows;
-    s.chunk = s.shared ? (int)std::min<int64_t>({a.gate_rows, std::max<int64_t>(1, a.rows / (2 * teams)), 64}) : 1;
-    s.per_span = div_up(s.span, s.chunk);
-    s.items = div_up(a.rows, s.span) * s.per_span;
+    s.rows_per_team = (uint32_t)div_up(a.rows, most_teams);
+    s.teams = div_up(a.rows, s.rows_per_team);
     return s;
 }
 
@@ -381,21 +397,18 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     }
     p.stage_bytes = std::max(p.stage_bytes, 4 * B * most);      // the blocks' column sums meet in the ring at the end
 
-    // blocks to an SM by registers (the kernels' launch bounds), then as many stages as keep about 96 KB on their way
+    // blocks to an SM by registers (the kernels' launch bounds); stages while the ring leaves L1 about half of the SM's memory
     const int registers = 65536 / (ring_threads(p.big) * ring_blocks(backward, branch, p.big, B == 8));
     int per_sm = std::max(1, 65536 / (registers * T));
-    const int room = 220 * 1024;
-    while (per_sm > 1 && (2 * p.stage_bytes + 2048) * per_sm > room) --per_sm;
+    while (per_sm > 1 && (2 * p.stage_bytes + 2048) * per_sm > 200 * 1024) --per_sm;
     p.stages = 2;
-    for (int n : {3, 4, 6, 8}) {
-        if ((n * p.stage_bytes + 2048) * per_sm > room || (p.stages - 1) * p.stage_bytes * per_sm >= 96 * 1024) break;
-        p.stages = n;
+    while (p.stages < 4 && (p.stages + 1) * p.stage_bytes * per_sm <= 100 * 1024) ++p.stages;
+    static_cast<RowSplit&>(p) = split_rows(a, (int64_t)kSms * per_sm / p.cluster * p.teams_per_block);
+    p.blocks = (int)div_up(p.teams, p.teams_per_block) * p.cluster;
+    if (!p.shared) {                     // rows in turn: over every team that is launched
+        p.teams = (int64_t)p.blocks / p.cluster * p.teams_per_block;
+        p.rows_per_team = (uint32_t)div_up(a.rows, p.teams);
     }
-    const int64_t most_teams = (int64_t)kSms * per_sm / p.cluster * p.teams_per_block;
-    static_cast<RowSplit&>(p) = split_rows(a, most_teams);
-    const int64_t groups = std::min<int64_t>(div_up(p.items, p.teams_per_block), most_teams / p.teams_per_block);
-    p.blocks = (int)groups * p.cluster;
-    p.teams = groups * p.teams_per_block;
     return p;
 }
 
@@ -427,7 +440,7 @@ BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
         p.slab_rows = p.ring.blocks / p.ring.cluster;
     } else {
         p.split = split_rows(a, kLoopBlocks);
-        p.slab_rows = (int)std::min<int64_t>(p.split.items, kLoopBlocks);
+        p.slab_rows = (int)p.split.teams;
     }
     const size_t row = (size_t)a.width * branch_bytes(a.dtype);
     const auto take = [&](size_t bytes) {
@@ -439,8 +452,7 @@ BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
     column_outputs(a, outs);
     for (int k = 0; k < kColumnSums; ++k)
         p.slabs.column[k] = !outs[k] ? nullptr : p.slab_rows == 1 ? outs[k] : take(row * p.slab_rows);
-    if (a.dgate && p.split.shared)
-        p.slabs.gate = p.split.per_span == 1 && a.dgate_stride == a.width ? a.dgate : take(row * p.split.items);
+    if (a.dgate && p.split.shared) p.slabs.gate = take(row * (p.split.teams + a.rows / a.gate_rows));
     return p;
 }
 
@@ -464,20 +476,25 @@ cudaError_t launch_backward(const kanb200_block_args& a, const BackwardPlan& p, 
     if (e != cudaSuccess) return e;
     void* outs[kColumnSums];
     column_outputs(a, outs);
-    SlabSums sums;
-    int n = 0;
+    SlabSums sums{};
     for (int k = 0; k < kColumnSums; ++k)
-        if (outs[k] && p.slabs.column[k] != outs[k]) sums.part[n++] = {p.slabs.column[k], outs[k], a.width};
-    const unsigned cols = (unsigned)div_up(a.width, 32);
-    if (n > 0) {
-        sum_slabs_kernel<B><<<dim3(cols, 1, n), 256, 0, st>>>(sums, a.width, p.slab_rows, 1);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        if (outs[k] && p.slabs.column[k] != outs[k]) {
+            sums.slab[sums.parameters] = p.slabs.column[k];
+            sums.dst[sums.parameters++] = outs[k];
+        }
+    sums.slab_rows = p.slab_rows;
+    int64_t spans = 0;
+    if (p.slabs.gate && a.rows > p.split.rows_per_team && p.split.rows_per_team % a.gate_rows != 0) {
+        sums.gate_slab = p.slabs.gate;
+        sums.dgate = a.dgate;
+        sums.dgate_stride = a.dgate_stride;
+        sums.gate_rows = a.gate_rows;
+        sums.rows_per_team = p.split.rows_per_team;
+        sums.spans = spans = a.rows / a.gate_rows;
     }
-    if (p.slabs.gate && p.slabs.gate != a.dgate) {
-        const int64_t spans = p.split.items / p.split.per_span;
-        sums.part[0] = {p.slabs.gate, a.dgate, a.dgate_stride};
-        sum_slabs_kernel<B><<<dim3(cols, (unsigned)std::min<int64_t>(spans, 65535), 1), 256, 0, st>>>(
-            sums, a.width, p.split.per_span, spans);
+    if (sums.parameters + spans > 0) {
+        const dim3 grid((unsigned)div_up(a.width, 32), (unsigned)(sums.parameters + std::min<int64_t>(spans, 4096)));
+        sum_slabs_kernel<B><<<grid, kSumWarps * 32, 0, st>>>(sums, (int)a.width);
         e = cudaGetLastError();
     }
     return e;

@@ -16,19 +16,18 @@ enum { kSumScale, kSumPostWeight, kSumPostBias, kSumNextWeight, kSumNextBias, kC
 
 struct BackwardSlabs {
     void* column[kColumnSums];       // [slab rows, width] each; NULL = not needed
-    void* gate;                      // [items, width]: per-item sums of dgate (the output itself with one item per span)
+    void* gate;                      // [teams + gate rows, width]: dgate of the part of a gate row's span that team t takes, at
+                                     // row t + (gate row); NULL = no shared gate, or dgate not needed
 };
 
-// Rows are dealt out as items of `chunk` consecutive rows.  With a shared gate an item stays within the rows of one gate
-// row (a span), so that its gate is read once and its share of dgate leaves as one slab row.
+// Teams take at most rows_per_team rows each: with a shared gate consecutive ones, otherwise every teams-th.
 struct RowSplit {
-    bool shared;
-    int64_t span, per_span, items;   // rows per gate row, items per span
-    int chunk;
+    bool shared;                     // gate_rows rows share a gate row
+    uint32_t rows_per_team;
+    int64_t teams;                   // with a shared gate: those that have rows
 };
 
 struct RingPlan : RowSplit {
-    int64_t teams;                   // of the launch
     int lanes;                       // 4, 8, 16 or 32
     int warps;                       // of a team, in one block (lanes == 32)
     int teams_per_block, cluster;
@@ -37,13 +36,12 @@ struct RingPlan : RowSplit {
 };
 
 // Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers for the sums
-// that are parameter gradients (20 V floats behind a branch, 8 V behind a norm alone).
-constexpr int ring_chunks(bool backward, bool branch, bool f64) { return backward && branch ? (f64 ? 1 : 2) : f64 ? 2 : 4; }
+// that are parameter gradients (12 to 20 V values behind a branch, 8 V at a norm).  Four chunks behind a branch spill: the
+// 8-bit gated backward of 16384 x 2048 took 278 us instead of 243.
+constexpr int ring_chunks(bool backward, bool branch, bool f64) { return (backward && branch ? 2 : 4) / (f64 ? 2 : 1); }
 // Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.
 constexpr int ring_threads(bool big) { return big ? 512 : 256; }
-constexpr int ring_blocks(bool backward, bool branch, bool big, bool f64) {
-    return big ? 1 : backward || branch || f64 ? 2 : 3;
-}
+constexpr int ring_blocks(bool backward, bool branch, bool big, bool f64) { return big ? 1 : 2; }
 
 // Bytes of one tensor in a stage of the ring: elements of less than 4 bytes that cannot be copied four at a time are not
 // there.  Values that may come as codes need room for either.

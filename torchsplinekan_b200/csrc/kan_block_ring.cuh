@@ -2,17 +2,20 @@
 // launch, and its share of the next rows is already on its way into shared memory.
 //
 //   * A team of threads owns a row at a time: 4, 8 or 16 lanes, W warps, or the warps of a cluster of up to 8 blocks.
-//     Teams take rows (or, with a shared gate, runs of rows under one gate row) in turn.
-//   * Memory -> registers goes through a ring of 2 to 8 rows in shared memory, filled by cp.async.  A thread copies
+//     Teams take rows in turn; with a shared gate a team takes consecutive rows, so that a gate row is read, and its
+//     gradient leaves, once per team (consecutive rows everywhere cost 5 to 10 % of the bandwidth: norm of 65536 x 1024
+//     forward 99 us against 91).
+//   * Memory -> registers goes through a ring of 2 to 4 rows in shared memory, filled by cp.async.  A thread copies
 //     exactly what it reads back itself, so the ring needs no barrier: only its own cp.async group to have landed.  The
 //     bytes in flight then do not depend on registers or on how many warps wait in a barrier.
 //   * The sums over rows that are the parameters' gradients stay in registers; one slab row per block leaves the kernel at
-//     its end.  Parameters are read again for every row, from L1.
+//     its end.  Parameters are read again for every row, from L1: the ring leaves room for them (with 3 rows instead of 2
+//     the gated backward of 16384 x 1024 took 206 us instead of 135, the parameters then came from L2).
 //   * Sums over a row: lanes by shuffles, warps through shared memory with a barrier of the team alone, blocks of a
 //     cluster through each other's shared memory; every thread gets the same bits.
-//   * V: what a row costs besides its elements -- its sums, barriers, waits, addresses, about 100 instructions -- is
-//     shared by 4 V elements.  With V = 1 the kernels were bound by issue slots (norm of 65536 x 1024: 232 instructions
-//     per warp and row forward, 345 backward, 76 % of the issue slots taken at 58 % of the copy bandwidth).
+//   * Issue slots bound these kernels before bandwidth does, so: what a row costs besides its elements (sums, barriers,
+//     addresses) is shared by 4 V elements; distances between a thread's elements are constants; float arithmetic works
+//     on pairs (one instruction for two elements).
 #pragma once
 #include <cooperative_groups.h>
 
@@ -33,13 +36,9 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() {
 }
 // all but the newest stages - 1 groups have landed
 __device__ __forceinline__ void copies_wait_oldest(int stages) {
-    switch (stages) {
-        case 2: copies_wait<1>(); break;
-        case 3: copies_wait<2>(); break;
-        case 4: copies_wait<3>(); break;
-        case 6: copies_wait<5>(); break;
-        default: copies_wait<7>(); break;        // 8
-    }
+    if (stages == 2) copies_wait<1>();
+    else if (stages == 3) copies_wait<2>();
+    else copies_wait<3>();
 }
 
 // Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other; a thread has four of each,
@@ -52,6 +51,7 @@ template <int LANES, int V, bool VEC> struct Columns {
     __device__ __forceinline__ bool ok(int j, int e) const { return at(j, VEC ? 0 : e) < width; }
 };
 
+// ---- four elements --------------------------------------------------------------------------------------------------
 template <typename T> struct alignas(4 * sizeof(T) > 16 ? 16 : 4 * sizeof(T)) Quad {
     T v[4];
 };
@@ -74,6 +74,145 @@ template <typename T> __device__ __forceinline__ void store_quad(T* p, const Qua
     }
 }
 
+// Four values in the branch's type; float works on pairs (sm_100's two-element FMA pipe instructions).
+template <typename B> struct alignas(16) Four {
+    B v[4];
+};
+template <typename B> __device__ __forceinline__ Four<B> four(B s) { return {{s, s, s, s}}; }
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split_pair(unsigned long long p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+#define KANB200_PAIRWISE(name, instruction)                                                                          \
+    __device__ __forceinline__ Four<float> name(const Four<float>& x, const Four<float>& y) {                        \
+        Four<float> r;                                                                                               \
+        _Pragma("unroll") for (int e = 0; e < 4; e += 2) {                                                           \
+            unsigned long long p;                                                                                    \
+            asm(instruction " %0, %1, %2;" : "=l"(p) : "l"(pair_of(x.v[e], x.v[e + 1])), "l"(pair_of(y.v[e], y.v[e + 1]))); \
+            split_pair(p, r.v[e], r.v[e + 1]);                                                                       \
+        }                                                                                                            \
+        return r;                                                                                                    \
+    }
+KANB200_PAIRWISE(operator+, "add.rn.f32x2")
+KANB200_PAIRWISE(operator*, "mul.rn.f32x2")
+#undef KANB200_PAIRWISE
+// x y + z, rounded once
+__device__ __forceinline__ Four<float> fma4(const Four<float>& x, const Four<float>& y, const Four<float>& z) {
+    Four<float> r;
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+        unsigned long long p;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;"
+            : "=l"(p)
+            : "l"(pair_of(x.v[e], x.v[e + 1])), "l"(pair_of(y.v[e], y.v[e + 1])), "l"(pair_of(z.v[e], z.v[e + 1])));
+        split_pair(p, r.v[e], r.v[e + 1]);
+    }
+    return r;
+}
+__device__ __forceinline__ Four<double> operator+(const Four<double>& x, const Four<double>& y) {
+    return {{x.v[0] + y.v[0], x.v[1] + y.v[1], x.v[2] + y.v[2], x.v[3] + y.v[3]}};
+}
+__device__ __forceinline__ Four<double> operator*(const Four<double>& x, const Four<double>& y) {
+    return {{x.v[0] * y.v[0], x.v[1] * y.v[1], x.v[2] * y.v[2], x.v[3] * y.v[3]}};
+}
+__device__ __forceinline__ Four<double> fma4(const Four<double>& x, const Four<double>& y, const Four<double>& z) {
+    return {{fma(x.v[0], y.v[0], z.v[0]), fma(x.v[1], y.v[1], z.v[1]), fma(x.v[2], y.v[2], z.v[2]), fma(x.v[3], y.v[3], z.v[3])}};
+}
+template <typename B> __device__ __forceinline__ B total(const Four<B>& x) { return (x.v[0] + x.v[2]) + (x.v[1] + x.v[3]); }
+
+template <typename S> __device__ __forceinline__ Four<Br<S>> widen4(const Quad<S>& q) {
+    return {{widen(q.v[0]), widen(q.v[1]), widen(q.v[2]), widen(q.v[3])}};
+}
+template <typename S> __device__ __forceinline__ Quad<S> narrow4(const Four<Br<S>>& x) {
+    Quad<S> q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.v[e] = narrow<S>(x.v[e]);
+    return q;
+}
+template <> __device__ __forceinline__ Quad<__nv_bfloat16> narrow4<__nv_bfloat16>(const Four<float>& x) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.v[0], x.v[1]), b = __floats2bfloat162_rn(x.v[2], x.v[3]);
+    return {{a.x, a.y, b.x, b.y}};
+}
+template <> __device__ __forceinline__ Quad<__half> narrow4<__half>(const Four<float>& x) {
+    const __half2 a = __floats2half2_rn(x.v[0], x.v[1]), b = __floats2half2_rn(x.v[2], x.v[3]);
+    return {{a.x, a.y, b.x, b.y}};
+}
+
+template <typename B> __device__ __forceinline__ Four<B> sigmoid4(const Four<B>& g) {
+    return {{gate_sigmoid(g.v[0]), gate_sigmoid(g.v[1]), gate_sigmoid(g.v[2]), gate_sigmoid(g.v[3])}};
+}
+template <typename B> __device__ __forceinline__ Four<B> gate4(int act, const Four<B>& g) {
+    if (act == kActNone) return g;
+    const Four<B> s = sigmoid4(g);
+    return act == kActSigmoid ? s : g * s;
+}
+// activation and derivative: sigmoid s, s (1 - s);  silu g s, s + g s (1 - s)
+template <typename B> __device__ __forceinline__ void gate4_grad(int act, const Four<B>& g, Four<B>& a, Four<B>& da) {
+    a = g;
+    da = four<B>(B(1));
+    if (act == kActNone) return;
+    const Four<B> s = sigmoid4(g), rest = fma4(s, four<B>(B(-1)), four<B>(B(1)));
+    a = act == kActSigmoid ? s : g * s;
+    da = act == kActSigmoid ? s * rest : fma4(a, rest, s);
+}
+
+// Codes of four elements as one word, lowest byte first.  int8 without conversions: the byte becomes the mantissa of
+// 2^23 + 128 + code, and back by adding 1.5 * 2^23, which leaves the rounded integer in the low bits.
+template <typename B> __device__ __forceinline__ Four<B> decode4(int format, uint32_t word, B scale);
+template <> __device__ __forceinline__ Four<float> decode4<float>(int format, uint32_t word, float scale) {
+    Four<float> r;
+    if (format == kPackInt8) {
+        const uint32_t w = word ^ 0x80808080u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[e] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + e));
+        r = r + four<float>(-8388736.0f);
+    } else {
+        const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word & 0xffffu), __NV_E4M3));
+        const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word >> 16), __NV_E4M3));
+        const float2 fa = __half22float2(a), fb = __half22float2(b);
+        r = {{fa.x, fa.y, fb.x, fb.y}};
+    }
+    return r * four<float>(scale);
+}
+template <> __device__ __forceinline__ Four<double> decode4<double>(int format, uint32_t word, double scale) {
+    Four<double> r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.v[e] = from_code<double>(format, word >> 8 * e & 0xffu, scale);
+    return r;
+}
+// |x / scale| is at most 127 (1 + 2^-21) by the choice of the scale, so rounding cannot leave the codes' range.  The product
+// is rounded before it is rounded to a code (the definition; the pairwise instructions above would be merged into one
+// multiply-add, which turns 63.49999952 into 63 where the float product is 63.5).
+__device__ __forceinline__ uint32_t encode4(int format, const Four<float>& x, float inv) {
+    float q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = __fmul_rn(x.v[e], inv);
+    uint32_t word;
+    if (format == kPackInt8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = __fadd_rn(q[e], 12582912.0f);
+        const uint32_t a = __byte_perm(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x0040);
+        const uint32_t b = __byte_perm(__float_as_uint(q[2]), __float_as_uint(q[3]), 0x0040);
+        word = __byte_perm(a, b, 0x5410);
+    } else {
+        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
+        word = a | b << 16;
+    }
+    return inv == 0.0f ? 0u : word;                          // a group that is not finite
+}
+__device__ __forceinline__ uint32_t encode4(int format, const Four<double>& x, double inv) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) word |= to_code(format, x.v[e], inv) << 8 * e;
+    return word;
+}
+
+// ---- rows <-> registers -----------------------------------------------------------------------------------------------
 // A thread's elements of one tensor on their way from a row in memory to registers.  Types of less than 4 bytes that
 // cannot be copied four at a time have no ring slot: they are loaded where they are used.  T is the block's most threads:
 // a slot's pieces are arrays over T threads, so that all distances in a stage are constants too.  `row` and `slot` point to
@@ -103,10 +242,10 @@ template <typename E, int LANES, int V, bool VEC, int T> struct Feed {
             }
         }
     }
-    static __device__ __forceinline__ void take(const char* stage, const E* row, const Cols& c, int j, E (&v)[4]) {
+    static __device__ __forceinline__ Quad<E> take(const char* stage, const E* row, const Cols& c, int j) {
         const char* src = stage + threadIdx.x * kPiece;
+        Quad<E> q{};
         if constexpr (VEC) {
-            Quad<E> q{};
             if (c.ok(j, 0)) {
                 if constexpr (kPieces == 2) {
                     reinterpret_cast<float4*>(&q)[0] = *reinterpret_cast<const float4*>(src + (2 * j) * T * kPiece);
@@ -115,61 +254,52 @@ template <typename E, int LANES, int V, bool VEC, int T> struct Feed {
                     q = *reinterpret_cast<const Quad<E>*>(src + j * T * kPiece);
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = q.v[e];
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = E{};
                 if (!c.ok(j, e)) continue;
-                if constexpr (kRing) v[e] = *reinterpret_cast<const E*>(src + (4 * j + e) * T * kPiece);
-                else v[e] = row[Cols::apart(j, e)];
+                if constexpr (kRing) q.v[e] = *reinterpret_cast<const E*>(src + (4 * j + e) * T * kPiece);
+                else q.v[e] = row[Cols::apart(j, e)];
             }
         }
+        return q;
     }
 };
 
 // `row`: the thread's own first element, here and below
 template <typename T, int LANES, int V, bool VEC>
-__device__ __forceinline__ void put(T* row, const Columns<LANES, V, VEC>& c, int j, const T (&v)[4]) {
+__device__ __forceinline__ void put(T* row, const Columns<LANES, V, VEC>& c, int j, const Quad<T>& q) {
     if constexpr (VEC) {
-        if (!c.ok(j, 0)) return;
-        Quad<T> q;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q.v[e] = v[e];
-        store_quad(row + c.apart(j, 0), q);
+        if (c.ok(j, 0)) store_quad(row + c.apart(j, 0), q);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (c.ok(j, e)) row[c.apart(j, e)] = v[e];
+            if (c.ok(j, e)) row[c.apart(j, e)] = q.v[e];
     }
 }
-
-// Four values of a parameter (or a shared gate row); 0 beyond the row.
-template <typename T, int LANES, int V, bool VEC>
-__device__ __forceinline__ void get(const T* row, const Columns<LANES, V, VEC>& c, int j, T (&v)[4]) {
-    if constexpr (VEC) {
-        Quad<T> q{};
-        if (c.ok(j, 0)) q = load_quad(row + c.apart(j, 0));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = q.v[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c.ok(j, e) ? row[c.apart(j, e)] : T(0);
-    }
-}
-
-// v = (v - mean) * rstd for the row's own columns, 0 beyond them
 template <typename B, int LANES, int V, bool VEC>
-__device__ __forceinline__ void normalise(const Columns<LANES, V, VEC>& c, int j, B mean, B rstd, B (&v)[4]) {
-    if constexpr (VEC) {                                   // beyond the row v is 0 and so are both moments taken
-        const B m = c.ok(j, 0) ? mean : B(0), r = c.ok(j, 0) ? rstd : B(0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (v[e] - m) * r;
+__device__ __forceinline__ void put(B* row, const Columns<LANES, V, VEC>& c, int j, const Four<B>& x) {
+    put(row, c, j, Quad<B>{{x.v[0], x.v[1], x.v[2], x.v[3]}});
+}
+// Four values of a parameter (or a shared gate row); 0 beyond the row.
+template <typename B, int LANES, int V, bool VEC>
+__device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, VEC>& c, int j) {
+    Quad<B> q{};
+    if constexpr (VEC) {
+        if (c.ok(j, 0)) q = load_quad(row + c.apart(j, 0));
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c.ok(j, e) ? (v[e] - mean) * rstd : B(0);
+        for (int e = 0; e < 4; ++e)
+            if (c.ok(j, e)) q.v[e] = row[c.apart(j, e)];
     }
+    return widen4<B>(q);
+}
+// x for the row's own columns, 0 beyond them
+template <typename B, int LANES, int V, bool VEC>
+__device__ __forceinline__ Four<B> within(const Columns<LANES, V, VEC>& c, int j, Four<B> x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.v[e] = c.ok(j, e) ? x.v[e] : B(0);
+    return x;
 }
 
 // 1 / sqrt: the float approximation (2 ulp) and a Newton step, instead of a correctly rounded root and division
@@ -229,93 +359,73 @@ template <typename B, int LANES, bool BIG> struct Team {
     }
 };
 
-// Rows of one team: item after item, `chunk` rows each.  Every team of a warp makes the same number of steps; a step
-// beyond an item's or the matrix's end is not active.
-struct RowCursor {
-    uint32_t item, row, last;
-    int pos;
-    __device__ __forceinline__ void enter(const RingPlan& p) {
-        pos = 0;
-        row = item;
-        last = item + 1;
-        if (p.shared) {
-            const uint32_t span = item / (uint32_t)p.per_span;
-            row = span * (uint32_t)p.span + (item - span * (uint32_t)p.per_span) * (uint32_t)p.chunk;
-            last = min(row + (uint32_t)p.chunk, (span + 1) * (uint32_t)p.span);
-        }
-        if (item >= (uint32_t)p.items) last = row = 0;
-    }
-    __device__ __forceinline__ bool active() const { return row < last; }
-    __device__ __forceinline__ void next(const RingPlan& p) {
-        ++row;
-        if (++pos >= p.chunk) {
-            item += (uint32_t)p.teams;
-            enter(p);
-        }
-    }
-};
 // start of a row: rows and strides are below 2^31 here, so one wide multiplication
 template <typename T> __device__ __forceinline__ T* row_at(T* base, uint32_t row, int64_t stride) {
     return base + (uint64_t)row * (uint32_t)stride;
 }
 
+// The team's place: its first column, and its first row.
 template <int LANES, int V, bool VEC, bool BIG, typename B>
-__device__ __forceinline__ void set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, LANES, BIG>& team,
-                                       Columns<LANES, V, VEC>& c, uint32_t& team_id, uint32_t& first_of_warp) {
+__device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, LANES, BIG>& team,
+                                           Columns<LANES, V, VEC>& c) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     team.scratch = scratch;
     team.cluster = BIG ? p.cluster : 1;
     team.rank = BIG && p.cluster > 1 ? (int)(blockIdx.x % p.cluster) : 0;
     const uint32_t group = BIG && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
+    uint32_t id;
     if (LANES == 32) {
         team.warps = p.warps;
         team.team = p.teams_per_block == 1 ? 0 : warp / p.warps;
         team.warp = warp - team.team * p.warps;
         team.lane = lane;
         c.col = (team.rank * p.warps + team.warp) * V * kPackGroup + (VEC ? 4 * lane : lane);
-        team_id = group * p.teams_per_block + team.team;
-        first_of_warp = team_id;
+        id = group * p.teams_per_block + team.team;
     } else {
         team.warps = 1;
         team.team = 0;
         team.warp = 0;
         team.lane = lane & (LANES - 1);
         c.col = VEC ? 4 * team.lane : team.lane;
-        team_id = group * p.teams_per_block + threadIdx.x / LANES;
-        first_of_warp = group * p.teams_per_block + warp * (32 / LANES);
+        id = group * p.teams_per_block + threadIdx.x / LANES;
     }
     c.width = width;
     if (BIG && p.cluster > 1) cooperative_groups::this_cluster().sync();      // every block's scratch exists
+    return id;
 }
 
-// Codes of a thread's elements and, from one lane each, the scales of their groups.  A group is a warp's chunk, or with
-// fewer lanes 32 / LANES chunks of the same threads.
+// Codes of a thread's elements and the scales of their groups.  A group is a warp's chunk, or with fewer lanes 32 / LANES
+// chunks of the same threads.  Each lane forms the scale and its reciprocal of one group only.
 template <typename B, int LANES, int V, bool VEC>
-__device__ __forceinline__ void put_codes(int format, const B (&v)[V][4], const Columns<LANES, V, VEC>& c, bool write,
+__device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], const Columns<LANES, V, VEC>& c, bool write,
                                           uint8_t* codes, B* scales, int lane) {
-    constexpr int kTogether = 32 / LANES < V ? 32 / LANES : V;
+    constexpr int kTogether = 32 / LANES < V ? 32 / LANES : V, kGroups = V / kTogether;
+    using Bits = typename AbsBits<B>::type;
+    Bits mine = 0;
 #pragma unroll
-    for (int j0 = 0; j0 < V; j0 += kTogether) {
-        typename AbsBits<B>::type top = 0;
+    for (int i = 0; i < kGroups; ++i) {
+        Bits top = 0;
 #pragma unroll
-        for (int j = j0; j < j0 + kTogether; ++j)
+        for (int j = i * kTogether; j < (i + 1) * kTogether; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, AbsBits<B>::of(c.ok(j, e) ? v[j][e] : B(0)));
-        const B scale = pack_scale<B>(format, AbsBits<B>::back(lanes_max<LANES>(top))), inv = pack_inverse<B>(scale);
+            for (int e = 0; e < 4; ++e) top = max(top, AbsBits<B>::of(c.ok(j, e) ? v[j].v[e] : B(0)));
+        top = lanes_max<LANES>(top);
+        if (kGroups == 1 || lane % kGroups == i) mine = top;
+    }
+    const B scale = pack_scale<B>(format, AbsBits<B>::back(mine)), inverse = pack_inverse<B>(scale);
+    const int first = (c.col - (VEC ? 4 * lane : lane)) / kPackGroup;          // the warp's first group
+    if (write && lane < kGroups && (first + lane) * kPackGroup < c.width) scales[first + lane] = scale;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        const B inv = kGroups == 1 ? inverse : __shfl_sync(0xffffffffu, inverse, i, LANES);
         if (!write) continue;
 #pragma unroll
-        for (int j = j0; j < j0 + kTogether; ++j) {
-            uint8_t q[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = (uint8_t)to_code(format, v[j][e], inv);
-            put<uint8_t, LANES, V, VEC>(codes, c, j, q);
+        for (int j = i * kTogether; j < (i + 1) * kTogether; ++j) {
+            const uint32_t word = encode4(format, v[j], inv);
+            put(codes, c, j, *reinterpret_cast<const Quad<uint8_t>*>(&word));
         }
-        if (lane == 0 && c.at(j0, 0) < c.width) scales[c.at(j0, 0) / kPackGroup] = scale;
     }
 }
-
-#define KANB200_EACH(j, e)                  \
-    _Pragma("unroll") for (int j = 0; j < V; ++j) _Pragma("unroll") for (int e = 0; e < 4; ++e)
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, bool VEC, bool BRANCH, bool BIG>
@@ -330,9 +440,8 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
     Columns<LANES, V, VEC> c;
-    uint32_t team_id, first_of_warp;
-    set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c, team_id, first_of_warp);
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const uint32_t id = set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c);
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const bool row_gate = BRANCH && a.gate && !p.shared;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const B eps = B(a.eps), per = B(1) / B(D);
@@ -343,31 +452,41 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
             *pb = static_cast<const B*>(a.post_bias) + c.col, *nw = static_cast<const B*>(a.next_weight) + c.col,
             *nb = static_cast<const B*>(a.next_bias) + c.col;
 
-    const auto issue = [&](const RowCursor& r, int stage) {
-        if (r.active()) {
+    const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
+                   last = p.shared ? min(first + p.rows_per_team, rows) : rows;
+    const auto issue = [&](uint32_t row, int stage) {
+        if (row < last) {
             const uint32_t at = ring_at + stage * p.stage_bytes;
-            FS::issue(at, row_at(x, r.row, a.x_stride), c);
-            if (BRANCH) FB::issue(at + at_y, row_at(y, r.row, a.y_stride), c);
-            if (row_gate) FB::issue(at + at_gate, row_at(gate, r.row, a.gate_stride), c);
+            FS::issue(at, row_at(x, row, a.x_stride), c);
+            if (BRANCH) FB::issue(at + at_y, row_at(y, row, a.y_stride), c);
+            if (row_gate) FB::issue(at + at_gate, row_at(gate, row, a.gate_stride), c);
         }
         copies_commit();
     };
     // the row's mean and 1 / deviation; two passes over registers, so that the variance has no cancellation
-    const auto moments = [&](int kind, const B (&v)[V][4], B& mean, B& rstd) {
+    const auto moments = [&](int kind, const Four<B> (&v)[V], B& mean, B& rstd) {
         mean = B(0);
-        B s[1] = {B(0)};
+        Four<B> acc = four<B>(B(0));
+        B s[1];
         if (kind == kNormLayer) {
-            KANB200_EACH(j, e) s[0] += v[j][e];             // columns beyond the row hold 0
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc = acc + v[j];           // columns beyond the row hold 0
+            s[0] = total(acc);
             team.template sum<1>(s);
             mean = s[0] * per;
-            s[0] = B(0);
+            acc = four<B>(B(0));
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const Four<B> d = within<B>(c, j, v[j] + four<B>(-mean));
+                acc = fma4(d, d, acc);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc = fma4(v[j], v[j], acc);
         }
-        KANB200_EACH(j, e) {
-            const B d = c.ok(j, e) ? v[j][e] - mean : B(0);
-            s[0] += d * d;
-        }
+        s[0] = total(acc);
         team.template sum<1>(s);
-        rstd = rsqrt_newton(s[0] * per + eps);
+        rstd = rsqrt_newton(fma(s[0], per, eps));
     };
     const auto put_stats = [&](void* stats, uint32_t row, B mean, B rstd) {
         if (c.col == 0) {
@@ -377,105 +496,79 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
         }
     };
 
-    RowCursor now, ahead;
-    now.item = team_id;
-    now.enter(p);
-    ahead = now;
-    for (int s = 0; s + 1 < p.stages; ++s) {
-        issue(ahead, s);
-        ahead.next(p);
+    uint32_t span_end = first, span = 0;                    // of a shared gate: where its next row starts
+    if (p.shared) {
+        span = first / (uint32_t)a.gate_rows;
+        span_end = first;
     }
+    uint32_t ahead = first;
+    for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
     int stage = 0;
-    B t[V][4];                                              // scale act(gate) of a shared gate
-    for (uint32_t lead = first_of_warp; lead < (uint32_t)p.items;) {
+    Four<B> t[V];                                           // act(gate) of a shared gate
+    // every team makes the same number of steps: teams that share a warp meet in its shuffles
+    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
         issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
-        ahead.next(p);
         copies_wait_oldest(p.stages);
-        const bool live = now.active();
+        const bool live = row < last;
+        if (LANES == 32 && !live) break;                    // a whole team, alone in its warps
         const char* at = ring + stage * p.stage_bytes;
-        const uint32_t row = now.row;
         const uint64_t dense = (uint64_t)row * (uint32_t)D + (uint32_t)c.col;      // of dense tensors
-        B o[V][4] = {};
-        if (BRANCH) {
-            B v[V][4] = {};
-            if (live)
+        Four<B> o[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) FB::take(at + at_y, row_at(y, row, a.y_stride), c, j, v[j]);
+        for (int j = 0; j < V; ++j) o[j] = four<B>(B(0));
+        if (BRANCH) {
+            Four<B> v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = live ? widen4<B>(FB::take(at + at_y, row_at(y, row, a.y_stride), c, j)) : four<B>(B(0));
             if (a.y_codes)
-                put_codes<B, LANES, V, VEC>(a.checkpoint, v, c, live, static_cast<uint8_t*>(a.y_codes) + dense,
-                                            row_at(static_cast<B*>(a.y_scales), row, groups), team.lane);
-            B mean = B(0), rstd = B(1);
+                put_codes<B>(a.checkpoint, v, c, live, static_cast<uint8_t*>(a.y_codes) + dense,
+                             row_at(static_cast<B*>(a.y_scales), row, groups), team.lane);
             if (a.post_norm != kNormNone) {
+                B mean, rstd;
                 moments(a.post_norm, v, mean, rstd);
                 if (a.post_stats && live) put_stats(a.post_stats, row, mean, rstd);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = (v[j] + four<B>(-mean)) * four<B>(rstd);
             }
-            if (p.shared && now.pos == 0 && live) {
-                const B* shared = row_at(gate, row / (uint32_t)a.gate_rows, a.gate_stride);
+            if (p.shared && row >= span_end && live) {
+                span = row / (uint32_t)a.gate_rows;
+                span_end = (span + 1) * (uint32_t)a.gate_rows;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    get<B, LANES, V, VEC>(shared, c, j, t[j]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) t[j][e] = gate_value<B>(a.gate_act, t[j][e]);
-                }
+                for (int j = 0; j < V; ++j) t[j] = gate4<B>(a.gate_act, get(row_at(gate, span, a.gate_stride), c, j));
             }
             // out = x + scale act(gate) z; what v becomes is the branch's summand
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                B w[4];
-                normalise<B>(c, j, mean, rstd, v[j]);
-                if (a.post_weight) {
-                    get<B, LANES, V, VEC>(pw, c, j, w);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[j][e] *= w[e];
-                }
-                if (a.post_bias) {
-                    get<B, LANES, V, VEC>(pb, c, j, w);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[j][e] += w[e];
-                }
-                if (p.shared)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[j][e] *= t[j][e];
-                if (a.scale) {
-                    get<B, LANES, V, VEC>(scale, c, j, w);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[j][e] *= w[e];
-                }
+                if (a.post_weight) v[j] = v[j] * get(pw, c, j);
+                if (a.post_bias) v[j] = v[j] + get(pb, c, j);
+                if (p.shared) v[j] = v[j] * t[j];
+                if (a.scale) v[j] = v[j] * get(scale, c, j);
             }
             if (row_gate) {
-                B g[V][4] = {};
-                if (live)
+                Four<B> g[V];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) FB::take(at + at_gate, row_at(gate, row, a.gate_stride), c, j, g[j]);
+                for (int j = 0; j < V; ++j)
+                    g[j] = live ? widen4<B>(FB::take(at + at_gate, row_at(gate, row, a.gate_stride), c, j)) : four<B>(B(0));
                 if (a.gate_codes)
-                    put_codes<B, LANES, V, VEC>(a.checkpoint, g, c, live, static_cast<uint8_t*>(a.gate_codes) + dense,
-                                                row_at(static_cast<B*>(a.gate_scales), row, groups), team.lane);
-                KANB200_EACH(j, e) v[j][e] *= gate_value<B>(a.gate_act, g[j][e]);
+                    put_codes<B>(a.checkpoint, g, c, live, static_cast<uint8_t*>(a.gate_codes) + dense,
+                                 row_at(static_cast<B*>(a.gate_scales), row, groups), team.lane);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = v[j] * gate4<B>(a.gate_act, g[j]);
             }
             if (live)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    S xv[4];
-                    FS::take(at, row_at(x, row, a.x_stride), c, j, xv);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        xv[e] = narrow<S>(widen(xv[e]) + v[j][e]);
-                        o[j][e] = c.ok(j, e) ? widen(xv[e]) : B(0);
-                    }
-                    put<S, LANES, V, VEC>(static_cast<S*>(a.out) + dense, c, j, xv);
+                    const Quad<S> q = narrow4<S>(widen4<S>(FS::take(at, row_at(x, row, a.x_stride), c, j)) + v[j]);
+                    o[j] = within<B>(c, j, widen4<S>(q));
+                    put(static_cast<S*>(a.out) + dense, c, j, q);
                 }
         } else if (live) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                S xv[4];
-                FS::take(at, row_at(x, row, a.x_stride), c, j, xv);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] = widen(xv[e]);
-            }
+            for (int j = 0; j < V; ++j) o[j] = widen4<S>(FS::take(at, row_at(x, row, a.x_stride), c, j));
         }
         if (a.x_codes)
-            put_codes<B, LANES, V, VEC>(a.checkpoint, o, c, live, static_cast<uint8_t*>(a.x_codes) + dense,
-                                        row_at(static_cast<B*>(a.x_scales), row, groups), team.lane);
+            put_codes<B>(a.checkpoint, o, c, live, static_cast<uint8_t*>(a.x_codes) + dense,
+                         row_at(static_cast<B*>(a.x_scales), row, groups), team.lane);
         if (!BRANCH || a.next_norm != kNormNone) {
             B mean, rstd;
             moments(a.next_norm, o, mean, rstd);
@@ -483,23 +576,12 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
             if (live)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    B w[4];
-                    normalise<B>(c, j, mean, rstd, o[j]);
-                    if (a.next_weight) {
-                        get<B, LANES, V, VEC>(nw, c, j, w);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][e] *= w[e];
-                    }
-                    if (a.next_bias) {
-                        get<B, LANES, V, VEC>(nb, c, j, w);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][e] += w[e];
-                    }
-                    put<B, LANES, V, VEC>(static_cast<B*>(a.h) + dense, c, j, o[j]);
+                    o[j] = (o[j] + four<B>(-mean)) * four<B>(rstd);
+                    if (a.next_weight) o[j] = o[j] * get(nw, c, j);
+                    if (a.next_bias) o[j] = o[j] + get(nb, c, j);
+                    put(static_cast<B*>(a.h) + dense, c, j, o[j]);
                 }
         }
-        now.next(p);
-        if (now.pos == 0) lead += (uint32_t)p.teams;
         stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
     copies_wait<0>();
@@ -520,19 +602,21 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
     Columns<LANES, V, VEC> c;
-    uint32_t team_id, first_of_warp;
-    set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c, team_id, first_of_warp);
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const uint32_t id = set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c);
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const bool row_gate = BRANCH && (a.gate || a.gate_codes) && !p.shared;
     const B per = B(1) / B(D);
+    const Four<B> zero = four<B>(B(0));
 
     const S *x = static_cast<const S*>(a.x) + c.col, *dout = static_cast<const S*>(a.dout) + c.col;
     const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col,
             *dh = static_cast<const B*>(a.dh) + c.col, *scale = static_cast<const B*>(a.scale) + c.col,
             *pw = static_cast<const B*>(a.post_weight) + c.col, *pb = static_cast<const B*>(a.post_bias) + c.col,
             *nw = static_cast<const B*>(a.next_weight) + c.col;
-    B sum_scale[V][4] = {}, sum_pw[V][4] = {}, sum_pb[V][4] = {}, sum_nw[V][4] = {}, sum_nb[V][4] = {}, sum_gate[V][4] = {};
+    Four<B> sum_scale[V], sum_pw[V], sum_pb[V], sum_nw[V], sum_nb[V], sum_gate[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum_scale[j] = sum_pw[j] = sum_pb[j] = sum_nw[j] = sum_nb[j] = sum_gate[j] = zero;
 
     // a tensor that may be there as codes: codes and their groups' scales, or the values themselves
     const auto issue_kept = [&](uint32_t at, const void* codes, const void* scales, auto* values, int64_t stride, uint32_t row) {
@@ -548,225 +632,187 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
             Feed<E, LANES, V, VEC, T>::issue(at, row_at(values, row, stride), c);
         }
     };
-    const auto take_kept = [&](const char* at, const void* codes, auto* values, int64_t stride, uint32_t row, int j, B (&v)[4]) {
+    const auto take_kept = [&](const char* at, const void* codes, auto* values, int64_t stride, uint32_t row, int j) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
         if (codes) {
-            uint8_t q[4];
-            FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c, j, q);
+            const Quad<uint8_t> q = FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c, j);
             const B s = c.at(j, 0) < D ? *reinterpret_cast<const B*>(at + 4 * V * T + (j * T + threadIdx.x) * sizeof(B)) : B(0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = from_code<B>(a.checkpoint, q[e], s);
-        } else {
-            E raw[4];
-            Feed<E, LANES, V, VEC, T>::take(at, row_at(values, row, stride), c, j, raw);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = widen(raw[e]);
+            return decode4<B>(a.checkpoint, *reinterpret_cast<const uint32_t*>(&q), s);
         }
+        return widen4<E>(Feed<E, LANES, V, VEC, T>::take(at, row_at(values, row, stride), c, j));
     };
-    const auto issue = [&](const RowCursor& r, int stage) {
-        if (r.active()) {
+    const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
+                   last = p.shared ? min(first + p.rows_per_team, rows) : rows;
+    const auto issue = [&](uint32_t row, int stage) {
+        if (row < last) {
             const uint32_t at = ring_at + stage * p.stage_bytes;
-            if (a.dout) FS::issue(at + At::dout, row_at(dout, r.row, a.dout_stride), c);
+            if (a.dout) FS::issue(at + At::dout, row_at(dout, row, a.dout_stride), c);
             if (NEXT) {
-                FB::issue(at + At::dh, row_at(dh, r.row, a.dh_stride), c);
-                issue_kept(at + At::x, a.x_codes, a.x_scales, x, a.x_stride, r.row);
+                FB::issue(at + At::dh, row_at(dh, row, a.dh_stride), c);
+                issue_kept(at + At::x, a.x_codes, a.x_scales, x, a.x_stride, row);
                 copy_async<2 * sizeof(B)>(at + At::next_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
-                                          static_cast<const B*>(a.next_stats) + 2 * (uint64_t)r.row);
+                                          static_cast<const B*>(a.next_stats) + 2 * (uint64_t)row);
             }
             if (BRANCH) {
-                issue_kept(at + At::y, a.y_codes, a.y_scales, y, a.y_stride, r.row);
-                if (row_gate) issue_kept(at + At::gate, a.gate_codes, a.gate_scales, gate, a.gate_stride, r.row);
+                issue_kept(at + At::y, a.y_codes, a.y_scales, y, a.y_stride, row);
+                if (row_gate) issue_kept(at + At::gate, a.gate_codes, a.gate_scales, gate, a.gate_stride, row);
                 if (a.post_norm != kNormNone)
                     copy_async<2 * sizeof(B)>(at + At::post_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
-                                              static_cast<const B*>(a.post_stats) + 2 * (uint64_t)r.row);
+                                              static_cast<const B*>(a.post_stats) + 2 * (uint64_t)row);
             }
         }
         copies_commit();
     };
 
-    RowCursor now, ahead;
-    now.item = team_id;
-    now.enter(p);
-    ahead = now;
-    for (int s = 0; s + 1 < p.stages; ++s) {
-        issue(ahead, s);
-        ahead.next(p);
+    uint32_t span = 0, span_first = first, span_end = first;             // of a shared gate: the rows under its row
+    if (p.shared) {
+        span = first / (uint32_t)a.gate_rows;
+        span_first = span * (uint32_t)a.gate_rows;
+        span_end = span_first + (uint32_t)a.gate_rows;
     }
+    uint32_t ahead = first;
+    for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
     int stage = 0;
-    for (uint32_t lead = first_of_warp; lead < (uint32_t)p.items;) {
+    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
         issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
-        ahead.next(p);
         copies_wait_oldest(p.stages);
-        const bool live = now.active();
+        const bool live = row < last;
+        if (LANES == 32 && !live) break;
         const char* at = ring + stage * p.stage_bytes;
-        const uint32_t row = now.row;
         const uint64_t dense = (uint64_t)row * (uint32_t)D + (uint32_t)c.col;      // of dense tensors
-        B g[V][4] = {};                                     // gradient of the norm's input, then of y
-        if (a.dout && live)
+        Four<B> g[V];                                       // gradient of the norm's input, then of y
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                S raw[4];
-                FS::take(at + At::dout, row_at(dout, row, a.dout_stride), c, j, raw);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) g[j][e] = widen(raw[e]);
-            }
+        for (int j = 0; j < V; ++j)
+            g[j] = a.dout && live ? widen4<S>(FS::take(at + At::dout, row_at(dout, row, a.dout_stride), c, j)) : zero;
         if (NEXT) {
-            B v[V][4] = {}, d[V][4] = {}, mean = B(0), rstd = B(0), s[2] = {B(0), B(0)};
+            Four<B> v[V], d[V], s0 = zero, s1 = zero;
+            B rstd = B(0);
             if (live) {
                 const B* stats = reinterpret_cast<const B*>(at + At::next_stats + threadIdx.x * 2 * sizeof(B));
-                mean = stats[0];
+                const B mean = stats[0];
                 rstd = stats[1];
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    FB::take(at + At::dh, row_at(dh, row, a.dh_stride), c, j, d[j]);
-                    take_kept(at + At::x, a.x_codes, x, a.x_stride, row, j, v[j]);
-                    normalise<B>(c, j, mean, rstd, v[j]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sum_nw[j][e] += d[j][e] * v[j][e];
-                        sum_nb[j][e] += d[j][e];
-                    }
-                    if (a.next_weight) {
-                        B w[4];
-                        get<B, LANES, V, VEC>(nw, c, j, w);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) d[j][e] *= w[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[0] += d[j][e];
-                        s[1] += d[j][e] * v[j][e];
-                    }
+                    d[j] = widen4<B>(FB::take(at + At::dh, row_at(dh, row, a.dh_stride), c, j));
+                    v[j] = take_kept(at + At::x, a.x_codes, x, a.x_stride, row, j);
+                    v[j] = within<B>(c, j, (v[j] + four<B>(-mean)) * four<B>(rstd));          // the normalised row
+                    sum_nw[j] = fma4(d[j], v[j], sum_nw[j]);
+                    sum_nb[j] = sum_nb[j] + d[j];
+                    if (a.next_weight) d[j] = d[j] * get(nw, c, j);
+                    s0 = s0 + d[j];
+                    s1 = fma4(d[j], v[j], s1);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = d[j] = zero;
             }
+            B s[2] = {total(s0), total(s1)};
             team.template sum<2>(s);
-            const B flat = a.next_norm == kNormLayer ? s[0] * per : B(0), along = s[1] * per;
-            KANB200_EACH(j, e) g[j][e] += rstd * (d[j][e] - flat - v[j][e] * along);
+            const Four<B> flat = four<B>(a.next_norm == kNormLayer ? -s[0] * per : B(0)), along = four<B>(-s[1] * per);
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[j] = fma4(four<B>(rstd), fma4(v[j], along, d[j] + flat), g[j]);
         }
         if (a.dx && live)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                S o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = narrow<S>(g[j][e]);
-                put<S, LANES, V, VEC>(static_cast<S*>(a.dx) + dense, c, j, o);
-            }
+            for (int j = 0; j < V; ++j) put(static_cast<S*>(a.dx) + dense, c, j, narrow4<S>(g[j]));
         if (BRANCH) {
-            B v[V][4] = {}, mean = B(0), rstd = B(1), s[2] = {B(0), B(0)};
+            Four<B> v[V], s0 = zero, s1 = zero;
+            B rstd = B(1);
             if (live) {
+                B mean = B(0);
                 if (a.post_norm != kNormNone) {
                     const B* stats = reinterpret_cast<const B*>(at + At::post_stats + threadIdx.x * 2 * sizeof(B));
                     mean = stats[0];
                     rstd = stats[1];
                 }
-                const B* shared = p.shared ? row_at(gate, row / (uint32_t)a.gate_rows, a.gate_stride) : nullptr;
+                if (p.shared && row == span_end) {
+                    ++span;
+                    span_first = span_end;
+                    span_end += (uint32_t)a.gate_rows;
+                }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    B w[4], act[4], dact[4], z[4];
-                    take_kept(at + At::y, a.y_codes, y, a.y_stride, row, j, v[j]);
-                    normalise<B>(c, j, mean, rstd, v[j]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        z[e] = v[j][e];
-                        act[e] = B(1);
-                        dact[e] = B(0);
-                    }
+                    v[j] = take_kept(at + At::y, a.y_codes, y, a.y_stride, row, j);
+                    if (a.post_norm != kNormNone) v[j] = within<B>(c, j, (v[j] + four<B>(-mean)) * four<B>(rstd));
+                    Four<B> z = v[j], w;
                     if (a.post_weight) {
-                        get<B, LANES, V, VEC>(pw, c, j, w);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) z[e] *= w[e];
+                        w = get(pw, c, j);
+                        z = z * w;
                     }
-                    if (a.post_bias) {
-                        B b[4];
-                        get<B, LANES, V, VEC>(pb, c, j, b);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) z[e] += b[e];
-                    }
+                    if (a.post_bias) z = z + get(pb, c, j);
                     if (p.shared || row_gate) {
-                        B gv[4];
-                        if (p.shared) get<B, LANES, V, VEC>(shared, c, j, gv);
-                        else take_kept(at + At::gate, a.gate_codes, gate, a.gate_stride, row, j, gv);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) gate_value_grad<B>(a.gate_act, gv[e], act[e], dact[e]);
+                        Four<B> act, dact;
+                        const Four<B> gv = p.shared ? get(row_at(gate, span, a.gate_stride), c, j)
+                                                    : take_kept(at + At::gate, a.gate_codes, gate, a.gate_stride, row, j);
+                        gate4_grad<B>(a.gate_act, gv, act, dact);
+                        const Four<B> gz = g[j] * z;
+                        sum_scale[j] = fma4(gz, act, sum_scale[j]);
+                        Four<B> dg = gz * dact;
+                        if (a.scale) {
+                            const Four<B> sc = get(scale, c, j);
+                            dg = dg * sc;
+                            act = act * sc;
+                        }
+                        if (p.shared) sum_gate[j] = sum_gate[j] + dg;
+                        else if (a.dgate) put(row_at(static_cast<B*>(a.dgate) + c.col, row, a.dgate_stride), c, j, dg);
+                        g[j] = g[j] * act;
+                    } else {
+                        sum_scale[j] = fma4(g[j], z, sum_scale[j]);
+                        if (a.scale) g[j] = g[j] * get(scale, c, j);
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum_scale[j][e] += g[j][e] * act[e] * z[e];
-                    if (a.scale) {
-                        B sc[4];
-                        get<B, LANES, V, VEC>(scale, c, j, sc);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) g[j][e] *= sc[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        z[e] *= g[j][e] * dact[e];                          // this row's share of dgate
-                        g[j][e] *= act[e];
-                        sum_pw[j][e] += g[j][e] * v[j][e];
-                        sum_pb[j][e] += g[j][e];
-                    }
-                    if (p.shared) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum_gate[j][e] += z[e];
-                    } else if (a.dgate) {
-                        put<B, LANES, V, VEC>(row_at(static_cast<B*>(a.dgate) + c.col, row, a.dgate_stride), c, j, z);
-                    }
-                    if (a.post_weight)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) g[j][e] *= w[e];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[0] += g[j][e];
-                        s[1] += g[j][e] * v[j][e];
-                    }
+                    sum_pw[j] = fma4(g[j], v[j], sum_pw[j]);
+                    sum_pb[j] = sum_pb[j] + g[j];
+                    if (a.post_weight) g[j] = g[j] * w;
+                    s0 = s0 + g[j];
+                    s1 = fma4(g[j], v[j], s1);
                 }
             }
             if (a.dy) {
                 if (a.post_norm != kNormNone) {
+                    B s[2] = {total(s0), total(s1)};
                     team.template sum<2>(s);
-                    const B flat = a.post_norm == kNormLayer ? s[0] * per : B(0), along = s[1] * per;
-                    KANB200_EACH(j, e) g[j][e] = rstd * (g[j][e] - flat - v[j][e] * along);
+                    const Four<B> flat = four<B>(a.post_norm == kNormLayer ? -s[0] * per : B(0)), along = four<B>(-s[1] * per);
+                    if (live)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) g[j] = four<B>(rstd) * fma4(v[j], along, g[j] + flat);
                 }
                 if (live)
 #pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        put<B, LANES, V, VEC>(row_at(static_cast<B*>(a.dy) + c.col, row, a.dy_stride), c, j, g[j]);
+                    for (int j = 0; j < V; ++j) put(row_at(static_cast<B*>(a.dy) + c.col, row, a.dy_stride), c, j, g[j]);
             }
-            if (slabs.gate && now.pos + 1 == p.chunk) {
+            if (slabs.gate && live && (row + 1 == span_end || row + 1 == last)) {
+                // a gate row whose rows are all this team's is finished here, otherwise its share goes to a slab
+                B* to = first <= span_first && row + 1 == span_end
+                            ? row_at(static_cast<B*>(a.dgate) + c.col, span, a.dgate_stride)
+                            : static_cast<B*>(slabs.gate) + (uint64_t)(id + span) * (uint32_t)D + c.col;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    if (now.item < (uint32_t)p.items)
-                        put<B, LANES, V, VEC>(static_cast<B*>(slabs.gate) + (uint64_t)now.item * (uint32_t)D + c.col, c, j, sum_gate[j]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum_gate[j][e] = B(0);
+                    put(to, c, j, sum_gate[j]);
+                    sum_gate[j] = zero;
                 }
             }
         }
-        now.next(p);
-        if (now.pos == 0) lead += (uint32_t)p.teams;
         stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
     copies_wait<0>();
 
     // one slab row per block: the teams' sums, added in the order of the teams
     const uint32_t block = BIG && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
-    Quad<B>* shelf = reinterpret_cast<Quad<B>*>(ring);
+    Four<B>* shelf = reinterpret_cast<Four<B>*>(ring);
     const int per_team = blockDim.x / p.teams_per_block;
-    const auto leave = [&](int which, B (&v)[V][4]) {
+    const auto leave = [&](int which, Four<B> (&v)[V]) {
         if (!slabs.column[which]) return;
         B* row = static_cast<B*>(slabs.column[which]) + (uint64_t)block * (uint32_t)D + c.col;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             if (p.teams_per_block > 1) {
                 __syncthreads();
-#pragma unroll
-                for (int e = 0; e < 4; ++e) shelf[threadIdx.x].v[e] = v[j][e];
+                shelf[threadIdx.x] = v[j];
                 __syncthreads();
                 if ((int)threadIdx.x >= per_team) continue;
-                for (int i = 1; i < p.teams_per_block; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[j][e] += shelf[i * per_team + threadIdx.x].v[e];
+                for (int i = 1; i < p.teams_per_block; ++i) v[j] = v[j] + shelf[i * per_team + threadIdx.x];
             }
-            put<B, LANES, V, VEC>(row, c, j, v[j]);
+            put(row, c, j, v[j]);
         }
     };
     if (BRANCH) {
@@ -779,7 +825,6 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
         leave(kSumNextBias, sum_nb);
     }
 }
-#undef KANB200_EACH
 
 }  // namespace kanb200
 
@@ -811,17 +856,20 @@ cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...)
 
 template <typename S, int LANES, bool VEC, bool BIG>
 cudaError_t ring_forward_as(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st) {
-    constexpr bool f64 = sizeof(S) == 8;
-    return a.y ? ring_launch(p, st, ring_forward_kernel<S, LANES, ring_chunks(false, true, f64), VEC, true, BIG>, a, p)
-               : ring_launch(p, st, ring_forward_kernel<S, LANES, ring_chunks(false, false, f64), VEC, false, BIG>, a, p);
+    constexpr int V = ring_chunks(false, true, sizeof(S) == 8);
+    return a.y ? ring_launch(p, st, ring_forward_kernel<S, LANES, V, VEC, true, BIG>, a, p)
+               : ring_launch(p, st, ring_forward_kernel<S, LANES, V, VEC, false, BIG>, a, p);
 }
 template <typename S, int LANES, bool VEC, bool BIG>
 cudaError_t ring_backward_as(const kanb200_block_args& a, const RingPlan& p, const BackwardSlabs& slabs, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
-    constexpr int alone = ring_chunks(true, false, f64), branch = ring_chunks(true, true, f64);
-    if (!a.has_branch) return ring_launch(p, st, ring_backward_kernel<S, LANES, alone, VEC, false, true, BIG>, a, p, slabs);
-    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, branch, VEC, true, true, BIG>, a, p, slabs)
-                : ring_launch(p, st, ring_backward_kernel<S, LANES, branch, VEC, true, false, BIG>, a, p, slabs);
+    if (!a.has_branch)
+        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, false, f64), VEC, false, true, BIG>,
+                           a, p, slabs);
+    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), VEC, true, true, BIG>,
+                              a, p, slabs)
+                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), VEC, true, false, BIG>,
+                              a, p, slabs);
 }
 
 #define KANB200_RING_DISPATCH(name, ...)                                                                    \
