@@ -370,7 +370,6 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     const int B = (int)branch_bytes(a.dtype), S = a.dtype == KANB200_F64 ? 8 : a.dtype == KANB200_F32 ? 4 : 2;
     const bool branch = backward ? a.has_branch : a.y != nullptr;
     const int per_warp = warp_columns(a, backward), V = per_warp / kPackGroup;
-    p.vec = four_at_once(a);
     p.lanes = 4;
     while (p.lanes < 32 && p.lanes * 4 * V < a.width) p.lanes *= 2;
     const int all = (int)div_up(a.width, per_warp);
@@ -381,28 +380,28 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.teams_per_block = p.big ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
     p.threads = p.lanes == 32 ? 32 * p.warps * p.teams_per_block : 256;
     const int T = p.threads;
+    const bool vec = four_at_once(a);
+    p.mode = !vec ? kScalar : p.lanes * 4 * V * (p.lanes == 32 ? p.warps * p.cluster : 1) == a.width ? kFull : kVector;
 
     // a stage of the ring: BackwardStage, or x, y and a gate per row
     const int most = ring_threads(p.big);
     const bool row_gate = branch && (a.gate || a.gate_codes) && !(a.gate && a.gate_rows > 1);
     if (backward) {
         const auto take = [&](bool there, int bytes) { p.stage_bytes += there ? bytes : 0; };
-        take(a.dh, ring_bytes(B, p.vec, V, most) + ring_kept_bytes(S, p.vec, V, most, B) + 2 * B * most);
-        take(branch, ring_kept_bytes(B, p.vec, V, most, B) + 2 * B * most);
-        take(a.dout || row_gate, ring_bytes(S, p.vec, V, most));
-        take(row_gate, ring_kept_bytes(B, p.vec, V, most, B));
+        take(a.dh, ring_bytes(B, vec, V, most) + ring_kept_bytes(S, vec, V, most, B) + 2 * B * most);
+        take(branch, ring_kept_bytes(B, vec, V, most, B) + 2 * B * most);
+        take(a.dout || row_gate, ring_bytes(S, vec, V, most));
+        take(row_gate, ring_kept_bytes(B, vec, V, most, B));
     } else {
-        p.stage_bytes = ring_bytes(S, p.vec, V, most) + (branch ? ring_bytes(B, p.vec, V, most) : 0) +
-                        (row_gate ? ring_bytes(B, p.vec, V, most) : 0);
+        p.stage_bytes = ring_bytes(S, vec, V, most) + (branch ? ring_bytes(B, vec, V, most) : 0) +
+                        (row_gate ? ring_bytes(B, vec, V, most) : 0);
     }
     p.stage_bytes = std::max(p.stage_bytes, 4 * B * most);      // the blocks' column sums meet in the ring at the end
 
-    // blocks to an SM by registers (the kernels' launch bounds); stages while the ring leaves L1 about half of the SM's memory
+    // blocks to an SM by registers (the kernels' launch bounds) and shared memory
     const int registers = 65536 / (ring_threads(p.big) * ring_blocks(backward, branch, p.big, B == 8));
     int per_sm = std::max(1, 65536 / (registers * T));
     while (per_sm > 1 && (2 * p.stage_bytes + 2048) * per_sm > 200 * 1024) --per_sm;
-    p.stages = 2;
-    while (p.stages < 4 && (p.stages + 1) * p.stage_bytes * per_sm <= 100 * 1024) ++p.stages;
     static_cast<RowSplit&>(p) = split_rows(a, (int64_t)kSms * per_sm / p.cluster * p.teams_per_block);
     p.blocks = (int)div_up(p.teams, p.teams_per_block) * p.cluster;
     if (!p.shared) {                     // rows in turn: over every team that is launched

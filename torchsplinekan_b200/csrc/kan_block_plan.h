@@ -27,12 +27,15 @@ struct RowSplit {
     int64_t teams;                   // with a shared gate: those that have rows
 };
 
+enum { kFull, kVector, kScalar };    // how a thread reaches its columns, see Columns
+
 struct RingPlan : RowSplit {
     int lanes;                       // 4, 8, 16 or 32
     int warps;                       // of a team, in one block (lanes == 32)
     int teams_per_block, cluster;
-    int threads, blocks, stages, stage_bytes;
-    bool vec, big;
+    int threads, blocks, stage_bytes;
+    int mode;                        // kFull, kVector or kScalar
+    bool big;
 };
 
 // Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers for the sums

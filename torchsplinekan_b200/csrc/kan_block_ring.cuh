@@ -5,12 +5,12 @@
 //     Teams take rows in turn; with a shared gate a team takes consecutive rows, so that a gate row is read, and its
 //     gradient leaves, once per team (consecutive rows everywhere cost 5 to 10 % of the bandwidth: norm of 65536 x 1024
 //     forward 99 us against 91).
-//   * Memory -> registers goes through a ring of 2 to 4 rows in shared memory, filled by cp.async.  A thread copies
+//   * Memory -> registers goes through a ring of two rows in shared memory, filled by cp.async.  A thread copies
 //     exactly what it reads back itself, so the ring needs no barrier: only its own cp.async group to have landed.  The
 //     bytes in flight then do not depend on registers or on how many warps wait in a barrier.
 //   * The sums over rows that are the parameters' gradients stay in registers; one slab row per block leaves the kernel at
 //     its end.  Parameters are read again for every row, from L1: the ring leaves room for them (with 3 rows instead of 2
-//     the gated backward of 16384 x 1024 took 206 us instead of 135, the parameters then came from L2).
+//     the gated backward of 16384 x 1024 took 180 us instead of 122, the parameters then came from L2).
 //   * Sums over a row: lanes by shuffles, warps through shared memory with a barrier of the team alone, blocks of a
 //     cluster through each other's shared memory; every thread gets the same bits.
 //   * Issue slots bound these kernels before bandwidth does, so: what a row costs besides its elements (sums, barriers,
@@ -34,21 +34,17 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT> __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
-// all but the newest stages - 1 groups have landed
-__device__ __forceinline__ void copies_wait_oldest(int stages) {
-    if (stages == 2) copies_wait<1>();
-    else if (stages == 3) copies_wait<2>();
-    else copies_wait<3>();
-}
-
 // Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other; a thread has four of each,
-// side by side (VEC: rows, strides and pointers allow four elements at once) or LANES apart.  Distances between a thread's
-// elements are constants, so a row costs one address per tensor.
-template <int LANES, int V, bool VEC> struct Columns {
+// side by side (kFull, kVector: rows, strides and pointers allow four elements at once) or LANES apart (kScalar).  kFull:
+// the team's columns are exactly the row's, so nothing is masked (a third of the instructions of the gated backward were
+// predicates, selects and zeros).  Distances between a thread's elements are constants, so a row costs one address per tensor.
+template <int LANES, int V, int MODE> struct Columns {
     int col, width;
-    static __device__ __forceinline__ constexpr int apart(int j, int e) { return j * 4 * LANES + (VEC ? e : LANES * e); }
+    static __device__ __forceinline__ constexpr int apart(int j, int e) {
+        return j * 4 * LANES + (MODE != kScalar ? e : LANES * e);
+    }
     __device__ __forceinline__ int at(int j, int e) const { return col + apart(j, e); }
-    __device__ __forceinline__ bool ok(int j, int e) const { return at(j, VEC ? 0 : e) < width; }
+    __device__ __forceinline__ bool ok(int j, int e) const { return MODE == kFull || at(j, MODE == kScalar ? e : 0) < width; }
 };
 
 // ---- four elements --------------------------------------------------------------------------------------------------
@@ -217,8 +213,9 @@ __device__ __forceinline__ uint32_t encode4(int format, const Four<double>& x, d
 // cannot be copied four at a time have no ring slot: they are loaded where they are used.  T is the block's most threads:
 // a slot's pieces are arrays over T threads, so that all distances in a stage are constants too.  `row` and `slot` point to
 // the thread's own first element and place.
-template <typename E, int LANES, int V, bool VEC, int T> struct Feed {
-    using Cols = Columns<LANES, V, VEC>;
+template <typename E, int LANES, int V, int MODE, int T> struct Feed {
+    using Cols = Columns<LANES, V, MODE>;
+    static constexpr bool VEC = MODE != kScalar;
     static constexpr bool kRing = VEC || sizeof(E) >= 4;
     static constexpr int kPiece = VEC ? (4 * sizeof(E) > 16 ? 16 : 4 * (int)sizeof(E)) : (int)sizeof(E);
     static constexpr int kPieces = 4 * (int)sizeof(E) / kPiece;             // per chunk
@@ -267,9 +264,9 @@ template <typename E, int LANES, int V, bool VEC, int T> struct Feed {
 };
 
 // `row`: the thread's own first element, here and below
-template <typename T, int LANES, int V, bool VEC>
-__device__ __forceinline__ void put(T* row, const Columns<LANES, V, VEC>& c, int j, const Quad<T>& q) {
-    if constexpr (VEC) {
+template <typename T, int LANES, int V, int MODE>
+__device__ __forceinline__ void put(T* row, const Columns<LANES, V, MODE>& c, int j, const Quad<T>& q) {
+    if constexpr (MODE != kScalar) {
         if (c.ok(j, 0)) store_quad(row + c.apart(j, 0), q);
     } else {
 #pragma unroll
@@ -277,15 +274,15 @@ __device__ __forceinline__ void put(T* row, const Columns<LANES, V, VEC>& c, int
             if (c.ok(j, e)) row[c.apart(j, e)] = q.v[e];
     }
 }
-template <typename B, int LANES, int V, bool VEC>
-__device__ __forceinline__ void put(B* row, const Columns<LANES, V, VEC>& c, int j, const Four<B>& x) {
+template <typename B, int LANES, int V, int MODE>
+__device__ __forceinline__ void put(B* row, const Columns<LANES, V, MODE>& c, int j, const Four<B>& x) {
     put(row, c, j, Quad<B>{{x.v[0], x.v[1], x.v[2], x.v[3]}});
 }
 // Four values of a parameter (or a shared gate row); 0 beyond the row.
-template <typename B, int LANES, int V, bool VEC>
-__device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, VEC>& c, int j) {
+template <typename B, int LANES, int V, int MODE>
+__device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, MODE>& c, int j) {
     Quad<B> q{};
-    if constexpr (VEC) {
+    if constexpr (MODE != kScalar) {
         if (c.ok(j, 0)) q = load_quad(row + c.apart(j, 0));
     } else {
 #pragma unroll
@@ -295,8 +292,8 @@ __device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, VEC
     return widen4<B>(q);
 }
 // x for the row's own columns, 0 beyond them
-template <typename B, int LANES, int V, bool VEC>
-__device__ __forceinline__ Four<B> within(const Columns<LANES, V, VEC>& c, int j, Four<B> x) {
+template <typename B, int LANES, int V, int MODE>
+__device__ __forceinline__ Four<B> within(const Columns<LANES, V, MODE>& c, int j, Four<B> x) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x.v[e] = c.ok(j, e) ? x.v[e] : B(0);
     return x;
@@ -365,9 +362,9 @@ template <typename T> __device__ __forceinline__ T* row_at(T* base, uint32_t row
 }
 
 // The team's place: its first column, and its first row.
-template <int LANES, int V, bool VEC, bool BIG, typename B>
+template <int LANES, int V, int MODE, bool BIG, typename B>
 __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, LANES, BIG>& team,
-                                           Columns<LANES, V, VEC>& c) {
+                                           Columns<LANES, V, MODE>& c) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     team.scratch = scratch;
     team.cluster = BIG ? p.cluster : 1;
@@ -379,14 +376,14 @@ __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScr
         team.team = p.teams_per_block == 1 ? 0 : warp / p.warps;
         team.warp = warp - team.team * p.warps;
         team.lane = lane;
-        c.col = (team.rank * p.warps + team.warp) * V * kPackGroup + (VEC ? 4 * lane : lane);
+        c.col = (team.rank * p.warps + team.warp) * V * kPackGroup + (MODE != kScalar ? 4 * lane : lane);
         id = group * p.teams_per_block + team.team;
     } else {
         team.warps = 1;
         team.team = 0;
         team.warp = 0;
         team.lane = lane & (LANES - 1);
-        c.col = VEC ? 4 * team.lane : team.lane;
+        c.col = MODE != kScalar ? 4 * team.lane : team.lane;
         id = group * p.teams_per_block + threadIdx.x / LANES;
     }
     c.width = width;
@@ -396,8 +393,8 @@ __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScr
 
 // Codes of a thread's elements and the scales of their groups.  A group is a warp's chunk, or with fewer lanes 32 / LANES
 // chunks of the same threads.  Each lane forms the scale and its reciprocal of one group only.
-template <typename B, int LANES, int V, bool VEC>
-__device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], const Columns<LANES, V, VEC>& c, bool write,
+template <typename B, int LANES, int V, int MODE>
+__device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], const Columns<LANES, V, MODE>& c, bool write,
                                           uint8_t* codes, B* scales, int lane) {
     constexpr int kTogether = 32 / LANES < V ? 32 / LANES : V, kGroups = V / kTogether;
     using Bits = typename AbsBits<B>::type;
@@ -413,7 +410,7 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], con
         if (kGroups == 1 || lane % kGroups == i) mine = top;
     }
     const B scale = pack_scale<B>(format, AbsBits<B>::back(mine)), inverse = pack_inverse<B>(scale);
-    const int first = (c.col - (VEC ? 4 * lane : lane)) / kPackGroup;          // the warp's first group
+    const int first = (c.col - (MODE != kScalar ? 4 * lane : lane)) / kPackGroup;          // the warp's first group
     if (write && lane < kGroups && (first + lane) * kPackGroup < c.width) scales[first + lane] = scale;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
@@ -428,19 +425,19 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], con
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
-template <typename S, int LANES, int V, bool VEC, bool BRANCH, bool BIG>
+template <typename S, int LANES, int V, int MODE, bool BRANCH, bool BIG>
 __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, BIG, sizeof(S) == 8))
     ring_forward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p) {
     using B = Br<S>;
     constexpr int T = ring_threads(BIG);
-    using FS = Feed<S, LANES, V, VEC, T>;
-    using FB = Feed<B, LANES, V, VEC, T>;
+    using FS = Feed<S, LANES, V, MODE, T>;
+    using FB = Feed<B, LANES, V, MODE, T>;
     constexpr int at_y = FS::kBytes, at_gate = at_y + FB::kBytes;
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
-    Columns<LANES, V, VEC> c;
-    const uint32_t id = set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c);
+    Columns<LANES, V, MODE> c;
+    const uint32_t id = set_up<LANES, V, MODE, BIG, B>(p, (int)a.width, &scratch, team, c);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const bool row_gate = BRANCH && a.gate && !p.shared;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
@@ -501,14 +498,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
         span = first / (uint32_t)a.gate_rows;
         span_end = first;
     }
-    uint32_t ahead = first;
-    for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
+    issue(first, 0);
     int stage = 0;
     Four<B> t[V];                                           // act(gate) of a shared gate
     // every team makes the same number of steps: teams that share a warp meet in its shuffles
-    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
-        issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
-        copies_wait_oldest(p.stages);
+    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, stage ^= 1) {
+        issue(row + next, stage ^ 1);
+        copies_wait<1>();                                   // all but the newest group
         const bool live = row < last;
         if (LANES == 32 && !live) break;                    // a whole team, alone in its warps
         const char* at = ring + stage * p.stage_bytes;
@@ -582,27 +578,26 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
                     put(static_cast<B*>(a.h) + dense, c, j, o[j]);
                 }
         }
-        stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
     copies_wait<0>();
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
-template <typename S, int LANES, int V, bool VEC, bool BRANCH, bool NEXT, bool BIG>
+template <typename S, int LANES, int V, int MODE, bool BRANCH, bool NEXT, bool BIG>
 __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, BIG, sizeof(S) == 8))
     ring_backward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p,
                          const __grid_constant__ BackwardSlabs slabs) {
     using B = Br<S>;
     constexpr int T = ring_threads(BIG);
-    using FS = Feed<S, LANES, V, VEC, T>;
-    using FB = Feed<B, LANES, V, VEC, T>;
-    using FQ = Feed<uint8_t, LANES, V, VEC, T>;
-    using At = BackwardStage<NEXT, BRANCH, V, T, VEC, (int)sizeof(S), (int)sizeof(B)>;
+    using FS = Feed<S, LANES, V, MODE, T>;
+    using FB = Feed<B, LANES, V, MODE, T>;
+    using FQ = Feed<uint8_t, LANES, V, MODE, T>;
+    using At = BackwardStage<NEXT, BRANCH, V, T, MODE != kScalar, (int)sizeof(S), (int)sizeof(B)>;
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
-    Columns<LANES, V, VEC> c;
-    const uint32_t id = set_up<LANES, V, VEC, BIG, B>(p, (int)a.width, &scratch, team, c);
+    Columns<LANES, V, MODE> c;
+    const uint32_t id = set_up<LANES, V, MODE, BIG, B>(p, (int)a.width, &scratch, team, c);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const bool row_gate = BRANCH && (a.gate || a.gate_codes) && !p.shared;
@@ -629,7 +624,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
             for (int j = 0; j < V; ++j)
                 if (c.at(j, 0) < D) copy_async<sizeof(B)>(dst + j * T * (uint32_t)sizeof(B), from + j * 4 * LANES / kPackGroup);
         } else {
-            Feed<E, LANES, V, VEC, T>::issue(at, row_at(values, row, stride), c);
+            Feed<E, LANES, V, MODE, T>::issue(at, row_at(values, row, stride), c);
         }
     };
     const auto take_kept = [&](const char* at, const void* codes, auto* values, int64_t stride, uint32_t row, int j) {
@@ -639,7 +634,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
             const B s = c.at(j, 0) < D ? *reinterpret_cast<const B*>(at + 4 * V * T + (j * T + threadIdx.x) * sizeof(B)) : B(0);
             return decode4<B>(a.checkpoint, *reinterpret_cast<const uint32_t*>(&q), s);
         }
-        return widen4<E>(Feed<E, LANES, V, VEC, T>::take(at, row_at(values, row, stride), c, j));
+        return widen4<E>(Feed<E, LANES, V, MODE, T>::take(at, row_at(values, row, stride), c, j));
     };
     const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
                    last = p.shared ? min(first + p.rows_per_team, rows) : rows;
@@ -670,12 +665,11 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
         span_first = span * (uint32_t)a.gate_rows;
         span_end = span_first + (uint32_t)a.gate_rows;
     }
-    uint32_t ahead = first;
-    for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
+    issue(first, 0);
     int stage = 0;
-    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
-        issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
-        copies_wait_oldest(p.stages);
+    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, stage ^= 1) {
+        issue(row + next, stage ^ 1);
+        copies_wait<1>();                                   // all but the newest group
         const bool live = row < last;
         if (LANES == 32 && !live) break;
         const char* at = ring + stage * p.stage_bytes;
@@ -792,7 +786,6 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
                 }
             }
         }
-        stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
     copies_wait<0>();
 
@@ -833,7 +826,7 @@ namespace kanb200 {
 
 template <typename... P>
 cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...), const P&... args) {
-    const int bytes = p.stages * p.stage_bytes;
+    const int bytes = 2 * p.stage_bytes;
     cudaError_t e = cudaSuccess;
     if (bytes > 48 * 1024 - (int)sizeof(TeamScratch))
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -854,38 +847,48 @@ cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...)
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename S, int LANES, bool VEC, bool BIG>
+template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_forward_as(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st) {
     constexpr int V = ring_chunks(false, true, sizeof(S) == 8);
-    return a.y ? ring_launch(p, st, ring_forward_kernel<S, LANES, V, VEC, true, BIG>, a, p)
-               : ring_launch(p, st, ring_forward_kernel<S, LANES, V, VEC, false, BIG>, a, p);
+    return a.y ? ring_launch(p, st, ring_forward_kernel<S, LANES, V, MODE, true, BIG>, a, p)
+               : ring_launch(p, st, ring_forward_kernel<S, LANES, V, MODE, false, BIG>, a, p);
 }
-template <typename S, int LANES, bool VEC, bool BIG>
+template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_backward_as(const kanb200_block_args& a, const RingPlan& p, const BackwardSlabs& slabs, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
     if (!a.has_branch)
-        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, false, f64), VEC, false, true, BIG>,
+        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, false, f64), MODE, false, true, BIG>,
                            a, p, slabs);
-    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), VEC, true, true, BIG>,
+    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), MODE, true, true, BIG>,
                               a, p, slabs)
-                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), VEC, true, false, BIG>,
+                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), MODE, true, false, BIG>,
                               a, p, slabs);
 }
 
-#define KANB200_RING_DISPATCH(name, ...)                                                                    \
-    if (p.big) return p.vec ? name<S, 32, true, true>(__VA_ARGS__) : name<S, 32, false, true>(__VA_ARGS__);       \
-    if (p.lanes == 32) return p.vec ? name<S, 32, true, false>(__VA_ARGS__) : name<S, 32, false, false>(__VA_ARGS__); \
-    if (p.lanes == 16) return p.vec ? name<S, 16, true, false>(__VA_ARGS__) : name<S, 16, false, false>(__VA_ARGS__); \
-    if (p.lanes == 8) return p.vec ? name<S, 8, true, false>(__VA_ARGS__) : name<S, 8, false, false>(__VA_ARGS__);    \
-    return p.vec ? name<S, 4, true, false>(__VA_ARGS__) : name<S, 4, false, false>(__VA_ARGS__)
+// name<S, LANES, MODE, BIG>(...) for the plan's lanes and mode
+#define KANB200_RING_MODE(name, lanes, big, ...)                                              \
+    switch (p.mode) {                                                                         \
+        case kFull: return name<S, lanes, kFull, big>(__VA_ARGS__);                           \
+        case kVector: return name<S, lanes, kVector, big>(__VA_ARGS__);                       \
+        default: return name<S, lanes, kScalar, big>(__VA_ARGS__);                            \
+    }
+#define KANB200_RING_DISPATCH(name, ...)                                                      \
+    if (p.big) KANB200_RING_MODE(name, 32, true, __VA_ARGS__)                                 \
+    switch (p.lanes) {                                                                        \
+        case 32: KANB200_RING_MODE(name, 32, false, __VA_ARGS__)                              \
+        case 16: KANB200_RING_MODE(name, 16, false, __VA_ARGS__)                              \
+        case 8: KANB200_RING_MODE(name, 8, false, __VA_ARGS__)                                \
+        default: KANB200_RING_MODE(name, 4, false, __VA_ARGS__)                               \
+    }
 
 template <typename S> cudaError_t ring_forward(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st) {
-    KANB200_RING_DISPATCH(ring_forward_as, a, p, st);
+    KANB200_RING_DISPATCH(ring_forward_as, a, p, st)
 }
 template <typename S>
 cudaError_t ring_backward(const kanb200_block_args& a, const RingPlan& p, const BackwardSlabs& slabs, cudaStream_t st) {
-    KANB200_RING_DISPATCH(ring_backward_as, a, p, slabs, st);
+    KANB200_RING_DISPATCH(ring_backward_as, a, p, slabs, st)
 }
 #undef KANB200_RING_DISPATCH
+#undef KANB200_RING_MODE
 
 }  // namespace kanb200
