@@ -47,167 +47,6 @@ template <int LANES, int V, int MODE> struct Columns {
     __device__ __forceinline__ bool ok(int j, int e) const { return MODE == kFull || at(j, MODE == kScalar ? e : 0) < width; }
 };
 
-// ---- four elements --------------------------------------------------------------------------------------------------
-template <typename T> struct alignas(4 * sizeof(T) > 16 ? 16 : 4 * sizeof(T)) Quad {
-    T v[4];
-};
-template <typename T> __device__ __forceinline__ Quad<T> load_quad(const T* p) {
-    Quad<T> q;
-    if constexpr (sizeof(T) == 8) {
-        reinterpret_cast<float4*>(&q)[0] = reinterpret_cast<const float4*>(p)[0];
-        reinterpret_cast<float4*>(&q)[1] = reinterpret_cast<const float4*>(p)[1];
-    } else {
-        q = *reinterpret_cast<const Quad<T>*>(p);
-    }
-    return q;
-}
-template <typename T> __device__ __forceinline__ void store_quad(T* p, const Quad<T>& q) {
-    if constexpr (sizeof(T) == 8) {
-        reinterpret_cast<float4*>(p)[0] = reinterpret_cast<const float4*>(&q)[0];
-        reinterpret_cast<float4*>(p)[1] = reinterpret_cast<const float4*>(&q)[1];
-    } else {
-        *reinterpret_cast<Quad<T>*>(p) = q;
-    }
-}
-
-// Four values in the branch's type; float works on pairs (sm_100's two-element FMA pipe instructions).
-template <typename B> struct alignas(16) Four {
-    B v[4];
-};
-template <typename B> __device__ __forceinline__ Four<B> four(B s) { return {{s, s, s, s}}; }
-__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void split_pair(unsigned long long p, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
-}
-#define KANB200_PAIRWISE(name, instruction)                                                                          \
-    __device__ __forceinline__ Four<float> name(const Four<float>& x, const Four<float>& y) {                        \
-        Four<float> r;                                                                                               \
-        _Pragma("unroll") for (int e = 0; e < 4; e += 2) {                                                           \
-            unsigned long long p;                                                                                    \
-            asm(instruction " %0, %1, %2;" : "=l"(p) : "l"(pair_of(x.v[e], x.v[e + 1])), "l"(pair_of(y.v[e], y.v[e + 1]))); \
-            split_pair(p, r.v[e], r.v[e + 1]);                                                                       \
-        }                                                                                                            \
-        return r;                                                                                                    \
-    }
-KANB200_PAIRWISE(operator+, "add.rn.f32x2")
-KANB200_PAIRWISE(operator*, "mul.rn.f32x2")
-#undef KANB200_PAIRWISE
-// x y + z, rounded once
-__device__ __forceinline__ Four<float> fma4(const Four<float>& x, const Four<float>& y, const Four<float>& z) {
-    Four<float> r;
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-        unsigned long long p;
-        asm("fma.rn.f32x2 %0, %1, %2, %3;"
-            : "=l"(p)
-            : "l"(pair_of(x.v[e], x.v[e + 1])), "l"(pair_of(y.v[e], y.v[e + 1])), "l"(pair_of(z.v[e], z.v[e + 1])));
-        split_pair(p, r.v[e], r.v[e + 1]);
-    }
-    return r;
-}
-__device__ __forceinline__ Four<double> operator+(const Four<double>& x, const Four<double>& y) {
-    return {{x.v[0] + y.v[0], x.v[1] + y.v[1], x.v[2] + y.v[2], x.v[3] + y.v[3]}};
-}
-__device__ __forceinline__ Four<double> operator*(const Four<double>& x, const Four<double>& y) {
-    return {{x.v[0] * y.v[0], x.v[1] * y.v[1], x.v[2] * y.v[2], x.v[3] * y.v[3]}};
-}
-__device__ __forceinline__ Four<double> fma4(const Four<double>& x, const Four<double>& y, const Four<double>& z) {
-    return {{fma(x.v[0], y.v[0], z.v[0]), fma(x.v[1], y.v[1], z.v[1]), fma(x.v[2], y.v[2], z.v[2]), fma(x.v[3], y.v[3], z.v[3])}};
-}
-template <typename B> __device__ __forceinline__ B total(const Four<B>& x) { return (x.v[0] + x.v[2]) + (x.v[1] + x.v[3]); }
-
-template <typename S> __device__ __forceinline__ Four<Br<S>> widen4(const Quad<S>& q) {
-    return {{widen(q.v[0]), widen(q.v[1]), widen(q.v[2]), widen(q.v[3])}};
-}
-template <typename S> __device__ __forceinline__ Quad<S> narrow4(const Four<Br<S>>& x) {
-    Quad<S> q;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q.v[e] = narrow<S>(x.v[e]);
-    return q;
-}
-template <> __device__ __forceinline__ Quad<__nv_bfloat16> narrow4<__nv_bfloat16>(const Four<float>& x) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x.v[0], x.v[1]), b = __floats2bfloat162_rn(x.v[2], x.v[3]);
-    return {{a.x, a.y, b.x, b.y}};
-}
-template <> __device__ __forceinline__ Quad<__half> narrow4<__half>(const Four<float>& x) {
-    const __half2 a = __floats2half2_rn(x.v[0], x.v[1]), b = __floats2half2_rn(x.v[2], x.v[3]);
-    return {{a.x, a.y, b.x, b.y}};
-}
-
-template <typename B> __device__ __forceinline__ Four<B> sigmoid4(const Four<B>& g) {
-    return {{gate_sigmoid(g.v[0]), gate_sigmoid(g.v[1]), gate_sigmoid(g.v[2]), gate_sigmoid(g.v[3])}};
-}
-template <typename B> __device__ __forceinline__ Four<B> gate4(int act, const Four<B>& g) {
-    if (act == kActNone) return g;
-    const Four<B> s = sigmoid4(g);
-    return act == kActSigmoid ? s : g * s;
-}
-// activation and derivative: sigmoid s, s (1 - s);  silu g s, s + g s (1 - s)
-template <typename B> __device__ __forceinline__ void gate4_grad(int act, const Four<B>& g, Four<B>& a, Four<B>& da) {
-    a = g;
-    da = four<B>(B(1));
-    if (act == kActNone) return;
-    const Four<B> s = sigmoid4(g), rest = fma4(s, four<B>(B(-1)), four<B>(B(1)));
-    a = act == kActSigmoid ? s : g * s;
-    da = act == kActSigmoid ? s * rest : fma4(a, rest, s);
-}
-
-// Codes of four elements as one word, lowest byte first.  int8 without conversions: the byte becomes the mantissa of
-// 2^23 + 128 + code, and back by adding 1.5 * 2^23, which leaves the rounded integer in the low bits.
-template <typename B> __device__ __forceinline__ Four<B> decode4(int format, uint32_t word, B scale);
-template <> __device__ __forceinline__ Four<float> decode4<float>(int format, uint32_t word, float scale) {
-    Four<float> r;
-    if (format == kPackInt8) {
-        const uint32_t w = word ^ 0x80808080u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r.v[e] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + e));
-        r = r + four<float>(-8388736.0f);
-    } else {
-        const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word & 0xffffu), __NV_E4M3));
-        const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word >> 16), __NV_E4M3));
-        const float2 fa = __half22float2(a), fb = __half22float2(b);
-        r = {{fa.x, fa.y, fb.x, fb.y}};
-    }
-    return r * four<float>(scale);
-}
-template <> __device__ __forceinline__ Four<double> decode4<double>(int format, uint32_t word, double scale) {
-    Four<double> r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r.v[e] = from_code<double>(format, word >> 8 * e & 0xffu, scale);
-    return r;
-}
-// |x / scale| is at most 127 (1 + 2^-21) by the choice of the scale, so rounding cannot leave the codes' range.  The product
-// is rounded before it is rounded to a code (the definition; the pairwise instructions above would be merged into one
-// multiply-add, which turns 63.49999952 into 63 where the float product is 63.5).
-__device__ __forceinline__ uint32_t encode4(int format, const Four<float>& x, float inv) {
-    float q[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = __fmul_rn(x.v[e], inv);
-    uint32_t word;
-    if (format == kPackInt8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = __fadd_rn(q[e], 12582912.0f);
-        const uint32_t a = __byte_perm(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x0040);
-        const uint32_t b = __byte_perm(__float_as_uint(q[2]), __float_as_uint(q[3]), 0x0040);
-        word = __byte_perm(a, b, 0x5410);
-    } else {
-        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
-        word = a | b << 16;
-    }
-    return inv == 0.0f ? 0u : word;                          // a group that is not finite
-}
-__device__ __forceinline__ uint32_t encode4(int format, const Four<double>& x, double inv) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) word |= to_code(format, x.v[e], inv) << 8 * e;
-    return word;
-}
-
 // ---- rows <-> registers -----------------------------------------------------------------------------------------------
 // A thread's elements of one tensor on their way from a row in memory to registers.  Types of less than 4 bytes that
 // cannot be copied four at a time have no ring slot: they are loaded where they are used.  T is the block's most threads:

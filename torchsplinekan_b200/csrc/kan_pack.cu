@@ -1,5 +1,8 @@
 // 8-bit checkpoints of activations: pack (codes and one scale per 128 columns of a row) and unpack.
-// Bandwidth bounds both: 4 + 1.03 bytes per float32 element in either direction.
+//
+// Bandwidth bounds both: 4 + 1.03 bytes per float32 element in either direction.  A warp takes kRun groups one after the
+// other in the order of (row, group), so that every lane has kRun 16-byte loads under way and forms the scale and its
+// reciprocal (a division) of one group only; narrow rows share a warp.
 #include "kan_block.cuh"
 
 #include <algorithm>
@@ -7,76 +10,183 @@
 namespace kanb200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kRun = 4;
 
-// A warp per group of 128 columns.
-template <typename S>
+// Where a run of kRun chunks lies.  LANES lanes share a row's group (fewer than 32: rows of up to 4 LANES columns, one
+// group, 32 / LANES rows to a chunk).
+template <int LANES, bool VEC> struct Run {
+    int64_t row, rows;
+    int group, groups, lane, width;
+
+    __device__ __forceinline__ Run(int64_t rows_, int width_) : rows(rows_), width(width_) {
+        const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+        lane = threadIdx.x & (LANES - 1);
+        if (LANES == 32) {
+            groups = (width + kPackGroup - 1) / kPackGroup;
+            const int64_t first = warp * kRun;
+            row = first / groups;
+            group = (int)(first - row * groups);
+        } else {
+            groups = 1;
+            group = 0;
+            row = warp * kRun * (32 / LANES) + (threadIdx.x & 31) / LANES;
+        }
+    }
+    __device__ __forceinline__ void next() {
+        if (LANES < 32) {
+            row += 32 / LANES;
+        } else if (++group == groups) {
+            group = 0;
+            ++row;
+        }
+    }
+    __device__ __forceinline__ int column(int e) const { return group * kPackGroup + (VEC ? 4 * lane + e : lane + LANES * e); }
+    __device__ __forceinline__ bool ok(int e) const { return row < rows && column(VEC ? 0 : e) < width; }
+    __device__ __forceinline__ int64_t scale_at() const { return row * groups + group; }
+};
+
+template <typename S, int LANES, bool VEC>
 __global__ void __launch_bounds__(kThreads) pack_kernel(int format, const S* __restrict__ x, int64_t x_stride,
                                                        uint8_t* __restrict__ codes, Br<S>* __restrict__ scales,
-                                                       int64_t rows, int64_t width) {
+                                                       int64_t rows, int width) {
     using B = Br<S>;
-    const int lane = threadIdx.x & 31;
-    const int64_t groups = (width + kPackGroup - 1) / kPackGroup, total = rows * groups;
-    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < total;
-         i += (int64_t)gridDim.x * (kThreads / 32)) {
-        const int64_t row = i / groups, first = (i - row * groups) * kPackGroup;
-        B v[4];
-        typename AbsBits<B>::type top = 0;
+    using Bits = typename AbsBits<B>::type;
+    Four<B> v[kRun];
+    {
+        Run<LANES, VEC> r(rows, width);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t c = first + e * 32 + lane;
-            v[e] = c < width ? widen(x[row * x_stride + c]) : B(0);
-            top = max(top, AbsBits<B>::of(v[e]));
-        }
-        const B scale = pack_scale<B>(format, AbsBits<B>::back(lanes_max<32>(top))), inv = pack_inverse<B>(scale);
+        for (int i = 0; i < kRun; ++i, r.next()) {
+            Quad<S> q{};
+            if constexpr (VEC) {
+                if (r.ok(0)) q = load_quad(x + r.row * x_stride + r.column(0));
+            } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t c = first + e * 32 + lane;
-            if (c < width) codes[row * width + c] = (uint8_t)to_code(format, v[e], inv);
+                for (int e = 0; e < 4; ++e)
+                    if (r.ok(e)) q.v[e] = x[r.row * x_stride + r.column(e)];
+            }
+            v[i] = widen4<S>(q);
         }
-        if (lane == 0) scales[i] = scale;
+    }
+    Run<LANES, VEC> r(rows, width);
+    Bits mine = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        Bits top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, AbsBits<B>::of(v[i].v[e]));
+        top = lanes_max<LANES>(top);
+        if (r.lane % kRun == i) mine = top;
+    }
+    const B scale = pack_scale<B>(format, AbsBits<B>::back(mine)), inverse = pack_inverse<B>(scale);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i, r.next()) {
+        const B inv = __shfl_sync(0xffffffffu, inverse, i, LANES);
+        if (r.lane == i && r.row < rows) scales[r.scale_at()] = scale;
+        const uint32_t word = encode4(format, v[i], inv);
+        uint8_t* at = codes + r.row * width + r.column(0);
+        if constexpr (VEC) {
+            if (r.ok(0)) *reinterpret_cast<uint32_t*>(at) = word;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r.ok(e)) at[LANES * e] = (uint8_t)(word >> 8 * e);
+        }
     }
 }
 
-template <typename S>
+template <typename S, int LANES, bool VEC>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(int format, const uint8_t* __restrict__ codes,
                                                          const Br<S>* __restrict__ scales, S* __restrict__ x,
-                                                         int64_t rows, int64_t width) {
+                                                         int64_t rows, int width) {
     using B = Br<S>;
-    const int lane = threadIdx.x & 31;
-    const int64_t groups = (width + kPackGroup - 1) / kPackGroup, total = rows * groups;
-    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < total;
-         i += (int64_t)gridDim.x * (kThreads / 32)) {
-        const int64_t row = i / groups, first = (i - row * groups) * kPackGroup;
-        const B scale = scales[i];
+    uint32_t word[kRun];
+    B scale[kRun];
+    {
+        Run<LANES, VEC> r(rows, width);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t c = first + e * 32 + lane;
-            if (c < width) x[row * width + c] = narrow<S>(from_code<B>(format, codes[row * width + c], scale));
+        for (int i = 0; i < kRun; ++i, r.next()) {
+            const uint8_t* at = codes + r.row * width + r.column(0);
+            word[i] = 0;
+            if constexpr (VEC) {
+                if (r.ok(0)) word[i] = *reinterpret_cast<const uint32_t*>(at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (r.ok(e)) word[i] |= (uint32_t)at[LANES * e] << 8 * e;
+            }
+            scale[i] = r.row < rows ? scales[r.scale_at()] : B(0);
+        }
+    }
+    Run<LANES, VEC> r(rows, width);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i, r.next()) {
+        const Quad<S> q = narrow4<S>(decode4<B>(format, word[i], scale[i]));
+        S* at = x + r.row * width + r.column(0);
+        if constexpr (VEC) {
+            if (r.ok(0)) store_quad(at, q);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r.ok(e)) at[LANES * e] = q.v[e];
         }
     }
 }
 
-int grid_for(int64_t rows, int64_t width) {
-    const int64_t warps = rows * ((width + kPackGroup - 1) / kPackGroup);
-    return (int)std::min<int64_t>((warps + kThreads / 32 - 1) / (kThreads / 32), 148 * 64);
+struct Shape {
+    int lanes;
+    bool vec;
+    unsigned blocks;
+};
+// false: more blocks than a grid can have
+bool shape_of(int64_t rows, int64_t width, bool vec, Shape& s) {
+    s.lanes = width <= 16 ? 4 : width <= 32 ? 8 : width <= 64 ? 16 : 32;
+    s.vec = vec && width % 4 == 0;
+    const int64_t chunks = s.lanes == 32 ? rows * ((width + kPackGroup - 1) / kPackGroup) : (rows * s.lanes + 31) / 32;
+    const int64_t blocks = (chunks + kRun * (kThreads / 32) - 1) / (kRun * (kThreads / 32));
+    s.blocks = (unsigned)blocks;
+    return blocks < ((int64_t)1 << 31);
+}
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+template <typename S> constexpr size_t quad_alignment() { return 4 * sizeof(S) > 16 ? 16 : 4 * sizeof(S); }
+
+// body.template operator()<LANES, VEC>() for a shape
+template <typename F> void with_shape(const Shape& s, F body) {
+    const auto lanes = [&](auto l) {
+        if (s.vec) body(l, std::true_type{});
+        else body(l, std::false_type{});
+    };
+    switch (s.lanes) {
+        case 4: return lanes(std::integral_constant<int, 4>{});
+        case 8: return lanes(std::integral_constant<int, 8>{});
+        case 16: return lanes(std::integral_constant<int, 16>{});
+        default: return lanes(std::integral_constant<int, 32>{});
+    }
 }
 
 template <typename S>
 cudaError_t pack(int format, const void* x, int64_t x_stride, void* codes, void* scales, int64_t rows, int64_t width,
                  cudaStream_t st) {
-    pack_kernel<S><<<grid_for(rows, width), kThreads, 0, st>>>(format, static_cast<const S*>(x), x_stride,
-                                                               static_cast<uint8_t*>(codes), static_cast<Br<S>*>(scales),
-                                                               rows, width);
+    Shape s;
+    if (!shape_of(rows, width, x_stride % 4 == 0 && aligned(x, quad_alignment<S>()) && aligned(codes, 4), s))
+        return cudaErrorInvalidValue;
+    with_shape(s, [&](auto lanes, auto vec) {
+        pack_kernel<S, lanes, vec><<<s.blocks, kThreads, 0, st>>>(format, static_cast<const S*>(x), x_stride,
+                                                                  static_cast<uint8_t*>(codes), static_cast<Br<S>*>(scales),
+                                                                  rows, (int)width);
+    });
     return cudaGetLastError();
 }
 
 template <typename S>
 cudaError_t unpack(int format, const void* codes, const void* scales, void* x, int64_t rows, int64_t width,
                    cudaStream_t st) {
-    unpack_kernel<S><<<grid_for(rows, width), kThreads, 0, st>>>(format, static_cast<const uint8_t*>(codes),
-                                                                 static_cast<const Br<S>*>(scales), static_cast<S*>(x),
-                                                                 rows, width);
+    Shape s;
+    if (!shape_of(rows, width, aligned(x, quad_alignment<S>()) && aligned(codes, 4), s)) return cudaErrorInvalidValue;
+    with_shape(s, [&](auto lanes, auto vec) {
+        unpack_kernel<S, lanes, vec><<<s.blocks, kThreads, 0, st>>>(format, static_cast<const uint8_t*>(codes),
+                                                                    static_cast<const Br<S>*>(scales), static_cast<S*>(x),
+                                                                    rows, (int)width);
+    });
     return cudaGetLastError();
 }
 
