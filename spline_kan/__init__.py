@@ -18,7 +18,7 @@ import sys as _sys
 import torchsplinekan_b200 as _impl
 from torchsplinekan_b200 import _C, block, dense_backend, fused, kan, kan_linear, pruning
 from torchsplinekan_b200 import KAN, KANLinear, __version__
-from torchsplinekan_b200.block import block_norm, gated_residual, pack_activation, unpack_activation
+from torchsplinekan_b200.block import BlockNorm, GatedResidual, block_norm, gated_residual, pack_activation, unpack_activation
 from torchsplinekan_b200.pruning import PruneResult, prune_nodes
 
 reference_backend = dense_backend
@@ -29,5 +29,5 @@ for _name, _mod in (("_C", _C), ("reference_backend", dense_backend), ("block", 
     _sys.modules[f"{__name__}.{_name}"] = _mod
 del _name, _mod
 
-__all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "block_norm", "gated_residual",
+__all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "BlockNorm", "GatedResidual", "block_norm", "gated_residual",
            "pack_activation", "unpack_activation", "__version__"]

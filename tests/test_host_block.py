@@ -134,3 +134,32 @@ def test_c_abi_refuses_before_any_launch():
     assert pk(dtype=5) == pk(form=0) == pk(x=None) == pk(stride=-1) == pk(rows=-1) == pk(width=0) == _native.EINVAL
     assert pk(rows=0) == 0
     assert lib.kanb200_unpack_activation(0, 3, p, p, p, 4, 8, None) == _native.EINVAL
+
+
+def test_networks_of_blocks_on_the_dense_backend():
+    torch.manual_seed(1)
+    net = sk.KAN([6, 8, 8, 2], norm="rms", residual=True, gate="silu", activation_checkpoint="int8").double()
+    assert net.widths == [6, 8, 8, 2] and net.layers[1].out_features == 16
+    x = torch.randn(5, 6, dtype=torch.float64, requires_grad=True)
+    h = sk.block_norm(x, net.norms[0].weight)
+    h = net.layers[0](h)
+    y = net.layers[1](sk.block_norm(h, net.norms[1].weight))
+    c = net.connections["1"]
+    z = h + c.scale * torch.nn.functional.silu(y[:, 8:]) * sk.block_norm(y[:, :8].contiguous(), c.post_weight)
+    want = net.layers[2](sk.block_norm(z, net.norms[2].weight))
+    assert torch.allclose(net(x), want, atol=1e-12)
+    assert torch.autograd.gradcheck(lambda t: net(t), (x,))
+    frozen = net.export_inference()
+    assert torch.allclose(frozen(x), net(x), atol=1e-10) and not any(p.requires_grad for p in frozen.parameters())
+    y, reg = net.forward_with_regularization(x)
+    assert torch.allclose(y, net(x)) and torch.allclose(reg, net.regularization_loss(x=x))
+    plain = sk.KAN([6, 8, 2])
+    assert sorted(k for k, _ in plain.named_parameters()) == sorted(k for k, _ in sk.KAN.from_layers(list(plain.layers)).named_parameters())
+    for bad, words in ((dict(norm="batch"), "norm"), (dict(gate="silu"), "residual"), (dict(gate="relu", residual=True), "gate"),
+                       (dict(residual=True), "equal widths"), (dict(activation_checkpoint="int4"), "activation_checkpoint")):
+        with pytest.raises(ValueError, match=words):
+            sk.KAN([6, 8, 2], **bad)
+    with pytest.raises(ValueError, match="share eps"):
+        sk.GatedResidual(8)(torch.zeros(2, 8), torch.zeros(2, 8), sk.BlockNorm(8, eps=1e-3))
+    with pytest.raises(ValueError, match="chains"):
+        sk.KAN([4, 4, 4], residual=True).prune(torch.zeros(3, 4))

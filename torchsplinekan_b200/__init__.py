@@ -18,7 +18,7 @@ except ImportError as exc:            # no fallback: say how to build and stop
         "torchsplinekan_b200: the compiled operator layer (_C) or lib/libkan_b200.so is missing or stale; "
         "build them with `python torchsplinekan_b200/build.py` (needs nvcc and g++).  "
         f"This package has no fallback implementation.  [{exc}]") from exc
-from .block import block_norm, gated_residual, pack_activation, unpack_activation
+from .block import BlockNorm, GatedResidual, block_norm, gated_residual, pack_activation, unpack_activation
 from .kan_linear import KANLinear
 from .kan import KAN
 from .data_parallel import GradientBucket, HostBatchPrefetcher, global_edge_means, shard_rows
@@ -27,5 +27,5 @@ from .pruning import PruneResult, prune_nodes
 __version__ = "0.1.0"
 
 __all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "GradientBucket", "HostBatchPrefetcher", "shard_rows", "global_edge_means",
-           "block_norm", "gated_residual", "pack_activation", "unpack_activation",
+           "BlockNorm", "GatedResidual", "block_norm", "gated_residual", "pack_activation", "unpack_activation",
            "__version__"]

@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.nn as nn
 
 from . import _C
 
@@ -93,3 +94,48 @@ def pack_activation(x: torch.Tensor, format: str = "int8") -> Tuple[torch.Tensor
 def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``codes * scales`` in ``dtype`` (default: the type of the scales)."""
     return _C.unpack_activation(codes, scales, scales.dtype if dtype is None else dtype)
+
+
+class BlockNorm(nn.Module):
+    """:func:`block_norm` with its parameters: weight (ones) and, for "layer", bias (zeros)."""
+
+    def __init__(self, width: int, kind: str = "rms", eps: float = 1e-6, checkpoint: Optional[str] = None) -> None:
+        super().__init__()
+        if _code(NORMS, "kind", kind) == 0:
+            raise ValueError("kind must be 'rms' or 'layer', got None")
+        _code(CHECKPOINTS, "checkpoint", checkpoint)
+        self.kind, self.eps, self.checkpoint = kind, eps, checkpoint
+        self.weight = nn.Parameter(torch.ones(width))
+        self.bias = nn.Parameter(torch.zeros(width)) if kind == "layer" else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return block_norm(x, self.weight, self.bias, kind=self.kind, eps=self.eps,
+                          checkpoint=self.checkpoint if x.is_cuda else None)
+
+
+class GatedResidual(nn.Module):
+    """:func:`gated_residual` with its parameters: scale (``scale_init``) and those of the post norm.
+
+    ``gate``: None, "sigmoid" or "silu": the activation of the second half of ``y``, which then holds value and gate side
+    by side.  ``next_norm``: the :class:`BlockNorm` of the next block, fused into the same pass."""
+
+    def __init__(self, width: int, gate: Optional[str] = None, post_norm: Optional[str] = "rms", scale_init: float = 1.0,
+                 eps: float = 1e-6, checkpoint: Optional[str] = None) -> None:
+        super().__init__()
+        _code(GATE_ACTIVATIONS, "gate", gate)
+        _code(NORMS, "post_norm", post_norm)
+        _code(CHECKPOINTS, "checkpoint", checkpoint)
+        self.gate, self.post_norm, self.eps, self.checkpoint = gate, post_norm, eps, checkpoint
+        self.scale = nn.Parameter(torch.full((width,), float(scale_init)))
+        self.post_weight = nn.Parameter(torch.ones(width)) if post_norm is not None else None
+        self.post_bias = nn.Parameter(torch.zeros(width)) if post_norm == "layer" else None
+
+    def forward(self, x: torch.Tensor, y: torch.Tensor, next_norm: Optional[BlockNorm] = None):
+        if next_norm is not None and next_norm.eps != self.eps:
+            raise ValueError(f"the norms of one connection share eps, got {self.eps} and {next_norm.eps}")
+        return gated_residual(x, y, gate="packed" if self.gate else None, gate_activation=self.gate, scale=self.scale,
+                              post_norm=self.post_norm, post_weight=self.post_weight, post_bias=self.post_bias,
+                              next_norm=next_norm.kind if next_norm is not None else None,
+                              next_weight=next_norm.weight if next_norm is not None else None,
+                              next_bias=next_norm.bias if next_norm is not None else None, eps=self.eps,
+                              checkpoint=self.checkpoint if x.is_cuda else None)

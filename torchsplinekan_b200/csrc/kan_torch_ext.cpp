@@ -791,35 +791,76 @@ struct KANFunction : public torch::autograd::Function<KANFunction> {
                      &spline_scaler = saved[4];
         const int64_t k = ctx->saved_data["order"].toInt();
         const bool has_scaler = ctx->saved_data["has_scaler"].toBool();
-        const bool allow_sink = ctx->saved_data["allow_sink"].toBool();
-        const bool has_base = has(base_weight);
-        const Tensor& D = grad_outputs[0];
-        Tensor gx, gb, gs, gc;
         if (at::GradMode::is_enabled()) {
+            Tensor gx, gb, gs, gc;
             std::tie(gx, gb, gs, gc) =
-                kan_backward_composite(D, x, grid, base_weight, spline_weight, spline_scaler, k, has_scaler);
-        } else {
-            const bool need_x = ctx->needs_input_grad(0);
-            const bool need_base = ctx->needs_input_grad(2) && has_base;
-            const bool need_spline = ctx->needs_input_grad(3) || (has_scaler && ctx->needs_input_grad(4));
-            bool sunk = false;
-            bool any_sink;
-            {
-                std::lock_guard<std::mutex> lock(g_sink_mutex);
-                any_sink = !g_sinks.empty();
-            }
-            if (any_sink && allow_sink)
-                sunk = sink_backward(need_x, ctx->needs_input_grad(2), ctx->needs_input_grad(3),
-                                     ctx->needs_input_grad(4), D, x, grid, base_weight, spline_weight, spline_scaler, k,
-                                     has_scaler, gx);
-            if (sunk) return {gx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-            Grads g = backward_impl(D, x, grid, base_weight, spline_weight, spline_scaler, k, has_scaler, need_x,
-                                    need_base, need_spline);
-            gx = g.gx; gb = g.gb; gs = g.gs; gc = g.gc;
+                kan_backward_composite(grad_outputs[0], x, grid, base_weight, spline_weight, spline_scaler, k, has_scaler);
+            return {gx, Tensor(), has(base_weight) ? gb : Tensor(), gs, has_scaler ? gc : Tensor(), Tensor(), Tensor()};
         }
-        return {gx, Tensor(), has_base ? gb : Tensor(), gs, has_scaler ? gc : Tensor(), Tensor(), Tensor()};
+        return native_backward(ctx, grad_outputs[0], x, grid, base_weight, spline_weight, spline_scaler, k, has_scaler);
+    }
+
+    // Gradients from the native kernels, those that are not needed left out; slots of the seven inputs of apply.
+    static torch::autograd::variable_list native_backward(torch::autograd::AutogradContext* ctx, const Tensor& D,
+                                                          const Tensor& x, const Tensor& grid, const Tensor& base_weight,
+                                                          const Tensor& spline_weight, const Tensor& spline_scaler,
+                                                          int64_t k, bool has_scaler) {
+        const bool has_base = has(base_weight);
+        const bool need_x = ctx->needs_input_grad(0);
+        const bool need_base = ctx->needs_input_grad(2) && has_base;
+        const bool need_spline = ctx->needs_input_grad(3) || (has_scaler && ctx->needs_input_grad(4));
+        bool any_sink;
+        {
+            std::lock_guard<std::mutex> lock(g_sink_mutex);
+            any_sink = !g_sinks.empty();
+        }
+        if (any_sink && ctx->saved_data["allow_sink"].toBool()) {
+            Tensor gx;
+            if (sink_backward(need_x, ctx->needs_input_grad(2), ctx->needs_input_grad(3), ctx->needs_input_grad(4), D, x,
+                              grid, base_weight, spline_weight, spline_scaler, k, has_scaler, gx))
+                return {gx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        }
+        Grads g = backward_impl(D, x, grid, base_weight, spline_weight, spline_scaler, k, has_scaler, need_x, need_base,
+                                need_spline);
+        return {g.gx, Tensor(), has_base ? g.gb : Tensor(), g.gs, has_scaler ? g.gc : Tensor(), Tensor(), Tensor()};
     }
 };
+
+// The same layer with its input kept for the backward as 8-bit codes (kanb200_pack_activation) instead of itself: the
+// backward restores it into memory that lives for that call only.
+struct KANCheckpointedFunction : public torch::autograd::Function<KANCheckpointedFunction> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& grid,
+                          const Tensor& base_weight, const Tensor& spline_weight, const Tensor& spline_scaler,
+                          int64_t spline_order, bool has_scaler, int64_t format) {
+        ctx->saved_data["order"] = spline_order;
+        ctx->saved_data["has_scaler"] = has_scaler;
+        ctx->saved_data["allow_sink"] = g_sinks_disabled.load() == 0;
+        Tensor y = forward_impl(x, grid, base_weight, spline_weight, spline_scaler, spline_order, has_scaler);
+        const kan_ext::Packed p = kan_ext::pack_rows(x, (int)format);
+        ctx->save_for_backward({p.codes, p.scales, grid, base_weight, spline_weight, spline_scaler});
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grad_outputs) {
+        const auto saved = ctx->get_saved_variables();
+        TORCH_CHECK(!at::GradMode::is_enabled(),
+                    "KANLinear: create_graph=True needs the layer's input itself, not its 8-bit checkpoint");
+        const Tensor x = kan_ext::unpack_rows(saved[0], saved[1], saved[4].scalar_type());
+        auto grads = KANFunction::native_backward(ctx, grad_outputs[0], x, saved[2], saved[3], saved[4], saved[5],
+                                                  ctx->saved_data["order"].toInt(),
+                                                  ctx->saved_data["has_scaler"].toBool());
+        grads.emplace_back();
+        return grads;
+    }
+};
+
+Tensor kan_apply_checkpointed(const Tensor& x, const Tensor& grid, const Tensor& base_weight, const Tensor& spline_weight,
+                              const Tensor& spline_scaler, int64_t spline_order, bool has_scaler, int64_t format) {
+    TORCH_CHECK(format == KANB200_PACK_INT8 || format == KANB200_PACK_E4M3, "kan_apply_checkpointed: unknown format");
+    return KANCheckpointedFunction::apply(x, grid, base_weight, spline_weight, spline_scaler, spline_order, has_scaler,
+                                          format);
+}
 
 Tensor kan_apply(const Tensor& x, const Tensor& grid, const Tensor& base_weight, const Tensor& spline_weight,
                  const Tensor& spline_scaler, int64_t spline_order, bool has_scaler) {
@@ -924,6 +965,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("kan_apply", &kan_apply, py::arg("x"), py::arg("grid"), py::arg("base_weight"), py::arg("spline_weight"),
           py::arg("spline_scaler"), py::arg("spline_order"), py::arg("has_scaler"),
           "autograd-aware forward; the call KANLinear uses");
+    m.def("kan_apply_checkpointed", &kan_apply_checkpointed, py::arg("x"), py::arg("grid"), py::arg("base_weight"),
+          py::arg("spline_weight"), py::arg("spline_scaler"), py::arg("spline_order"), py::arg("has_scaler"),
+          py::arg("format"), "kan_apply that keeps x for the backward as 8-bit codes");
     m.def("kan_backward_composite",
           [](const Tensor& go, const Tensor& x, const Tensor& grid, const Tensor& bw, const Tensor& sw, const Tensor& sc,
              int64_t order, bool has_scaler) {

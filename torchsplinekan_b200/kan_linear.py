@@ -14,6 +14,7 @@ import torch.nn.functional as F
 
 from . import _C
 from . import fused as _fused
+from .block import CHECKPOINTS
 from .dense_backend import (ReferenceKANLayer, compute_basis, curve2coeff, edge_abs_mean_dense, fit_spline_coeffs,
                             regularization_from_edge_means)
 
@@ -44,12 +45,20 @@ class KANLinear(nn.Module):
     The native kernels fuse SiLU; any other base activation is evaluated with
     PyTorch and only the spline branch runs natively.  ``create_graph=True``
     is exact on every backend.
+
+    ``activation_checkpoint`` (no counterpart in the reference): None, "int8" or "e4m3": what the native
+    backward needs of the input is kept as 8-bit codes (:func:`~torchsplinekan_b200.pack_activation`)
+    instead of the input itself, a quarter of its float32 memory.  The output is the same; the
+    gradients are those at the restored input.  ``create_graph=True`` then raises, the dense backend
+    does not use it, and :meth:`forward_with_regularization` keeps its input (the edge statistic needs
+    it), so it does not either.
     """
 
     def __init__(self, in_features: int, out_features: int, grid_size: int = 5, spline_order: int = 3,
                  scale_noise: float = 0.1, scale_base: float = 1.0, scale_spline: float = 1.0,
                  enable_standalone_scale_spline: bool = True, base_activation=nn.SiLU, grid_eps: float = 0.02,
-                 grid_range: Tuple[float, float] = (-1.0, 1.0), backend: str = "auto") -> None:
+                 grid_range: Tuple[float, float] = (-1.0, 1.0), backend: str = "auto",
+                 activation_checkpoint: Optional[str] = None) -> None:
         super().__init__()
         if grid_size < 1:
             raise ValueError(f"grid_size must be >= 1, got {grid_size}")
@@ -57,6 +66,9 @@ class KANLinear(nn.Module):
             raise ValueError(f"spline_order must be 1, 2, or 3, got {spline_order}")
         if backend not in ("auto", "cuda", "reference"):
             raise ValueError(f"backend must be 'auto', 'cuda', or 'reference', got {backend!r}")
+        if activation_checkpoint not in CHECKPOINTS:
+            raise ValueError(f"activation_checkpoint must be one of {list(CHECKPOINTS)}, got {activation_checkpoint!r}")
+        self.activation_checkpoint = activation_checkpoint
         native_ok, why_not = native_config_supported(in_features, grid_size, spline_order)
         if backend == "cuda":
             if not native_ok:
@@ -115,9 +127,9 @@ class KANLinear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         which = self.backend_for(x)
         self.last_backend = which
-        return self._cuda_forward(x) if which == "cuda" else self._ref(x)
+        return self._cuda_forward(x, self.activation_checkpoint) if which == "cuda" else self._ref(x)
 
-    def _cuda_forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _cuda_forward(self, x: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
         if not x.is_cuda:
             raise RuntimeError("KANLinear with backend='cuda' received a CPU tensor. "
                                "Move the input and model to a CUDA device, or use backend='reference'.")
@@ -132,8 +144,12 @@ class KANLinear(nn.Module):
             if not fuse_base:
                 out = out + F.linear(self._ref.base_activation(xf), self.base_weight)
             return out.reshape(lead + (self.out_features,))
-        out = _C.kan_apply(xf, self.grid, self.base_weight if fuse_base else absent, self.spline_weight,
-                           self.spline_scaler if has_scaler else absent, self.spline_order, has_scaler)
+        args = (xf, self.grid, self.base_weight if fuse_base else absent, self.spline_weight,
+                self.spline_scaler if has_scaler else absent, self.spline_order, has_scaler)
+        if checkpoint is not None and torch.is_grad_enabled() and any(t.requires_grad for t in args[:5]):
+            out = _C.kan_apply_checkpointed(*args, CHECKPOINTS[checkpoint])
+        else:
+            out = _C.kan_apply(*args)
         if not fuse_base:
             out = out + F.linear(self._ref.base_activation(xf), self.base_weight)
         return out.reshape(lead + (self.out_features,))
@@ -337,7 +353,8 @@ class KANLinear(nn.Module):
             grid_size=self.grid_size if grid_size is None else grid_size, spline_order=self.spline_order,
             scale_noise=ref.scale_noise, scale_base=ref.scale_base, scale_spline=ref.scale_spline,
             enable_standalone_scale_spline=scaler, base_activation=copy.deepcopy(ref.base_activation),
-            grid_eps=ref.grid_eps, grid_range=ref.grid_range, backend=self.backend)
+            grid_eps=ref.grid_eps, grid_range=ref.grid_range, backend=self.backend,
+            activation_checkpoint=self.activation_checkpoint)
         return twin.to(device=self.grid.device, dtype=self.grid.dtype)
 
     @torch.no_grad()

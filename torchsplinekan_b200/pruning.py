@@ -72,6 +72,9 @@ def prune_nodes(model: KAN, x_calib: Optional[torch.Tensor] = None, threshold: f
     ``threshold``; ``model`` is left untouched.  ``keep`` lists the surviving indices per hidden
     layer explicitly (no scoring then); ``min_keep`` nodes per hidden layer always survive, chosen
     by the larger ``min(incoming, outgoing)`` (spline_kan/pruning.py:86-156)."""
+    if model.norms is not None or model.connections is not None:
+        raise ValueError("prune_nodes works on plain chains of layers: norms and residual connections tie the widths "
+                         "of their layers together")
     hidden = len(model.layers) - 1
     scores_in: List[torch.Tensor] = []
     scores_out: List[torch.Tensor] = []
