@@ -358,11 +358,12 @@ bool four_at_once(const kanb200_block_args& a) {
 int warp_columns(const kanb200_block_args& a, bool backward) {
     return kPackGroup * ring_chunks(backward, backward ? a.has_branch : a.y != nullptr, a.dtype == KANB200_F64);
 }
-// The ring kernels take rows of up to 8 blocks of 16 warps, and 32-bit row numbers and strides.
+int big_warps(const kanb200_block_args& a) { return ring_threads(true, a.dtype == KANB200_F64) / 32; }
+// The ring kernels take rows of up to 8 blocks of big_warps, and 32-bit row numbers and strides.
 bool ring_fits(const kanb200_block_args& a, bool backward) {
     for (int64_t n : {a.rows, a.x_stride, a.y_stride, a.gate_stride, a.dout_stride, a.dh_stride, a.dy_stride, a.dgate_stride})
         if (n >= ((int64_t)1 << 31) - 4096) return false;
-    return a.width <= (int64_t)8 * 16 * warp_columns(a, backward);
+    return a.width <= (int64_t)8 * big_warps(a) * warp_columns(a, backward);
 }
 
 RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
@@ -374,7 +375,7 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     while (p.lanes < 32 && p.lanes * 4 * V < a.width) p.lanes *= 2;
     const int all = (int)div_up(a.width, per_warp);
     p.cluster = 1;
-    while (div_up(all, p.cluster) > 16) p.cluster *= 2;
+    while (div_up(all, p.cluster) > big_warps(a)) p.cluster *= 2;
     p.warps = p.lanes == 32 ? (int)div_up(all, p.cluster) : 1;
     p.big = p.warps > 8 || p.cluster > 1;
     p.teams_per_block = p.big ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
@@ -384,7 +385,7 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.mode = !vec ? kScalar : p.lanes * 4 * V * (p.lanes == 32 ? p.warps * p.cluster : 1) == a.width ? kFull : kVector;
 
     // a stage of the ring: BackwardStage, or x, y and a gate per row
-    const int most = ring_threads(p.big);
+    const int most = ring_threads(p.big, B == 8);
     const bool row_gate = branch && (a.gate || a.gate_codes) && !(a.gate && a.gate_rows > 1);
     if (backward) {
         const auto take = [&](bool there, int bytes) { p.stage_bytes += there ? bytes : 0; };
@@ -398,10 +399,16 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     }
     p.stage_bytes = std::max(p.stage_bytes, 4 * B * most);      // the blocks' column sums meet in the ring at the end
 
-    // blocks to an SM by registers (the kernels' launch bounds) and shared memory
-    const int registers = 65536 / (ring_threads(p.big) * ring_blocks(backward, branch, p.big, B == 8));
+    // the backward's copies of next_weight, post_weight and scale
+    p.parameter_bytes = backward ? ((a.dh ? 1 : 0) + (branch ? 2 : 0)) * (p.threads / p.teams_per_block) * 4 * V * B : 0;
+
+    // blocks to an SM by registers (the kernels' launch bounds) and shared memory, then up to four stages while there is room
+    const int registers = 65536 / (ring_threads(p.big, false) * ring_blocks(p.big));
     int per_sm = std::max(1, 65536 / (registers * T));
-    while (per_sm > 1 && (2 * p.stage_bytes + 2048) * per_sm > 200 * 1024) --per_sm;
+    const auto fits = [&](int stages) { return (stages * p.stage_bytes + p.parameter_bytes + 2048) * per_sm <= 226 * 1024; };
+    while (per_sm > 1 && !fits(2)) --per_sm;
+    p.stages = 2;
+    while (p.stages < 4 && fits(p.stages + 1)) ++p.stages;
     static_cast<RowSplit&>(p) = split_rows(a, (int64_t)kSms * per_sm / p.cluster * p.teams_per_block);
     p.blocks = (int)div_up(p.teams, p.teams_per_block) * p.cluster;
     if (!p.shared) {                     // rows in turn: over every team that is launched

@@ -33,18 +33,19 @@ struct RingPlan : RowSplit {
     int lanes;                       // 4, 8, 16 or 32
     int warps;                       // of a team, in one block (lanes == 32)
     int teams_per_block, cluster;
-    int threads, blocks, stage_bytes;
+    int threads, blocks, stages, stage_bytes, parameter_bytes;
     int mode;                        // kFull, kVector or kScalar
     bool big;
 };
 
-// Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers for the sums
-// that are parameter gradients (12 to 20 V values behind a branch, 8 V at a norm).  Four chunks behind a branch spill: the
-// 8-bit gated backward of 16384 x 2048 took 278 us instead of 243.
-constexpr int ring_chunks(bool backward, bool branch, bool f64) { return (backward && branch ? 2 : 4) / (f64 ? 2 : 1); }
-// Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.
-constexpr int ring_threads(bool big) { return big ? 512 : 256; }
-constexpr int ring_blocks(bool backward, bool branch, bool big, bool f64) { return big ? 1 : 2; }
+// Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers: for the
+// parameters in the forward, behind a branch for the sums that are parameter gradients in the backward (20 V values; with
+// four chunks the 8-bit gated backward of 16384 x 2048 spilled and took 278 us instead of 243).
+constexpr int ring_chunks(bool backward, bool branch, bool f64) { return (backward && !branch ? 4 : 2) / (f64 ? 2 : 1); }
+// Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.  (Float64: 384,
+// the backward's ring and parameters have to fit an SM's shared memory.)
+constexpr int ring_threads(bool big, bool f64) { return !big ? 256 : f64 ? 384 : 512; }
+constexpr int ring_blocks(bool big) { return big ? 1 : 2; }
 
 // Bytes of one tensor in a stage of the ring: elements of less than 4 bytes that cannot be copied four at a time are not
 // there.  Values that may come as codes need room for either.

@@ -5,12 +5,13 @@
 //     Teams take rows in turn; with a shared gate a team takes consecutive rows, so that a gate row is read, and its
 //     gradient leaves, once per team (consecutive rows everywhere cost 5 to 10 % of the bandwidth: norm of 65536 x 1024
 //     forward 99 us against 91).
-//   * Memory -> registers goes through a ring of two rows in shared memory, filled by cp.async.  A thread copies
+//   * Memory -> registers goes through a ring of 2 to 4 rows in shared memory, filled by cp.async.  A thread copies
 //     exactly what it reads back itself, so the ring needs no barrier: only its own cp.async group to have landed.  The
 //     bytes in flight then do not depend on registers or on how many warps wait in a barrier.
-//   * The sums over rows that are the parameters' gradients stay in registers; one slab row per block leaves the kernel at
-//     its end.  Parameters are read again for every row, from L1: the ring leaves room for them (with 3 rows instead of 2
-//     the gated backward of 16384 x 1024 took 180 us instead of 122, the parameters then came from L2).
+//   * Parameters stay on chip: in registers in the forward, in shared memory in the backward, where the registers hold the
+//     sums over rows that are their gradients (one slab row per block leaves the kernel at its end).  Read from L1 for every
+//     row they came from L2 whenever the ring took most of the SM's memory, a few hundred cycles at a time (gated forward of
+//     16777 x 1000: 85 us, most of the stalls).
 //   * Sums over a row: lanes by shuffles, warps through shared memory with a barrier of the team alone, blocks of a
 //     cluster through each other's shared memory; every thread gets the same bits.
 //   * Issue slots bound these kernels before bandwidth does, so: what a row costs besides its elements (sums, barriers,
@@ -34,6 +35,13 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT> __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
+// all but the newest stages - 1 groups have landed
+__device__ __forceinline__ void copies_wait_oldest(int stages) {
+    if (stages == 2) copies_wait<1>();
+    else if (stages == 3) copies_wait<2>();
+    else copies_wait<3>();
+}
+
 // Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other; a thread has four of each,
 // side by side (kFull, kVector: rows, strides and pointers allow four elements at once) or LANES apart (kScalar).  kFull:
 // the team's columns are exactly the row's, so nothing is masked (a third of the instructions of the gated backward were
@@ -50,8 +58,8 @@ template <int LANES, int V, int MODE> struct Columns {
 // ---- rows <-> registers -----------------------------------------------------------------------------------------------
 // A thread's elements of one tensor on their way from a row in memory to registers.  Types of less than 4 bytes that
 // cannot be copied four at a time have no ring slot: they are loaded where they are used.  T is the block's most threads:
-// a slot's pieces are arrays over T threads, so that all distances in a stage are constants too.  `row` and `slot` point to
-// the thread's own first element and place.
+// a slot's pieces are arrays over T threads, so that all distances in a stage are constants too.  Places of columns beyond
+// the row hold 0 (clear_ring) and are never written.  `row` points to the thread's own first element.
 template <typename E, int LANES, int V, int MODE, int T> struct Feed {
     using Cols = Columns<LANES, V, MODE>;
     static constexpr bool VEC = MODE != kScalar;
@@ -80,22 +88,17 @@ template <typename E, int LANES, int V, int MODE, int T> struct Feed {
     }
     static __device__ __forceinline__ Quad<E> take(const char* stage, const E* row, const Cols& c, int j) {
         const char* src = stage + threadIdx.x * kPiece;
-        Quad<E> q{};
-        if constexpr (VEC) {
-            if (c.ok(j, 0)) {
-                if constexpr (kPieces == 2) {
-                    reinterpret_cast<float4*>(&q)[0] = *reinterpret_cast<const float4*>(src + (2 * j) * T * kPiece);
-                    reinterpret_cast<float4*>(&q)[1] = *reinterpret_cast<const float4*>(src + (2 * j + 1) * T * kPiece);
-                } else {
-                    q = *reinterpret_cast<const Quad<E>*>(src + j * T * kPiece);
-                }
-            }
+        Quad<E> q;
+        if constexpr (VEC && kPieces == 2) {
+            reinterpret_cast<float4*>(&q)[0] = *reinterpret_cast<const float4*>(src + (2 * j) * T * kPiece);
+            reinterpret_cast<float4*>(&q)[1] = *reinterpret_cast<const float4*>(src + (2 * j + 1) * T * kPiece);
+        } else if constexpr (VEC) {
+            q = *reinterpret_cast<const Quad<E>*>(src + j * T * kPiece);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (!c.ok(j, e)) continue;
                 if constexpr (kRing) q.v[e] = *reinterpret_cast<const E*>(src + (4 * j + e) * T * kPiece);
-                else q.v[e] = row[Cols::apart(j, e)];
+                else q.v[e] = c.ok(j, e) ? row[Cols::apart(j, e)] : E{};
             }
         }
         return q;
@@ -130,12 +133,24 @@ __device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, MOD
     }
     return widen4<B>(q);
 }
-// x for the row's own columns, 0 beyond them
 template <typename B, int LANES, int V, int MODE>
-__device__ __forceinline__ Four<B> within(const Columns<LANES, V, MODE>& c, int j, Four<B> x) {
+__device__ __forceinline__ Four<B> get_or(const void* p, const Columns<LANES, V, MODE>& c, int j, B absent) {
+    return p ? get(static_cast<const B*>(p) + c.col, c, j) : four<B>(absent);
+}
+// x - mean for the row's own columns; 0 beyond them, where x is 0
+template <typename B, int LANES, int V, int MODE>
+__device__ __forceinline__ Four<B> centre(const Columns<LANES, V, MODE>& c, int j, const Four<B>& x, B mean) {
+    Four<B> m = four<B>(-mean);
+    if constexpr (MODE == kVector) m = four<B>(c.ok(j, 0) ? -mean : B(0));
+    if constexpr (MODE == kScalar)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x.v[e] = c.ok(j, e) ? x.v[e] : B(0);
-    return x;
+        for (int e = 0; e < 4; ++e) m.v[e] = c.ok(j, e) ? -mean : B(0);
+    return x + m;
+}
+__device__ __forceinline__ void clear_ring(char* ring, int bytes) {
+    for (int at = threadIdx.x * 16; at < bytes; at += blockDim.x * 16)
+        *reinterpret_cast<float4*>(ring + at) = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
 }
 
 // 1 / sqrt: the float approximation (2 ulp) and a Newton step, instead of a correctly rounded root and division
@@ -265,10 +280,10 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], con
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, int MODE, bool BRANCH, bool BIG>
-__global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, BIG, sizeof(S) == 8))
+__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG))
     ring_forward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p) {
     using B = Br<S>;
-    constexpr int T = ring_threads(BIG);
+    constexpr int T = ring_threads(BIG, sizeof(S) == 8);
     using FS = Feed<S, LANES, V, MODE, T>;
     using FB = Feed<B, LANES, V, MODE, T>;
     constexpr int at_y = FS::kBytes, at_gate = at_y + FB::kBytes;
@@ -283,10 +298,18 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
     const B eps = B(a.eps), per = B(1) / B(D);
 
     const S* x = static_cast<const S*>(a.x) + c.col;
-    const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col,
-            *scale = static_cast<const B*>(a.scale) + c.col, *pw = static_cast<const B*>(a.post_weight) + c.col,
-            *pb = static_cast<const B*>(a.post_bias) + c.col, *nw = static_cast<const B*>(a.next_weight) + c.col,
-            *nb = static_cast<const B*>(a.next_bias) + c.col;
+    const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col;
+    Four<B> scale[V], pw[V], pb[V], nw[V], nb[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (BRANCH) {
+            scale[j] = get_or(a.scale, c, j, B(1));
+            pw[j] = get_or(a.post_weight, c, j, B(1));
+            pb[j] = get_or(a.post_bias, c, j, B(0));
+        }
+        nw[j] = get_or(a.next_weight, c, j, B(1));
+        nb[j] = get_or(a.next_bias, c, j, B(0));
+    }
 
     const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
                    last = p.shared ? min(first + p.rows_per_team, rows) : rows;
@@ -313,7 +336,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
             acc = four<B>(B(0));
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const Four<B> d = within<B>(c, j, v[j] + four<B>(-mean));
+                const Four<B> d = centre<B>(c, j, v[j], mean);
                 acc = fma4(d, d, acc);
             }
         } else {
@@ -337,13 +360,15 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
         span = first / (uint32_t)a.gate_rows;
         span_end = first;
     }
-    issue(first, 0);
+    if (MODE != kFull) clear_ring(ring, p.stages * p.stage_bytes);
+    uint32_t ahead = first;
+    for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
     int stage = 0;
     Four<B> t[V];                                           // act(gate) of a shared gate
     // every team makes the same number of steps: teams that share a warp meet in its shuffles
-    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, stage ^= 1) {
-        issue(row + next, stage ^ 1);
-        copies_wait<1>();                                   // all but the newest group
+    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
+        issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
+        copies_wait_oldest(p.stages);
         const bool live = row < last;
         if (LANES == 32 && !live) break;                    // a whole team, alone in its warps
         const char* at = ring + stage * p.stage_bytes;
@@ -363,7 +388,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
                 moments(a.post_norm, v, mean, rstd);
                 if (a.post_stats && live) put_stats(a.post_stats, row, mean, rstd);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = (v[j] + four<B>(-mean)) * four<B>(rstd);
+                for (int j = 0; j < V; ++j) v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);
             }
             if (p.shared && row >= span_end && live) {
                 span = row / (uint32_t)a.gate_rows;
@@ -374,10 +399,8 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
             // out = x + scale act(gate) z; what v becomes is the branch's summand
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if (a.post_weight) v[j] = v[j] * get(pw, c, j);
-                if (a.post_bias) v[j] = v[j] + get(pb, c, j);
+                v[j] = fma4(v[j], pw[j], pb[j]) * scale[j];
                 if (p.shared) v[j] = v[j] * t[j];
-                if (a.scale) v[j] = v[j] * get(scale, c, j);
             }
             if (row_gate) {
                 Four<B> g[V];
@@ -394,7 +417,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const Quad<S> q = narrow4<S>(widen4<S>(FS::take(at, row_at(x, row, a.x_stride), c, j)) + v[j]);
-                    o[j] = within<B>(c, j, widen4<S>(q));
+                    o[j] = widen4<S>(q);                              // 0 beyond the row, as all its terms are
                     put(static_cast<S*>(a.out) + dense, c, j, q);
                 }
         } else if (live) {
@@ -411,23 +434,22 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(false, BRANCH, 
             if (live)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    o[j] = (o[j] + four<B>(-mean)) * four<B>(rstd);
-                    if (a.next_weight) o[j] = o[j] * get(nw, c, j);
-                    if (a.next_bias) o[j] = o[j] + get(nb, c, j);
+                    o[j] = fma4(centre<B>(c, j, o[j], mean) * four<B>(rstd), nw[j], nb[j]);
                     put(static_cast<B*>(a.h) + dense, c, j, o[j]);
                 }
         }
+        stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
     copies_wait<0>();
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, int MODE, bool BRANCH, bool NEXT, bool BIG>
-__global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, BIG, sizeof(S) == 8))
+__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG))
     ring_backward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p,
                          const __grid_constant__ BackwardSlabs slabs) {
     using B = Br<S>;
-    constexpr int T = ring_threads(BIG);
+    constexpr int T = ring_threads(BIG, sizeof(S) == 8);
     using FS = Feed<S, LANES, V, MODE, T>;
     using FB = Feed<B, LANES, V, MODE, T>;
     using FQ = Feed<uint8_t, LANES, V, MODE, T>;
@@ -445,9 +467,19 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
 
     const S *x = static_cast<const S*>(a.x) + c.col, *dout = static_cast<const S*>(a.dout) + c.col;
     const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col,
-            *dh = static_cast<const B*>(a.dh) + c.col, *scale = static_cast<const B*>(a.scale) + c.col,
-            *pw = static_cast<const B*>(a.post_weight) + c.col, *pb = static_cast<const B*>(a.post_bias) + c.col,
-            *nw = static_cast<const B*>(a.next_weight) + c.col;
+            *dh = static_cast<const B*>(a.dh) + c.col, *pb = static_cast<const B*>(a.post_bias) + c.col;
+    // parameters, chunk after chunk of the team's threads: teams of a block share them
+    const int per_team = blockDim.x / p.teams_per_block, in_team = threadIdx.x % per_team;
+    Four<B>* shelf = reinterpret_cast<Four<B>*>(ring + p.stages * p.stage_bytes);
+    Four<B> *const nw = shelf + in_team, *const pw = shelf + (NEXT ? V * per_team : 0) + in_team, *const scale = pw + V * per_team;
+    if ((int)threadIdx.x < per_team)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (NEXT) nw[j * per_team] = get_or(a.next_weight, c, j, B(1));
+            if (BRANCH) pw[j * per_team] = get_or(a.post_weight, c, j, B(1));
+            if (BRANCH) scale[j * per_team] = get_or(a.scale, c, j, B(1));
+        }
+    __syncthreads();
     Four<B> sum_scale[V], sum_pw[V], sum_pb[V], sum_nw[V], sum_nb[V], sum_gate[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum_scale[j] = sum_pw[j] = sum_pb[j] = sum_nw[j] = sum_nb[j] = sum_gate[j] = zero;
@@ -470,7 +502,7 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
         if (codes) {
             const Quad<uint8_t> q = FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c, j);
-            const B s = c.at(j, 0) < D ? *reinterpret_cast<const B*>(at + 4 * V * T + (j * T + threadIdx.x) * sizeof(B)) : B(0);
+            const B s = *reinterpret_cast<const B*>(at + 4 * V * T + (j * T + threadIdx.x) * sizeof(B));
             return decode4<B>(a.checkpoint, *reinterpret_cast<const uint32_t*>(&q), s);
         }
         return widen4<E>(Feed<E, LANES, V, MODE, T>::take(at, row_at(values, row, stride), c, j));
@@ -504,11 +536,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
         span_first = span * (uint32_t)a.gate_rows;
         span_end = span_first + (uint32_t)a.gate_rows;
     }
-    issue(first, 0);
+    if (MODE != kFull) clear_ring(ring, p.stages * p.stage_bytes);
+    uint32_t ahead = first;
+    for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
     int stage = 0;
-    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, stage ^= 1) {
-        issue(row + next, stage ^ 1);
-        copies_wait<1>();                                   // all but the newest group
+    for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
+        issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
+        copies_wait_oldest(p.stages);
         const bool live = row < last;
         if (LANES == 32 && !live) break;
         const char* at = ring + stage * p.stage_bytes;
@@ -528,10 +562,10 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
                 for (int j = 0; j < V; ++j) {
                     d[j] = widen4<B>(FB::take(at + At::dh, row_at(dh, row, a.dh_stride), c, j));
                     v[j] = take_kept(at + At::x, a.x_codes, x, a.x_stride, row, j);
-                    v[j] = within<B>(c, j, (v[j] + four<B>(-mean)) * four<B>(rstd));          // the normalised row
+                    v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);          // the normalised row
                     sum_nw[j] = fma4(d[j], v[j], sum_nw[j]);
                     sum_nb[j] = sum_nb[j] + d[j];
-                    if (a.next_weight) d[j] = d[j] * get(nw, c, j);
+                    d[j] = d[j] * nw[j * per_team];
                     s0 = s0 + d[j];
                     s1 = fma4(d[j], v[j], s1);
                 }
@@ -566,12 +600,9 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     v[j] = take_kept(at + At::y, a.y_codes, y, a.y_stride, row, j);
-                    if (a.post_norm != kNormNone) v[j] = within<B>(c, j, (v[j] + four<B>(-mean)) * four<B>(rstd));
-                    Four<B> z = v[j], w;
-                    if (a.post_weight) {
-                        w = get(pw, c, j);
-                        z = z * w;
-                    }
+                    if (a.post_norm != kNormNone) v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);
+                    const Four<B> w = pw[j * per_team], sc = scale[j * per_team];
+                    Four<B> z = v[j] * w;
                     if (a.post_bias) z = z + get(pb, c, j);
                     if (p.shared || row_gate) {
                         Four<B> act, dact;
@@ -580,22 +611,17 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
                         gate4_grad<B>(a.gate_act, gv, act, dact);
                         const Four<B> gz = g[j] * z;
                         sum_scale[j] = fma4(gz, act, sum_scale[j]);
-                        Four<B> dg = gz * dact;
-                        if (a.scale) {
-                            const Four<B> sc = get(scale, c, j);
-                            dg = dg * sc;
-                            act = act * sc;
-                        }
+                        const Four<B> dg = gz * (dact * sc);
                         if (p.shared) sum_gate[j] = sum_gate[j] + dg;
                         else if (a.dgate) put(row_at(static_cast<B*>(a.dgate) + c.col, row, a.dgate_stride), c, j, dg);
-                        g[j] = g[j] * act;
+                        g[j] = g[j] * (act * sc);
                     } else {
                         sum_scale[j] = fma4(g[j], z, sum_scale[j]);
-                        if (a.scale) g[j] = g[j] * get(scale, c, j);
+                        g[j] = g[j] * sc;
                     }
                     sum_pw[j] = fma4(g[j], v[j], sum_pw[j]);
                     sum_pb[j] = sum_pb[j] + g[j];
-                    if (a.post_weight) g[j] = g[j] * w;
+                    g[j] = g[j] * w;
                     s0 = s0 + g[j];
                     s1 = fma4(g[j], v[j], s1);
                 }
@@ -625,13 +651,13 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(true, BRANCH, B
                 }
             }
         }
+        stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
     copies_wait<0>();
 
     // one slab row per block: the teams' sums, added in the order of the teams
     const uint32_t block = BIG && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
-    Four<B>* shelf = reinterpret_cast<Four<B>*>(ring);
-    const int per_team = blockDim.x / p.teams_per_block;
+    shelf = reinterpret_cast<Four<B>*>(ring);
     const auto leave = [&](int which, Four<B> (&v)[V]) {
         if (!slabs.column[which]) return;
         B* row = static_cast<B*>(slabs.column[which]) + (uint64_t)block * (uint32_t)D + c.col;
@@ -665,7 +691,7 @@ namespace kanb200 {
 
 template <typename... P>
 cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...), const P&... args) {
-    const int bytes = 2 * p.stage_bytes;
+    const int bytes = p.stages * p.stage_bytes + p.parameter_bytes;
     cudaError_t e = cudaSuccess;
     if (bytes > 48 * 1024 - (int)sizeof(TeamScratch))
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
