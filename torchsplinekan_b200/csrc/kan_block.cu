@@ -354,30 +354,50 @@ bool four_at_once(const kanb200_block_args& a) {
     return true;
 }
 
-// Columns that a warp of the ring kernels covers.
-int warp_columns(const kanb200_block_args& a, bool backward) {
-    return kPackGroup * ring_chunks(backward, backward ? a.has_branch : a.y != nullptr, a.dtype == KANB200_F64);
+// Warps for a row: `warps` in each of `cluster` blocks, of `chunks` chunks per thread.  At most 8 warps make a small block.
+struct Team {
+    int chunks, warps, cluster;
+    bool many, big;
+};
+Team team_for(const kanb200_block_args& a, bool backward) {
+    const bool branch = backward ? a.has_branch : a.y != nullptr, f64 = a.dtype == KANB200_F64;
+    Team t{};
+    t.many = !branch;
+    const auto cover = [&] {
+        t.chunks = ring_chunks(t.many, f64);
+        t.warps = (int)div_up(a.width, kPackGroup * t.chunks);
+    };
+    cover();
+    if (t.warps > 8 && !backward && !t.many) {
+        t.many = true;
+        cover();
+    }
+    t.big = t.warps > 8;
+    t.cluster = 1;
+    const int all = t.warps, most = ring_threads(t.big, f64) / 32;
+    while (div_up(all, t.cluster) > most) t.cluster *= 2;
+    t.warps = (int)div_up(all, t.cluster);
+    return t;
 }
-int big_warps(const kanb200_block_args& a) { return ring_threads(true, a.dtype == KANB200_F64) / 32; }
-// The ring kernels take rows of up to 8 blocks of big_warps, and 32-bit row numbers and strides.
+// The ring kernels take rows of up to 8 blocks, and 32-bit row numbers and strides.
 bool ring_fits(const kanb200_block_args& a, bool backward) {
     for (int64_t n : {a.rows, a.x_stride, a.y_stride, a.gate_stride, a.dout_stride, a.dh_stride, a.dy_stride, a.dgate_stride})
         if (n >= ((int64_t)1 << 31) - 4096) return false;
-    return a.width <= (int64_t)8 * big_warps(a) * warp_columns(a, backward);
+    return team_for(a, backward).cluster <= 8;
 }
 
 RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     RingPlan p{};
     const int B = (int)branch_bytes(a.dtype), S = a.dtype == KANB200_F64 ? 8 : a.dtype == KANB200_F32 ? 4 : 2;
     const bool branch = backward ? a.has_branch : a.y != nullptr;
-    const int per_warp = warp_columns(a, backward), V = per_warp / kPackGroup;
+    const Team team = team_for(a, backward);
+    const int V = team.chunks;
     p.lanes = 4;
     while (p.lanes < 32 && p.lanes * 4 * V < a.width) p.lanes *= 2;
-    const int all = (int)div_up(a.width, per_warp);
-    p.cluster = 1;
-    while (div_up(all, p.cluster) > big_warps(a)) p.cluster *= 2;
-    p.warps = p.lanes == 32 ? (int)div_up(all, p.cluster) : 1;
-    p.big = p.warps > 8 || p.cluster > 1;
+    p.cluster = team.cluster;
+    p.warps = team.warps;
+    p.big = team.big;
+    p.many = team.many;
     p.teams_per_block = p.big ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
     p.threads = p.lanes == 32 ? 32 * p.warps * p.teams_per_block : 256;
     const int T = p.threads;
@@ -405,10 +425,11 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     // blocks to an SM by registers (the kernels' launch bounds) and shared memory, then up to four stages while there is room
     const int registers = 65536 / (ring_threads(p.big, false) * ring_blocks(p.big));
     int per_sm = std::max(1, 65536 / (registers * T));
-    const auto fits = [&](int stages) { return (stages * p.stage_bytes + p.parameter_bytes + 2048) * per_sm <= 226 * 1024; };
+    const auto fits = [&](int stages) { return (stages * p.stage_bytes + p.parameter_bytes + 1024 + 768) * per_sm <= 228 * 1024; };
     while (per_sm > 1 && !fits(2)) --per_sm;
     p.stages = 2;
-    while (p.stages < 4 && fits(p.stages + 1)) ++p.stages;
+    if (backward || !branch || !p.many)                  // (parameters in memory need L1)
+        while (p.stages < 4 && fits(p.stages + 1)) ++p.stages;
     static_cast<RowSplit&>(p) = split_rows(a, (int64_t)kSms * per_sm / p.cluster * p.teams_per_block);
     p.blocks = (int)div_up(p.teams, p.teams_per_block) * p.cluster;
     if (!p.shared) {                     // rows in turn: over every team that is launched

@@ -34,14 +34,19 @@ struct RingPlan : RowSplit {
     int warps;                       // of a team, in one block (lanes == 32)
     int teams_per_block, cluster;
     int threads, blocks, stages, stage_bytes, parameter_bytes;
+    bool many;                       // chunks
     int mode;                        // kFull, kVector or kScalar
     bool big;
 };
 
-// Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers: for the
-// parameters in the forward, behind a branch for the sums that are parameter gradients in the backward (20 V values; with
-// four chunks the 8-bit gated backward of 16384 x 2048 spilled and took 278 us instead of 243).
-constexpr int ring_chunks(bool backward, bool branch, bool f64) { return (backward && !branch ? 4 : 2) / (f64 ? 2 : 1); }
+// Chunks of four columns per thread.  More share the cost of a row among more elements, fewer leave registers.
+//   * The forward behind a branch holds its parameters in registers with few chunks (rows that 8 warps cover that way) and
+//     reads them from memory with many (wider rows; larger blocks with few chunks left SMs half empty: gated forward of
+//     8176 x 2052, 190 us).
+//   * The backward behind a branch holds the sums that are parameter gradients (20 V values): few chunks always (with many the
+//     8-bit gated backward of 16384 x 2048 spilled and took 278 us instead of 243).
+//   * A norm alone takes many.
+constexpr int ring_chunks(bool many, bool f64) { return (many ? 4 : 2) / (f64 ? 2 : 1); }
 // Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.  (Float64: 384,
 // the backward's ring and parameters have to fit an SM's shared memory.)
 constexpr int ring_threads(bool big, bool f64) { return !big ? 256 : f64 ? 384 : 512; }

@@ -299,17 +299,24 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
 
     const S* x = static_cast<const S*>(a.x) + c.col;
     const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col;
-    Four<B> scale[V], pw[V], pb[V], nw[V], nb[V];
+    // parameters in registers, or with many chunks behind a branch in memory
+    constexpr bool kHeld = !BRANCH || V == ring_chunks(false, sizeof(S) == 8);
+    constexpr int H = kHeld ? V : 1;
+    Four<B> held[5][H];
+    const auto parameter = [&](int which, const void* p, int j, B absent) {
+        return kHeld ? held[which][kHeld ? j : 0] : get_or(p, c, j, absent);
+    };
+    if (kHeld)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        if (BRANCH) {
-            scale[j] = get_or(a.scale, c, j, B(1));
-            pw[j] = get_or(a.post_weight, c, j, B(1));
-            pb[j] = get_or(a.post_bias, c, j, B(0));
+        for (int j = 0; j < H; ++j) {
+            if (BRANCH) {
+                held[0][j] = get_or(a.scale, c, j, B(1));
+                held[1][j] = get_or(a.post_weight, c, j, B(1));
+                held[2][j] = get_or(a.post_bias, c, j, B(0));
+            }
+            held[3][j] = get_or(a.next_weight, c, j, B(1));
+            held[4][j] = get_or(a.next_bias, c, j, B(0));
         }
-        nw[j] = get_or(a.next_weight, c, j, B(1));
-        nb[j] = get_or(a.next_bias, c, j, B(0));
-    }
 
     const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
                    last = p.shared ? min(first + p.rows_per_team, rows) : rows;
@@ -399,7 +406,8 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
             // out = x + scale act(gate) z; what v becomes is the branch's summand
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                v[j] = fma4(v[j], pw[j], pb[j]) * scale[j];
+                v[j] = fma4(v[j], parameter(1, a.post_weight, j, B(1)), parameter(2, a.post_bias, j, B(0))) *
+                       parameter(0, a.scale, j, B(1));
                 if (p.shared) v[j] = v[j] * t[j];
             }
             if (row_gate) {
@@ -434,7 +442,8 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
             if (live)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    o[j] = fma4(centre<B>(c, j, o[j], mean) * four<B>(rstd), nw[j], nb[j]);
+                    o[j] = fma4(centre<B>(c, j, o[j], mean) * four<B>(rstd), parameter(3, a.next_weight, j, B(1)),
+                                parameter(4, a.next_bias, j, B(0)));
                     put(static_cast<B*>(a.h) + dense, c, j, o[j]);
                 }
         }
@@ -714,19 +723,22 @@ cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...)
 
 template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_forward_as(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st) {
-    constexpr int V = ring_chunks(false, true, sizeof(S) == 8);
-    return a.y ? ring_launch(p, st, ring_forward_kernel<S, LANES, V, MODE, true, BIG>, a, p)
-               : ring_launch(p, st, ring_forward_kernel<S, LANES, V, MODE, false, BIG>, a, p);
+    constexpr bool f64 = sizeof(S) == 8;
+    constexpr int few = ring_chunks(false, f64), many = ring_chunks(true, f64);
+    if (!a.y) return ring_launch(p, st, ring_forward_kernel<S, LANES, many, MODE, false, BIG>, a, p);
+    if constexpr (LANES == 32)
+        if (BIG || p.many) return ring_launch(p, st, ring_forward_kernel<S, LANES, many, MODE, true, BIG>, a, p);
+    return ring_launch(p, st, ring_forward_kernel<S, LANES, few, MODE, true, false>, a, p);
 }
 template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_backward_as(const kanb200_block_args& a, const RingPlan& p, const BackwardSlabs& slabs, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
     if (!a.has_branch)
-        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, false, f64), MODE, false, true, BIG>,
+        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, f64), MODE, false, true, BIG>,
                            a, p, slabs);
-    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), MODE, true, true, BIG>,
+    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, f64), MODE, true, true, BIG>,
                               a, p, slabs)
-                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, true, f64), MODE, true, false, BIG>,
+                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, f64), MODE, true, false, BIG>,
                               a, p, slabs);
 }
 
