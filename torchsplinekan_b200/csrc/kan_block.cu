@@ -409,8 +409,8 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     const bool row_gate = branch && (a.gate || a.gate_codes) && !(a.gate && a.gate_rows > 1);
     if (backward) {
         const auto take = [&](bool there, int bytes) { p.stage_bytes += there ? bytes : 0; };
-        take(a.dh, ring_bytes(B, vec, V, most) + ring_kept_bytes(S, vec, V, most, B) + 2 * B * most);
-        take(branch, ring_kept_bytes(B, vec, V, most, B) + 2 * B * most);
+        take(a.dh, ring_bytes(B, vec, V, most) + ring_kept_bytes(S, vec, V, most, B) + ring_stats_bytes(most, B));
+        take(branch, ring_kept_bytes(B, vec, V, most, B) + ring_stats_bytes(most, B));
         take(a.dout || row_gate, ring_bytes(S, vec, V, most));
         take(row_gate, ring_kept_bytes(B, vec, V, most, B));
     } else {

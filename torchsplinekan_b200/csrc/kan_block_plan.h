@@ -57,18 +57,21 @@ constexpr int ring_blocks(bool big) { return big ? 1 : 2; }
 constexpr int ring_bytes(int element, bool vec, int chunks, int threads) {
     return vec || element >= 4 ? 4 * element * chunks * threads : 0;
 }
+constexpr int ring_scale_bytes(int chunks, int threads, int branch) { return chunks * threads / 4 * branch; }
+constexpr int ring_stats_bytes(int threads, int branch) { return 2 * threads / 4 * branch; }        // a team has 4 lanes at least
 constexpr int ring_kept_bytes(int element, bool vec, int chunks, int threads, int branch) {
-    return ring_bytes(element, vec, chunks, threads) > (4 + branch) * chunks * threads
-               ? ring_bytes(element, vec, chunks, threads) : (4 + branch) * chunks * threads;
+    const int values = ring_bytes(element, vec, chunks, threads);
+    const int codes = 4 * chunks * threads + ring_scale_bytes(chunks, threads, branch);
+    return values > codes ? values : codes;
 }
 // A stage of the backward; what is not part of every call comes last.
 template <bool NEXT, bool BRANCH, int V, int T, bool VEC, int S, int B> struct BackwardStage {
     static constexpr int dh = 0;
     static constexpr int x = dh + (NEXT ? ring_bytes(B, VEC, V, T) : 0);
     static constexpr int next_stats = x + (NEXT ? ring_kept_bytes(S, VEC, V, T, B) : 0);
-    static constexpr int y = next_stats + (NEXT ? 2 * B * T : 0);
+    static constexpr int y = next_stats + (NEXT ? ring_stats_bytes(T, B) : 0);
     static constexpr int post_stats = y + (BRANCH ? ring_kept_bytes(B, VEC, V, T, B) : 0);
-    static constexpr int dout = post_stats + (BRANCH ? 2 * B * T : 0);
+    static constexpr int dout = post_stats + (BRANCH ? ring_stats_bytes(T, B) : 0);
     static constexpr int gate = dout + ring_bytes(S, VEC, V, T);
     static constexpr int end = gate + ring_kept_bytes(B, VEC, V, T, B);
 };

@@ -170,6 +170,7 @@ struct TeamScratch {                       // per block, in shared memory
 template <typename B, int LANES, bool BIG> struct Team {
     TeamScratch* scratch;
     int warps, team, warp, lane;           // warps of this block in a row's team; team and warp within the team
+    int group;                             // of 128 columns, the warp's first
     int cluster, rank;
     int phase = 0;
 
@@ -241,6 +242,7 @@ __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScr
         id = group * p.teams_per_block + threadIdx.x / LANES;
     }
     c.width = width;
+    team.group = (c.col - (MODE != kScalar ? 4 * team.lane : team.lane)) / kPackGroup;
     if (BIG && p.cluster > 1) cooperative_groups::this_cluster().sync();      // every block's scratch exists
     return id;
 }
@@ -249,7 +251,7 @@ __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScr
 // chunks of the same threads.  Each lane forms the scale and its reciprocal of one group only.
 template <typename B, int LANES, int V, int MODE>
 __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], const Columns<LANES, V, MODE>& c, bool write,
-                                          uint8_t* codes, B* scales, int lane) {
+                                          uint8_t* codes, B* scales, int lane, int first) {
     constexpr int kTogether = 32 / LANES < V ? 32 / LANES : V, kGroups = V / kTogether;
     using Bits = typename AbsBits<B>::type;
     Bits mine = 0;
@@ -264,7 +266,6 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], con
         if (kGroups == 1 || lane % kGroups == i) mine = top;
     }
     const B scale = pack_scale<B>(format, AbsBits<B>::back(mine)), inverse = pack_inverse<B>(scale);
-    const int first = (c.col - (MODE != kScalar ? 4 * lane : lane)) / kPackGroup;          // the warp's first group
     if (write && lane < kGroups && (first + lane) * kPackGroup < c.width) scales[first + lane] = scale;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
             for (int j = 0; j < V; ++j) v[j] = live ? widen4<B>(FB::take(at + at_y, row_at(y, row, a.y_stride), c, j)) : four<B>(B(0));
             if (a.y_codes)
                 put_codes<B>(a.checkpoint, v, c, live, static_cast<uint8_t*>(a.y_codes) + dense,
-                             row_at(static_cast<B*>(a.y_scales), row, groups), team.lane);
+                             row_at(static_cast<B*>(a.y_scales), row, groups), team.lane, team.group);
             if (a.post_norm != kNormNone) {
                 B mean, rstd;
                 moments(a.post_norm, v, mean, rstd);
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                     g[j] = live ? widen4<B>(FB::take(at + at_gate, row_at(gate, row, a.gate_stride), c, j)) : four<B>(B(0));
                 if (a.gate_codes)
                     put_codes<B>(a.checkpoint, g, c, live, static_cast<uint8_t*>(a.gate_codes) + dense,
-                                 row_at(static_cast<B*>(a.gate_scales), row, groups), team.lane);
+                                 row_at(static_cast<B*>(a.gate_scales), row, groups), team.lane, team.group);
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[j] = v[j] * gate4<B>(a.gate_act, g[j]);
             }
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
         }
         if (a.x_codes)
             put_codes<B>(a.checkpoint, o, c, live, static_cast<uint8_t*>(a.x_codes) + dense,
-                         row_at(static_cast<B*>(a.x_scales), row, groups), team.lane);
+                         row_at(static_cast<B*>(a.x_scales), row, groups), team.lane, team.group);
         if (!BRANCH || a.next_norm != kNormNone) {
             B mean, rstd;
             moments(a.next_norm, o, mean, rstd);
@@ -493,16 +494,18 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
 #pragma unroll
     for (int j = 0; j < V; ++j) sum_scale[j] = sum_pw[j] = sum_pb[j] = sum_nw[j] = sum_nb[j] = sum_gate[j] = zero;
 
+    // What a warp's lanes read in common (statistics, scales) one lane copies: a copy of one address by 32 lanes to 32 places
+    // takes 32 passes of the shared memory.  The lanes meet in a __syncwarp before they read it.
+    constexpr int kTogether = 32 / LANES < V ? 32 / LANES : V, kGroups = V / kTogether;
+    const int clique = threadIdx.x / LANES;
     // a tensor that may be there as codes: codes and their groups' scales, or the values themselves
     const auto issue_kept = [&](uint32_t at, const void* codes, const void* scales, auto* values, int64_t stride, uint32_t row) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
         if (codes) {
             FQ::issue(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c);
-            const B* from = static_cast<const B*>(scales) + (uint64_t)row * (uint32_t)groups + c.col / kPackGroup;
-            const uint32_t dst = at + 4 * V * T + threadIdx.x * (uint32_t)sizeof(B);
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (c.at(j, 0) < D) copy_async<sizeof(B)>(dst + j * T * (uint32_t)sizeof(B), from + j * 4 * LANES / kPackGroup);
+            if (team.lane < kGroups && team.group + team.lane < groups)
+                copy_async<sizeof(B)>(at + 4 * V * T + (clique * V + team.lane) * (uint32_t)sizeof(B),
+                                      static_cast<const B*>(scales) + (uint64_t)row * (uint32_t)groups + team.group + team.lane);
         } else {
             Feed<E, LANES, V, MODE, T>::issue(at, row_at(values, row, stride), c);
         }
@@ -511,10 +514,14 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(values)>>;
         if (codes) {
             const Quad<uint8_t> q = FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c, j);
-            const B s = *reinterpret_cast<const B*>(at + 4 * V * T + (j * T + threadIdx.x) * sizeof(B));
+            const B s = reinterpret_cast<const B*>(at + 4 * V * T)[clique * V + j / kTogether];
             return decode4<B>(a.checkpoint, *reinterpret_cast<const uint32_t*>(&q), s);
         }
         return widen4<E>(Feed<E, LANES, V, MODE, T>::take(at, row_at(values, row, stride), c, j));
+    };
+    const auto issue_stats = [&](uint32_t at, const void* stats, uint32_t row) {
+        if (team.lane == 0)
+            copy_async<2 * sizeof(B)>(at + clique * 2 * (uint32_t)sizeof(B), static_cast<const B*>(stats) + 2 * (uint64_t)row);
     };
     const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
                    last = p.shared ? min(first + p.rows_per_team, rows) : rows;
@@ -525,15 +532,12 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
             if (NEXT) {
                 FB::issue(at + At::dh, row_at(dh, row, a.dh_stride), c);
                 issue_kept(at + At::x, a.x_codes, a.x_scales, x, a.x_stride, row);
-                copy_async<2 * sizeof(B)>(at + At::next_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
-                                          static_cast<const B*>(a.next_stats) + 2 * (uint64_t)row);
+                issue_stats(at + At::next_stats, a.next_stats, row);
             }
             if (BRANCH) {
                 issue_kept(at + At::y, a.y_codes, a.y_scales, y, a.y_stride, row);
                 if (row_gate) issue_kept(at + At::gate, a.gate_codes, a.gate_scales, gate, a.gate_stride, row);
-                if (a.post_norm != kNormNone)
-                    copy_async<2 * sizeof(B)>(at + At::post_stats + threadIdx.x * 2 * (uint32_t)sizeof(B),
-                                              static_cast<const B*>(a.post_stats) + 2 * (uint64_t)row);
+                if (a.post_norm != kNormNone) issue_stats(at + At::post_stats, a.post_stats, row);
             }
         }
         copies_commit();
@@ -552,6 +556,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
     for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
         issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
         copies_wait_oldest(p.stages);
+        __syncwarp();
         const bool live = row < last;
         if (LANES == 32 && !live) break;
         const char* at = ring + stage * p.stage_bytes;
@@ -564,7 +569,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
             Four<B> v[V], d[V], s0 = zero, s1 = zero;
             B rstd = B(0);
             if (live) {
-                const B* stats = reinterpret_cast<const B*>(at + At::next_stats + threadIdx.x * 2 * sizeof(B));
+                const B* stats = reinterpret_cast<const B*>(at + At::next_stats) + 2 * clique;
                 const B mean = stats[0];
                 rstd = stats[1];
 #pragma unroll
@@ -597,7 +602,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
             if (live) {
                 B mean = B(0);
                 if (a.post_norm != kNormNone) {
-                    const B* stats = reinterpret_cast<const B*>(at + At::post_stats + threadIdx.x * 2 * sizeof(B));
+                    const B* stats = reinterpret_cast<const B*>(at + At::post_stats) + 2 * clique;
                     mean = stats[0];
                     rstd = stats[1];
                 }
