@@ -133,6 +133,10 @@ __device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, MOD
     }
     return widen4<B>(q);
 }
+// four values in shared memory, in 16-byte pieces (the compiler splits a copy of the structure)
+template <typename B> __device__ __forceinline__ Four<B> from_shelf(const Four<B>* at) {
+    return widen4<B>(load_quad(at->v));
+}
 template <typename B, int LANES, int V, int MODE>
 __device__ __forceinline__ Four<B> get_or(const void* p, const Columns<LANES, V, MODE>& c, int j, B absent) {
     return p ? get(static_cast<const B*>(p) + c.col, c, j) : four<B>(absent);
@@ -579,7 +583,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                     v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);          // the normalised row
                     sum_nw[j] = fma4(d[j], v[j], sum_nw[j]);
                     sum_nb[j] = sum_nb[j] + d[j];
-                    d[j] = d[j] * nw[j * per_team];
+                    d[j] = d[j] * from_shelf(nw + j * per_team);
                     s0 = s0 + d[j];
                     s1 = fma4(d[j], v[j], s1);
                 }
@@ -615,7 +619,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                 for (int j = 0; j < V; ++j) {
                     v[j] = take_kept(at + At::y, a.y_codes, y, a.y_stride, row, j);
                     if (a.post_norm != kNormNone) v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);
-                    const Four<B> w = pw[j * per_team], sc = scale[j * per_team];
+                    const Four<B> w = from_shelf(pw + j * per_team), sc = from_shelf(scale + j * per_team);
                     Four<B> z = v[j] * w;
                     if (a.post_bias) z = z + get(pb, c, j);
                     if (p.shared || row_gate) {
@@ -682,7 +686,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                 shelf[threadIdx.x] = v[j];
                 __syncthreads();
                 if ((int)threadIdx.x >= per_team) continue;
-                for (int i = 1; i < p.teams_per_block; ++i) v[j] = v[j] + shelf[i * per_team + threadIdx.x];
+                for (int i = 1; i < p.teams_per_block; ++i) v[j] = v[j] + from_shelf(shelf + i * per_team + threadIdx.x);
             }
             put(row, c, j, v[j]);
         }
