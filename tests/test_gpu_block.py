@@ -440,6 +440,31 @@ def test_refusals_on_the_device():
         torch.autograd.grad(out.sum(), t, create_graph=True)
 
 
+def test_graph_is_used_once_and_inputs_stay():
+    """A second backward without retain_graph, and an input changed in between, are errors; forward mode is refused."""
+    x = stream(5, 64, torch.float32).requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for call in (lambda t: sk.block_norm(t, w), lambda t: sk.block_norm(t, w, checkpoint="int8"),
+                 lambda t: sk.gated_residual(t, t * 1.0, scale=w, post_norm="rms")):
+        out = call(x).sum()
+        out.backward(retain_graph=True)
+        out.backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            out.backward()
+    t = x.detach() * 1.0
+    t.requires_grad_()
+    out = sk.block_norm(t, w)
+    with torch.no_grad():
+        t.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+        for call in (lambda: sk.block_norm(dual), lambda: sk.gated_residual(x, dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
 def test_no_rows():
     for dtype in (torch.float32, torch.bfloat16):
         x = torch.zeros(0, 64, dtype=dtype, device="cuda", requires_grad=True)

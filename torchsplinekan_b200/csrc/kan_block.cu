@@ -11,6 +11,9 @@
 #include "kan_block_plan.h"
 
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 namespace kanb200 {
 namespace {
@@ -425,7 +428,7 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     // blocks to an SM by registers (the kernels' launch bounds) and shared memory, then up to four stages while there is room
     const int registers = 65536 / (ring_threads(p.big, false) * ring_blocks(p.big));
     int per_sm = std::max(1, 65536 / (registers * T));
-    const auto fits = [&](int stages) { return (stages * p.stage_bytes + p.parameter_bytes + 1024 + 768) * per_sm <= 228 * 1024; };
+    const auto fits = [&](int stages) { return stages * p.stage_bytes + p.parameter_bytes <= 228 * 1024 / per_sm - 228 * 1024 + kSharedBytes; };
     while (per_sm > 1 && !fits(2)) --per_sm;
     p.stages = 2;
     if (backward || !branch || !p.many)                  // (parameters in memory need L1)
@@ -528,6 +531,19 @@ cudaError_t launch_backward(const kanb200_block_args& a, const BackwardPlan& p, 
 }
 
 }  // namespace
+
+cudaError_t allow_shared_memory(const void* kernel) {
+    static std::mutex mutex;
+    static std::set<std::pair<const void*, int>> allowed;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mutex);
+    if (allowed.count({kernel, device})) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
+    if (e == cudaSuccess) allowed.insert({kernel, device});
+    return e;
+}
 
 cudaError_t block_forward(const kanb200_block_args& a, cudaStream_t st) {
     switch (a.dtype) {

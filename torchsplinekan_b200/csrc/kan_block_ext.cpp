@@ -8,7 +8,12 @@
 #include <ATen/TensorUtils.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
+#include <array>
+#include <cmath>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -19,7 +24,7 @@ namespace kan_ext {
 namespace {
 
 namespace py = pybind11;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 int stream_code(const Tensor& t, const char* what) {
@@ -138,6 +143,7 @@ struct NormSaved {
 
 Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind, double eps, int64_t checkpoint,
                     NormSaved* saved) {
+    at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     const at::ScalarType type = branch_type(x);
@@ -169,50 +175,66 @@ Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t k
     return h;
 }
 
-bool wants_grad(std::initializer_list<Tensor> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor& t : ts)
-        if (t.defined() && t.requires_grad()) return true;
-    return false;
+bool wants_grad(std::initializer_list<Tensor> ts, const char* what) {
+    bool wanted = false;
+    for (const Tensor& t : ts) {
+        if (!t.defined()) continue;
+        TORCH_CHECK(!t._fw_grad(0).defined(), what, ": forward-mode derivatives are not available");
+        wanted = wanted || t.requires_grad();
+    }
+    return wanted && at::GradMode::is_enabled();
 }
 
-// The autograd node's inputs must be defined tensors: an absent one is an empty tensor there.
-const Tensor& or_absent(const Tensor& t) {
-    static const Tensor& absent = *new Tensor(at::empty({0}));
-    return t.defined() ? t : absent;
+// The autograd nodes are written out instead of through torch::autograd::Function: on small calls its context (a
+// dictionary, generic wrapping of inputs and outputs) cost as much as the launch.
+struct SavedNode : public torch::autograd::Node {
+    std::vector<SavedVariable> saved;
+    bool released = false;
+
+    void keep(const Tensor& t, bool is_output = false) { saved.emplace_back(t, is_output); }
+    Tensor kept(size_t i) {
+        TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+        return saved[i].unpack(shared_from_this());
+    }
+    bool need(size_t i) const { return i < num_outputs() && task_should_compute_output(i); }
+    void release_variables() override {
+        released = true;
+        for (SavedVariable& v : saved) v.reset_data();
+    }
+};
+template <typename N> std::shared_ptr<N> new_node(std::initializer_list<Tensor> inputs) {
+    std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+    torch::autograd::edge_list edges;
+    edges.reserve(inputs.size());
+    for (const Tensor& t : inputs)
+        edges.push_back(t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge());
+    node->set_next_edges(std::move(edges));
+    return node;
 }
-Tensor present(const Tensor& t) { return has(t) ? t : Tensor(); }
+int type_code(at::ScalarType t) {
+    return t == at::kFloat ? KANB200_F32 : t == at::kDouble ? KANB200_F64 : t == at::kHalf ? KANB200_F16 : KANB200_BF16;
+}
 
 Tensor or_undefined(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
-struct BlockNorm : public torch::autograd::Function<BlockNorm> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind,
-                          double eps, int64_t checkpoint) {
-        NormSaved s;
-        const Tensor weight = present(w);
-        Tensor h = norm_forward(x, weight, present(b), kind, eps, checkpoint, &s);
-        ctx->saved_data["kind"] = kind;
-        ctx->saved_data["eps"] = eps;
-        ctx->saved_data["checkpoint"] = checkpoint;
-        ctx->saved_data["shape"] = x.sizes().vec();
-        ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
-        ctx->save_for_backward({checkpoint != KANB200_PACK_NONE ? Tensor() : x, weight, s.stats, s.packed.codes, s.packed.scales});
-        return h;
-    }
+struct BlockNormNode : public SavedNode {
+    int64_t kind = 0, checkpoint = 0;
+    double eps = 0;
+    at::ScalarType type = at::kFloat;                       // of the stream
+    std::vector<int64_t> shape;
+    std::string name() const override { return "BlockNormBackward"; }
 
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &stats = saved[2], &codes = saved[3], &scales = saved[4];
-        const int64_t kind = ctx->saved_data["kind"].toInt(), checkpoint = ctx->saved_data["checkpoint"].toInt();
-        const double eps = ctx->saved_data["eps"].toDouble();
-        const auto shape = ctx->saved_data["shape"].toIntVector();
-        const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
-        Tensor dx, dw, db;
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list result(3);
+        if (!grads[0].defined()) return result;
+        const Tensor x = kept(0), w = kept(1), stats = kept(2), codes = kept(3), scales = kept(4);
         if (at::GradMode::is_enabled()) {
             TORCH_CHECK(checkpoint == KANB200_PACK_NONE,
                         "block_norm: create_graph=True needs the input itself, not its 8-bit checkpoint");
-            std::tie(dx, dw, db) = norm_gradient(x.to(branch_type(x)), w, grads[0], kind, eps);
-            return {dx.to(x.scalar_type()), dw, db, Tensor(), Tensor(), Tensor()};
+            std::tie(result[0], result[1], result[2]) = norm_gradient(x.to(branch_type(x)), w, grads[0], kind, eps);
+            result[0] = result[0].to(type);
+            return result;
         }
         c10::cuda::CUDAGuard guard(stats.device());
         const cudaStream_t st = at::cuda::getCurrentCUDAStream();
@@ -220,11 +242,10 @@ struct BlockNorm : public torch::autograd::Function<BlockNorm> {
         a.width = shape.back();
         a.rows = stats.size(0);
         const Rows xr = as_rows(x, a.rows, a.width), dr = as_rows(grads[0], a.rows, a.width);
-        if (ctx->needs_input_grad(0)) dx = at::empty(shape, stats.options().dtype(type));
-        if (ctx->needs_input_grad(1)) dw = at::empty({a.width}, stats.options());
-        if (ctx->needs_input_grad(2)) db = at::empty({a.width}, stats.options());
-        a.dtype = type == at::kFloat ? KANB200_F32 : type == at::kDouble ? KANB200_F64
-                  : type == at::kHalf ? KANB200_F16 : KANB200_BF16;
+        if (need(0)) result[0] = at::empty(shape, stats.options().dtype(type));
+        if (need(1)) result[1] = at::empty({a.width}, stats.options());
+        if (need(2)) result[2] = at::empty({a.width}, stats.options());
+        a.dtype = type_code(type);
         a.next_norm = (int)kind;
         a.checkpoint = (int)checkpoint;
         a.eps = eps;
@@ -237,11 +258,11 @@ struct BlockNorm : public torch::autograd::Function<BlockNorm> {
         a.x_scales = const_cast<void*>(cptr(scales));
         a.dh = dr.ptr();
         a.dh_stride = dr.stride;
-        a.dx = mptr(dx);
-        a.dnext_weight = mptr(dw);
-        a.dnext_bias = mptr(db);
+        a.dx = mptr(result[0]);
+        a.dnext_weight = mptr(result[1]);
+        a.dnext_bias = mptr(result[2]);
         run_backward(a, stats, st);
-        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+        return result;
     }
 };
 
@@ -251,8 +272,19 @@ Tensor block_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     check_norm(x, w, b, kind, eps, checkpoint);
     TORCH_CHECK(x.is_cuda() || checkpoint == KANB200_PACK_NONE, "block_norm: 8-bit checkpoints need CUDA tensors");
     if (!x.is_cuda() || x.numel() == 0) return norm_composite(x, w, b, kind, eps);
-    if (!wants_grad({x, w, b})) return norm_forward(x, w, b, kind, eps, checkpoint, nullptr);
-    return BlockNorm::apply(x, or_absent(w), or_absent(b), kind, eps, checkpoint);
+    if (!wants_grad({x, w, b}, "block_norm")) return norm_forward(x, w, b, kind, eps, checkpoint, nullptr);
+    NormSaved s;
+    Tensor h = norm_forward(x, w, b, kind, eps, checkpoint, &s);
+    auto node = new_node<BlockNormNode>({x, w, b});
+    node->kind = kind;
+    node->eps = eps;
+    node->checkpoint = checkpoint;
+    node->type = x.scalar_type();
+    node->shape = x.sizes().vec();
+    for (const Tensor& t : {checkpoint != KANB200_PACK_NONE ? Tensor() : x, w, s.stats, s.packed.codes, s.packed.scales})
+        node->keep(t);
+    torch::autograd::set_history(h, node);
+    return h;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -333,9 +365,19 @@ variable_list gated_composite(const Gated& g) {
 }
 
 struct GatedSaved {
-    Tensor post_stats, next_stats;
+    Tensor stats;                                            // [norms, rows, 2], the post norm's first
     Packed y, gate, out;
 };
+// the two norms' parts of it
+void stats_of(kanb200_block_args& a, const Tensor& stats, int64_t post, int64_t next) {
+    if (!stats.defined()) return;
+    char* at = static_cast<char*>(const_cast<void*>(cptr(stats)));
+    if (post != KANB200_NORM_NONE) {
+        a.post_stats = at;
+        at += a.rows * 2 * stats.element_size();
+    }
+    if (next != KANB200_NORM_NONE) a.next_stats = at;
+}
 
 void fill(kanb200_block_args& a, const Gated& g) {
     a.gate_act = (int)g.act;
@@ -361,6 +403,7 @@ void branch_rows(const Gated& g, Rows& y, const void*& gate, int64_t& gate_strid
 }
 
 variable_list gated_forward(const Gated& g, GatedSaved* saved) {
+    at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(g.x.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     const at::ScalarType type = branch_type(g.x);
@@ -371,10 +414,9 @@ variable_list gated_forward(const Gated& g, GatedSaved* saved) {
     fill(a, g);
     a.dtype = stream_code(g.x, "gated_residual");
     if (saved) {
-        if (g.post != KANB200_NORM_NONE) saved->post_stats = at::empty({g.rows, 2}, branch);
-        if (h.defined()) saved->next_stats = at::empty({g.rows, 2}, branch);
-        a.post_stats = mptr(saved->post_stats);
-        a.next_stats = mptr(saved->next_stats);
+        const int64_t norms = (g.post != KANB200_NORM_NONE) + (g.next != KANB200_NORM_NONE);
+        if (norms) saved->stats = at::empty({norms, g.rows, 2}, branch);
+        stats_of(a, saved->stats, g.post, g.next);
         if (g.checkpoint != KANB200_PACK_NONE) {
             a.checkpoint = (int)g.checkpoint;
             saved->y = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
@@ -416,61 +458,26 @@ variable_list gated_forward(const Gated& g, GatedSaved* saved) {
 // needs_input_grad / result slots
 enum { kX, kY, kGate, kScale, kPostWeight, kPostBias, kNextWeight, kNextBias, kGatedInputs };
 
-struct GatedResidual : public torch::autograd::Function<GatedResidual> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& y, const Tensor& gate,
-                                 const Tensor& scale, const Tensor& pw, const Tensor& pb, const Tensor& nw,
-                                 const Tensor& nb, bool packed, int64_t act, int64_t post, int64_t next, double eps,
-                                 int64_t checkpoint) {
-        Gated g{x, y, present(gate), present(scale), present(pw), present(pb), present(nw), present(nb),
-                packed, act, post, next, checkpoint, eps};
-        check_gated(g);
-        GatedSaved s;
-        variable_list outs = gated_forward(g, &s);
-        ctx->set_materialize_grads(false);
-        auto& d = ctx->saved_data;
-        d["packed"] = packed;
-        d["act"] = act;
-        d["post"] = post;
-        d["next"] = next;
-        d["eps"] = eps;
-        d["checkpoint"] = checkpoint;
-        d["gate_rows"] = g.gate_rows;
-        d["shape"] = x.sizes().vec();
-        d["dtype"] = (int64_t)x.scalar_type();
-        d["gate_shape"] = gate.sizes().vec();
-        const bool codes = checkpoint != KANB200_PACK_NONE;
-        const bool keep_gate = !codes || g.gate_rows > 1;
-        ctx->save_for_backward({next != KANB200_NORM_NONE && !codes ? outs[0] : Tensor(), codes ? Tensor() : y,
-                                keep_gate ? g.gate : Tensor(), g.scale, g.pw, g.pb, g.nw, s.post_stats, s.next_stats,
-                                s.out.codes, s.out.scales, s.y.codes, s.y.scales, s.gate.codes, s.gate.scales});
-        return outs;
-    }
+struct GatedResidualNode : public SavedNode {
+    Gated settings;                                          // without tensors
+    at::ScalarType type = at::kFloat;                        // of the stream
+    std::vector<int64_t> shape, gate_shape;
+    std::string name() const override { return "GatedResidualBackward"; }
 
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto v = ctx->get_saved_variables();
-        auto& d = ctx->saved_data;
-        Gated g;
-        g.packed = d["packed"].toBool();
-        g.act = d["act"].toInt();
-        g.post = d["post"].toInt();
-        g.next = d["next"].toInt();
-        g.eps = d["eps"].toDouble();
-        g.checkpoint = d["checkpoint"].toInt();
-        g.gate_rows = d["gate_rows"].toInt();
-        const auto shape = d["shape"].toIntVector(), gate_shape = d["gate_shape"].toIntVector();
-        const auto type = (at::ScalarType)d["dtype"].toInt();
-        g.width = shape.back();
-        g.rows = 1;
-        for (size_t i = 0; i + 1 < shape.size(); ++i) g.rows *= shape[i];
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list result(kGatedInputs);
+        const Tensor dout = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
+        if (!dout.defined() && !dh.defined()) return result;
+        std::array<Tensor, 14> v;
+        for (size_t i = 0; i < v.size(); ++i) v[i] = kept(i);
+        Gated g = settings;
         g.y = v[1];
         g.gate = v[2];
         g.scale = v[3];
         g.pw = v[4];
         g.pb = v[5];
         g.nw = v[6];
-        const Tensor dout = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
-        variable_list result(kGatedInputs + 6);
-        if (!dout.defined() && !dh.defined()) return result;
         if (at::GradMode::is_enabled()) {
             TORCH_CHECK(g.checkpoint == KANB200_PACK_NONE,
                         "gated_residual: create_graph=True needs the inputs themselves, not their 8-bit checkpoints");
@@ -484,11 +491,9 @@ struct GatedResidual : public torch::autograd::Function<GatedResidual> {
         kanb200_block_args a{};
         fill(a, g);
         if (!dh.defined()) a.next_norm = KANB200_NORM_NONE;
-        a.dtype = type == at::kFloat ? KANB200_F32 : type == at::kDouble ? KANB200_F64
-                  : type == at::kHalf ? KANB200_F16 : KANB200_BF16;
+        a.dtype = type_code(type);
         a.has_branch = 1;
         a.checkpoint = (int)g.checkpoint;
-        const auto need = [&](int i) { return ctx->needs_input_grad(i); };
         Tensor dx, dy, dgate;
         if (need(kX)) {
             // without a norm behind, the stream's gradient passes through unchanged
@@ -533,16 +538,15 @@ struct GatedResidual : public torch::autograd::Function<GatedResidual> {
         a.post_weight = cptr(pw);
         a.post_bias = cptr(pb);
         if (dh.defined()) a.next_weight = cptr(nw);
-        a.post_stats = const_cast<void*>(cptr(v[7]));
-        a.next_stats = const_cast<void*>(cptr(v[8]));
+        stats_of(a, v[7], g.post, g.next);
         if (dh.defined()) {
-            a.x_codes = const_cast<void*>(cptr(v[9]));
-            a.x_scales = const_cast<void*>(cptr(v[10]));
+            a.x_codes = const_cast<void*>(cptr(v[8]));
+            a.x_scales = const_cast<void*>(cptr(v[9]));
         }
-        a.y_codes = const_cast<void*>(cptr(v[11]));
-        a.y_scales = const_cast<void*>(cptr(v[12]));
-        a.gate_codes = const_cast<void*>(cptr(v[13]));
-        a.gate_scales = const_cast<void*>(cptr(v[14]));
+        a.y_codes = const_cast<void*>(cptr(v[10]));
+        a.y_scales = const_cast<void*>(cptr(v[11]));
+        a.gate_codes = const_cast<void*>(cptr(v[12]));
+        a.gate_scales = const_cast<void*>(cptr(v[13]));
         a.dout = dor.ptr();
         a.dout_stride = dor.stride;
         a.dh = dhr.ptr();
@@ -607,11 +611,26 @@ py::object gated_residual(const Tensor& x, const Tensor& y, const std::optional<
     variable_list outs;
     if (!x.is_cuda() || x.numel() == 0) {
         outs = gated_composite(g);
-    } else if (!wants_grad({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb})) {
+    } else if (!wants_grad({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb}, "gated_residual")) {
         outs = gated_forward(g, nullptr);
     } else {
-        outs = GatedResidual::apply(g.x, g.y, or_absent(g.gate), or_absent(g.scale), or_absent(g.pw), or_absent(g.pb),
-                                    or_absent(g.nw), or_absent(g.nb), packed, act, post, next, eps, checkpoint);
+        GatedSaved saved;
+        outs = gated_forward(g, &saved);
+        auto node = new_node<GatedResidualNode>({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb});
+        node->settings = g;
+        for (Tensor Gated::*t : {&Gated::x, &Gated::y, &Gated::gate, &Gated::scale, &Gated::pw, &Gated::pb, &Gated::nw, &Gated::nb})
+            node->settings.*t = Tensor();
+        node->type = x.scalar_type();
+        node->shape = x.sizes().vec();
+        if (g.gate.defined()) node->gate_shape = g.gate.sizes().vec();
+        for (Tensor& t : outs) torch::autograd::set_history(t, node);
+        const bool codes = checkpoint != KANB200_PACK_NONE, keep_gate = !codes || g.gate_rows > 1;
+        node->saved.reserve(14);
+        node->keep(next != KANB200_NORM_NONE && !codes ? outs[0] : Tensor(), true);
+        for (const Tensor& t : {codes ? Tensor() : g.y, keep_gate ? g.gate : Tensor(), g.scale, g.pw, g.pb, g.nw, saved.stats,
+                                saved.out.codes, saved.out.scales, saved.y.codes, saved.y.scales, saved.gate.codes,
+                                saved.gate.scales})
+            node->keep(t);
     }
     if (outs.size() == 1) return py::cast(outs[0]);
     return py::make_tuple(outs[0], outs[1]);

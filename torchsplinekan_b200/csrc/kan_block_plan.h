@@ -10,6 +10,8 @@
 namespace kanb200 {
 
 constexpr int kSms = 148;
+// Dynamic shared memory of a ring kernel's block: 228 KB of an SM less 1 KB per block and the kernel's own 768 bytes.
+constexpr int kSharedBytes = 227 * 1024 - 768;
 
 // Sums over rows that the backward returns, one slab each.
 enum { kSumScale, kSumPostWeight, kSumPostBias, kSumNextWeight, kSumNextBias, kColumnSums };
@@ -75,6 +77,9 @@ template <bool NEXT, bool BRANCH, int V, int T, bool VEC, int S, int B> struct B
     static constexpr int gate = dout + ring_bytes(S, VEC, V, T);
     static constexpr int end = gate + ring_kept_bytes(B, VEC, V, T, B);
 };
+
+// Lets a kernel have all of a block's shared memory on the current device; remembers the kernels that may.
+cudaError_t allow_shared_memory(const void* kernel);
 
 template <typename S> cudaError_t ring_forward(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st);
 template <typename S>

@@ -171,6 +171,8 @@ struct TeamScratch {                       // per block, in shared memory
     double block[2][kMaxSums][kMaxCluster];
 };
 
+static_assert(sizeof(TeamScratch) == 768, "kSharedBytes");
+
 template <typename B, int LANES, bool BIG> struct Team {
     TeamScratch* scratch;
     int warps, team, warp, lane;           // warps of this block in a row's team; team and warp within the team
@@ -710,10 +712,10 @@ namespace kanb200 {
 template <typename... P>
 cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...), const P&... args) {
     const int bytes = p.stages * p.stage_bytes + p.parameter_bytes;
-    cudaError_t e = cudaSuccess;
-    if (bytes > 48 * 1024 - (int)sizeof(TeamScratch))
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
+    if (bytes > 48 * 1024 - (int)sizeof(TeamScratch)) {
+        const cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel));
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)p.blocks);
     cfg.blockDim = dim3((unsigned)p.threads);
