@@ -47,7 +47,8 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     kind_code = _code(NORMS, "kind", kind)
     if kind_code == 0:
         raise ValueError("kind must be 'rms' or 'layer', got None")
-    return _C.block_norm(x, weight, bias, kind_code, eps, _code(CHECKPOINTS, "checkpoint", checkpoint))
+    return _C.block_norm(x, weight, bias, kind_code, eps, 0 if checkpoint is None else
+                         _code(CHECKPOINTS, "checkpoint", checkpoint))
 
 
 def gated_residual(x: torch.Tensor, y: torch.Tensor, *, gate: Union[torch.Tensor, str, None] = None,

@@ -210,6 +210,21 @@ __device__ __forceinline__ Four<double> operator*(const Four<double>& x, const F
 __device__ __forceinline__ Four<double> fma4(const Four<double>& x, const Four<double>& y, const Four<double>& z) {
     return {{fma(x.v[0], y.v[0], z.v[0]), fma(x.v[1], y.v[1], z.v[1]), fma(x.v[2], y.v[2], z.v[2]), fma(x.v[3], y.v[3], z.v[3])}};
 }
+// max(top, |x|), NaN if any is
+__device__ __forceinline__ float max_abs(float top, const Four<float>& x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(x.v[e])));
+    return top;
+}
+__device__ __forceinline__ double max_abs(double top, const Four<double>& x) {
+    unsigned long long t = AbsBits<double>::of(top);         // |x| as an integer orders like |x| with NaN on top
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned long long v = AbsBits<double>::of(x.v[e]);
+        t = v > t ? v : t;
+    }
+    return AbsBits<double>::back(t);
+}
 template <typename B> __device__ __forceinline__ B total(const Four<B>& x) { return (x.v[0] + x.v[2]) + (x.v[1] + x.v[3]); }
 
 template <typename S> __device__ __forceinline__ Four<Br<S>> widen4(const Quad<S>& q) {

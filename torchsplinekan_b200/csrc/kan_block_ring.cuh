@@ -263,12 +263,10 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], con
     Bits mine = 0;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-        Bits top = 0;
+        B largest = B(0);                                   // columns beyond the row hold 0
 #pragma unroll
-        for (int j = i * kTogether; j < (i + 1) * kTogether; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, AbsBits<B>::of(c.ok(j, e) ? v[j].v[e] : B(0)));
-        top = lanes_max<LANES>(top);
+        for (int j = i * kTogether; j < (i + 1) * kTogether; ++j) largest = max_abs(largest, v[j]);
+        const Bits top = lanes_max<LANES>(AbsBits<B>::of(largest));
         if (kGroups == 1 || lane % kGroups == i) mine = top;
     }
     const B scale = pack_scale<B>(format, AbsBits<B>::back(mine)), inverse = pack_inverse<B>(scale);

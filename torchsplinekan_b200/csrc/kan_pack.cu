@@ -24,7 +24,7 @@ template <int LANES, bool VEC> struct Run {
         if (LANES == 32) {
             groups = (width + kPackGroup - 1) / kPackGroup;
             const int64_t first = warp * kRun;
-            row = first / groups;
+            row = first >> 32 ? first / groups : (uint32_t)first / (uint32_t)groups;
             group = (int)(first - row * groups);
         } else {
             groups = 1;
@@ -46,14 +46,15 @@ template <int LANES, bool VEC> struct Run {
 };
 
 template <typename S, int LANES, bool VEC>
-__global__ void __launch_bounds__(kThreads) pack_kernel(int format, const S* __restrict__ x, int64_t x_stride,
+__global__ void __launch_bounds__(kThreads, sizeof(S) == 8 ? 3 : 6) pack_kernel(int format, const S* __restrict__ x, int64_t x_stride,
                                                        uint8_t* __restrict__ codes, Br<S>* __restrict__ scales,
                                                        int64_t rows, int width) {
     using B = Br<S>;
     using Bits = typename AbsBits<B>::type;
     Four<B> v[kRun];
+    const Run<LANES, VEC> start(rows, width);
     {
-        Run<LANES, VEC> r(rows, width);
+        Run<LANES, VEC> r = start;
 #pragma unroll
         for (int i = 0; i < kRun; ++i, r.next()) {
             Quad<S> q{};
@@ -67,14 +68,11 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(int format, const S* __r
             v[i] = widen4<S>(q);
         }
     }
-    Run<LANES, VEC> r(rows, width);
+    Run<LANES, VEC> r = start;
     Bits mine = 0;
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-        Bits top = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, AbsBits<B>::of(v[i].v[e]));
-        top = lanes_max<LANES>(top);
+        const Bits top = lanes_max<LANES>(AbsBits<B>::of(max_abs(B(0), v[i])));
         if (r.lane % kRun == i) mine = top;
     }
     const B scale = pack_scale<B>(format, AbsBits<B>::back(mine)), inverse = pack_inverse<B>(scale);
@@ -101,8 +99,9 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(int format, const uint
     using B = Br<S>;
     uint32_t word[kRun];
     B scale[kRun];
+    const Run<LANES, VEC> start(rows, width);
     {
-        Run<LANES, VEC> r(rows, width);
+        Run<LANES, VEC> r = start;
 #pragma unroll
         for (int i = 0; i < kRun; ++i, r.next()) {
             const uint8_t* at = codes + r.row * width + r.column(0);
@@ -117,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(int format, const uint
             scale[i] = r.row < rows ? scales[r.scale_at()] : B(0);
         }
     }
-    Run<LANES, VEC> r(rows, width);
+    Run<LANES, VEC> r = start;
 #pragma unroll
     for (int i = 0; i < kRun; ++i, r.next()) {
         const Quad<S> q = narrow4<S>(decode4<B>(format, word[i], scale[i]));
