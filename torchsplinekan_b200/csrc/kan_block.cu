@@ -367,7 +367,7 @@ Team team_for(const kanb200_block_args& a, bool backward) {
     Team t{};
     t.many = !branch;
     const auto cover = [&] {
-        t.chunks = ring_chunks(t.many, f64);
+        t.chunks = ring_chunks(t.many, t.big, f64);
         t.warps = (int)div_up(a.width, kPackGroup * t.chunks);
     };
     cover();
@@ -375,7 +375,10 @@ Team team_for(const kanb200_block_args& a, bool backward) {
         t.many = true;
         cover();
     }
-    t.big = t.warps > 8;
+    if (t.warps > 8) {
+        t.big = true;
+        cover();
+    }
     t.cluster = 1;
     const int all = t.warps, most = ring_threads(t.big, f64) / 32;
     while (div_up(all, t.cluster) > most) t.cluster *= 2;
@@ -426,7 +429,7 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.parameter_bytes = backward ? ((a.dh ? 1 : 0) + (branch ? 2 : 0)) * (p.threads / p.teams_per_block) * 4 * V * B : 0;
 
     // blocks to an SM by registers (the kernels' launch bounds) and shared memory, then up to four stages while there is room
-    const int registers = 65536 / (ring_threads(p.big, false) * ring_blocks(p.big));
+    const int registers = 65536 / (ring_threads(p.big, false) * ring_blocks(p.big, B == 8));
     int per_sm = std::max(1, 65536 / (registers * T));
     const auto fits = [&](int stages) { return stages * p.stage_bytes + p.parameter_bytes <= 228 * 1024 / per_sm - 228 * 1024 + kSharedBytes; };
     while (per_sm > 1 && !fits(2)) --per_sm;

@@ -42,63 +42,59 @@ __device__ __forceinline__ void copies_wait_oldest(int stages) {
     else copies_wait<3>();
 }
 
-// Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other; a thread has four of each,
-// side by side (kFull, kVector: rows, strides and pointers allow four elements at once) or LANES apart (kScalar).  kFull:
-// the team's columns are exactly the row's, so nothing is masked (a third of the instructions of the gated backward were
-// predicates, selects and zeros).  Distances between a thread's elements are constants, so a row costs one address per tensor.
-template <int LANES, int V, int MODE> struct Columns {
+// Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other.  A thread has four of each:
+// runs of SIDE columns, 16 bytes of the branch's type (kFull, kVector: rows, strides and pointers allow four elements at
+// once; float64: two runs, so that the lanes' accesses stay side by side) or single ones (kScalar).  kFull: the team's
+// columns are exactly the row's, so nothing is masked (a third of the instructions of the gated backward were predicates,
+// selects and zeros).  Distances between a thread's elements are constants, so a row costs one address per tensor.
+template <int LANES_, int V_, int MODE_, int SIDE_> struct Columns {
+    static constexpr int LANES = LANES_, V = V_, MODE = MODE_, SIDE = SIDE_;
     int col, width;
     static __device__ __forceinline__ constexpr int apart(int j, int e) {
-        return j * 4 * LANES + (MODE != kScalar ? e : LANES * e);
+        return j * 4 * LANES + e / SIDE * SIDE * LANES + e % SIDE;
     }
     __device__ __forceinline__ int at(int j, int e) const { return col + apart(j, e); }
-    __device__ __forceinline__ bool ok(int j, int e) const { return MODE == kFull || at(j, MODE == kScalar ? e : 0) < width; }
+    __device__ __forceinline__ bool ok(int j, int e) const { return MODE == kFull || at(j, e / SIDE * SIDE) < width; }
 };
 
-// ---- rows <-> registers -----------------------------------------------------------------------------------------------
-// A thread's elements of one tensor on their way from a row in memory to registers.  Types of less than 4 bytes that
-// cannot be copied four at a time have no ring slot: they are loaded where they are used.  T is the block's most threads:
-// a slot's pieces are arrays over T threads, so that all distances in a stage are constants too.  Places of columns beyond
-// the row hold 0 (clear_ring) and are never written.  `row` points to the thread's own first element.
-template <typename E, int LANES, int V, int MODE, int T> struct Feed {
-    using Cols = Columns<LANES, V, MODE>;
-    static constexpr bool VEC = MODE != kScalar;
-    static constexpr bool kRing = VEC || sizeof(E) >= 4;
-    static constexpr int kPiece = VEC ? (4 * sizeof(E) > 16 ? 16 : 4 * (int)sizeof(E)) : (int)sizeof(E);
-    static constexpr int kPieces = 4 * (int)sizeof(E) / kPiece;             // per chunk
-    static constexpr int kBytes = kRing ? 4 * (int)sizeof(E) * V * T : 0;   // of a stage
+// BYTES consecutive bytes as one access
+template <int BYTES> __device__ __forceinline__ void move(void* dst, const void* src) {
+    using T = std::conditional_t<BYTES == 16, float4, std::conditional_t<BYTES == 8, float2, std::conditional_t<
+                  BYTES == 4, uint32_t, std::conditional_t<BYTES == 2, uint16_t, uint8_t>>>>;
+    *static_cast<T*>(dst) = *static_cast<const T*>(src);
+}
 
-    static __device__ __forceinline__ void issue(uint32_t stage, const E* row, const Cols& c) {
-        if constexpr (!kRing) return;
-        const uint32_t dst = stage + threadIdx.x * kPiece;
+// ---- rows <-> registers -----------------------------------------------------------------------------------------------
+// A thread's elements of one tensor on their way from a row in memory to registers, run by run.  Runs of less than 4 bytes
+// have no ring slot: they are loaded where they are used.  T is the block's most threads: a slot's runs are arrays over T
+// threads, so that all distances in a stage are constants too.  Places of columns beyond the row hold 0 (clear_ring) and are
+// never written.  `row` points to the thread's own first element.
+template <typename E, typename C, int T> struct Feed {
+    static constexpr int kRun = C::SIDE * (int)sizeof(E), kRuns = 4 / C::SIDE;
+    static constexpr bool kRing = kRun >= 4;
+
+    static __device__ __forceinline__ void issue(uint32_t stage, const E* row, const C& c) {
+        if constexpr (kRing) {
+            const uint32_t dst = stage + threadIdx.x * kRun;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if constexpr (VEC) {
-                if (c.ok(j, 0))
+            for (int j = 0; j < C::V; ++j)
 #pragma unroll
-                    for (int p = 0; p < kPieces; ++p)
-                        copy_async<kPiece>(dst + (j * kPieces + p) * T * kPiece,
-                                           reinterpret_cast<const char*>(row + Cols::apart(j, 0)) + p * kPiece);
-            } else if constexpr (kRing) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c.ok(j, e)) copy_async<kPiece>(dst + (4 * j + e) * T * kPiece, row + Cols::apart(j, e));
-            }
+                for (int r = 0; r < kRuns; ++r)
+                    if (c.ok(j, r * C::SIDE)) copy_async<kRun>(dst + (j * kRuns + r) * T * kRun, row + C::apart(j, r * C::SIDE));
         }
     }
-    static __device__ __forceinline__ Quad<E> take(const char* stage, const E* row, const Cols& c, int j) {
-        const char* src = stage + threadIdx.x * kPiece;
+    static __device__ __forceinline__ Quad<E> take(const char* stage, const E* row, const C& c, int j) {
+        const char* src = stage + threadIdx.x * kRun;
         Quad<E> q;
-        if constexpr (VEC && kPieces == 2) {
-            reinterpret_cast<float4*>(&q)[0] = *reinterpret_cast<const float4*>(src + (2 * j) * T * kPiece);
-            reinterpret_cast<float4*>(&q)[1] = *reinterpret_cast<const float4*>(src + (2 * j + 1) * T * kPiece);
-        } else if constexpr (VEC) {
-            q = *reinterpret_cast<const Quad<E>*>(src + j * T * kPiece);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (kRing) q.v[e] = *reinterpret_cast<const E*>(src + (4 * j + e) * T * kPiece);
-                else q.v[e] = c.ok(j, e) ? row[Cols::apart(j, e)] : E{};
+        for (int r = 0; r < kRuns; ++r) {
+            E* to = q.v + r * C::SIDE;
+            if constexpr (kRing) {
+                move<kRun>(to, src + (j * kRuns + r) * T * kRun);
+            } else {
+#pragma unroll
+                for (int e = 0; e < C::SIDE; ++e) to[e] = E{};
+                if (c.ok(j, r * C::SIDE)) move<kRun>(to, row + C::apart(j, r * C::SIDE));
             }
         }
         return q;
@@ -106,50 +102,50 @@ template <typename E, int LANES, int V, int MODE, int T> struct Feed {
 };
 
 // `row`: the thread's own first element, here and below
-template <typename T, int LANES, int V, int MODE>
-__device__ __forceinline__ void put(T* row, const Columns<LANES, V, MODE>& c, int j, const Quad<T>& q) {
-    if constexpr (MODE != kScalar) {
-        if (c.ok(j, 0)) store_quad(row + c.apart(j, 0), q);
-    } else {
+template <typename T, typename C> __device__ __forceinline__ void put(T* row, const C& c, int j, const Quad<T>& q) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c.ok(j, e)) row[c.apart(j, e)] = q.v[e];
-    }
+    for (int r = 0; r < 4; r += C::SIDE)
+        if (c.ok(j, r)) move<C::SIDE * (int)sizeof(T)>(row + C::apart(j, r), q.v + r);
 }
-template <typename B, int LANES, int V, int MODE>
-__device__ __forceinline__ void put(B* row, const Columns<LANES, V, MODE>& c, int j, const Four<B>& x) {
+template <typename B, typename C> __device__ __forceinline__ void put(B* row, const C& c, int j, const Four<B>& x) {
     put(row, c, j, Quad<B>{{x.v[0], x.v[1], x.v[2], x.v[3]}});
 }
 // Four values of a parameter (or a shared gate row); 0 beyond the row.
-template <typename B, int LANES, int V, int MODE>
-__device__ __forceinline__ Four<B> get(const B* row, const Columns<LANES, V, MODE>& c, int j) {
+template <typename B, typename C> __device__ __forceinline__ Four<B> get(const B* row, const C& c, int j) {
     Quad<B> q{};
-    if constexpr (MODE != kScalar) {
-        if (c.ok(j, 0)) q = load_quad(row + c.apart(j, 0));
-    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c.ok(j, e)) q.v[e] = row[c.apart(j, e)];
-    }
+    for (int r = 0; r < 4; r += C::SIDE)
+        if (c.ok(j, r)) move<C::SIDE * (int)sizeof(B)>(q.v + r, row + C::apart(j, r));
     return widen4<B>(q);
 }
-// four values in shared memory, in 16-byte pieces (the compiler splits a copy of the structure)
-template <typename B> __device__ __forceinline__ Four<B> from_shelf(const Four<B>* at) {
-    return widen4<B>(load_quad(at->v));
-}
-template <typename B, int LANES, int V, int MODE>
-__device__ __forceinline__ Four<B> get_or(const void* p, const Columns<LANES, V, MODE>& c, int j, B absent) {
+template <typename B, typename C> __device__ __forceinline__ Four<B> get_or(const void* p, const C& c, int j, B absent) {
     return p ? get(static_cast<const B*>(p) + c.col, c, j) : four<B>(absent);
 }
 // x - mean for the row's own columns; 0 beyond them, where x is 0
-template <typename B, int LANES, int V, int MODE>
-__device__ __forceinline__ Four<B> centre(const Columns<LANES, V, MODE>& c, int j, const Four<B>& x, B mean) {
+template <typename B, typename C> __device__ __forceinline__ Four<B> centre(const C& c, int j, const Four<B>& x, B mean) {
     Four<B> m = four<B>(-mean);
-    if constexpr (MODE == kVector) m = four<B>(c.ok(j, 0) ? -mean : B(0));
-    if constexpr (MODE == kScalar)
+    if constexpr (C::MODE != kFull)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m.v[e] = c.ok(j, e) ? -mean : B(0);
+        for (int r = 0; r < 4; r += C::SIDE) {
+            const B own = c.ok(j, r) ? -mean : B(0);
+#pragma unroll
+            for (int e = 0; e < C::SIDE; ++e) m.v[r + e] = own;
+        }
     return x + m;
+}
+// A parameter's values in shared memory: 16-byte pieces, arrays over the threads of a team.  `at`: the thread's first piece.
+template <typename B> __device__ __forceinline__ void to_shelf(char* at, int threads, int j, const Four<B>& x) {
+    constexpr int kPieces = 4 * sizeof(B) / 16;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+        move<16>(at + (j * kPieces + p) * threads * 16, reinterpret_cast<const char*>(x.v) + 16 * p);
+}
+template <typename B> __device__ __forceinline__ Four<B> from_shelf(const char* at, int threads, int j) {
+    constexpr int kPieces = 4 * sizeof(B) / 16;
+    Quad<B> q;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) move<16>(reinterpret_cast<char*>(q.v) + 16 * p, at + (j * kPieces + p) * threads * 16);
+    return widen4<B>(q);
 }
 __device__ __forceinline__ void clear_ring(char* ring, int bytes) {
     for (int at = threadIdx.x * 16; at < bytes; at += blockDim.x * 16)
@@ -223,9 +219,9 @@ template <typename T> __device__ __forceinline__ T* row_at(T* base, uint32_t row
 }
 
 // The team's place: its first column, and its first row.
-template <int LANES, int V, int MODE, bool BIG, typename B>
-__device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, LANES, BIG>& team,
-                                           Columns<LANES, V, MODE>& c) {
+template <bool BIG, typename B, typename C>
+__device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, C::LANES, BIG>& team, C& c) {
+    constexpr int LANES = C::LANES, V = C::V;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     team.scratch = scratch;
     team.cluster = BIG ? p.cluster : 1;
@@ -237,27 +233,30 @@ __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScr
         team.team = p.teams_per_block == 1 ? 0 : warp / p.warps;
         team.warp = warp - team.team * p.warps;
         team.lane = lane;
-        c.col = (team.rank * p.warps + team.warp) * V * kPackGroup + (MODE != kScalar ? 4 * lane : lane);
+        c.col = (team.rank * p.warps + team.warp) * V * kPackGroup + C::SIDE * lane;
         id = group * p.teams_per_block + team.team;
     } else {
         team.warps = 1;
         team.team = 0;
         team.warp = 0;
         team.lane = lane & (LANES - 1);
-        c.col = MODE != kScalar ? 4 * team.lane : team.lane;
+        c.col = C::SIDE * team.lane;
         id = group * p.teams_per_block + threadIdx.x / LANES;
     }
     c.width = width;
-    team.group = (c.col - (MODE != kScalar ? 4 * team.lane : team.lane)) / kPackGroup;
+    team.group = (c.col - C::SIDE * team.lane) / kPackGroup;
     if (BIG && p.cluster > 1) cooperative_groups::this_cluster().sync();      // every block's scratch exists
     return id;
 }
 
+__device__ __forceinline__ uint32_t word_of(const Quad<uint8_t>& q) { return *reinterpret_cast<const uint32_t*>(q.v); }
+
 // Codes of a thread's elements and the scales of their groups.  A group is a warp's chunk, or with fewer lanes 32 / LANES
 // chunks of the same threads.  Each lane forms the scale and its reciprocal of one group only.
-template <typename B, int LANES, int V, int MODE>
-__device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], const Columns<LANES, V, MODE>& c, bool write,
-                                          uint8_t* codes, B* scales, int lane, int first) {
+template <typename B, typename C>
+__device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[C::V], const C& c, bool write, uint8_t* codes,
+                                          B* scales, int lane, int first) {
+    constexpr int LANES = C::LANES, V = C::V;
     constexpr int kTogether = 32 / LANES < V ? 32 / LANES : V, kGroups = V / kTogether;
     using Bits = typename AbsBits<B>::type;
     Bits mine = 0;
@@ -278,25 +277,27 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[V], con
 #pragma unroll
         for (int j = i * kTogether; j < (i + 1) * kTogether; ++j) {
             const uint32_t word = encode4(format, v[j], inv);
-            put(codes, c, j, *reinterpret_cast<const Quad<uint8_t>*>(&word));
+            put(codes, c, j, Quad<uint8_t>{{(uint8_t)word, (uint8_t)(word >> 8), (uint8_t)(word >> 16), (uint8_t)(word >> 24)}});
         }
     }
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, int MODE, bool BRANCH, bool BIG>
-__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG))
+__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG, sizeof(S) == 8))
     ring_forward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p) {
     using B = Br<S>;
     constexpr int T = ring_threads(BIG, sizeof(S) == 8);
-    using FS = Feed<S, LANES, V, MODE, T>;
-    using FB = Feed<B, LANES, V, MODE, T>;
-    constexpr int at_y = FS::kBytes, at_gate = at_y + FB::kBytes;
+    using C = Columns<LANES, V, MODE, MODE == kScalar ? 1 : 16 / (int)sizeof(B)>;
+    using FS = Feed<S, C, T>;
+    using FB = Feed<B, C, T>;
+    constexpr int at_y = ring_bytes((int)sizeof(S), MODE != kScalar, V, T),
+                  at_gate = at_y + ring_bytes((int)sizeof(B), MODE != kScalar, V, T);
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
-    Columns<LANES, V, MODE> c;
-    const uint32_t id = set_up<LANES, V, MODE, BIG, B>(p, (int)a.width, &scratch, team, c);
+    C c;
+    const uint32_t id = set_up<BIG, B>(p, (int)a.width, &scratch, team, c);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const bool row_gate = BRANCH && a.gate && !p.shared;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
@@ -305,23 +306,20 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
     const S* x = static_cast<const S*>(a.x) + c.col;
     const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col;
     // parameters in registers, or with many chunks behind a branch in memory
-    constexpr bool kHeld = !BRANCH || V == ring_chunks(false, sizeof(S) == 8);
-    constexpr int H = kHeld ? V : 1;
-    Four<B> held[5][H];
-    const auto parameter = [&](int which, const void* p, int j, B absent) {
-        return kHeld ? held[which][kHeld ? j : 0] : get_or(p, c, j, absent);
-    };
-    if (kHeld)
+    constexpr bool kHeld = !BRANCH || (sizeof(S) == 8 ? !BIG : V == 2);
+    Four<B> held[5][kHeld ? V : 1];
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            if (BRANCH) {
-                held[0][j] = get_or(a.scale, c, j, B(1));
-                held[1][j] = get_or(a.post_weight, c, j, B(1));
-                held[2][j] = get_or(a.post_bias, c, j, B(0));
-            }
-            held[3][j] = get_or(a.next_weight, c, j, B(1));
-            held[4][j] = get_or(a.next_bias, c, j, B(0));
-        }
+    for (int j = 0; j < (kHeld ? V : 1); ++j) {
+        held[0][j] = get_or(BRANCH ? a.scale : nullptr, c, j, B(1));
+        held[1][j] = get_or(BRANCH ? a.post_weight : nullptr, c, j, B(1));
+        held[2][j] = get_or(BRANCH ? a.post_bias : nullptr, c, j, B(0));
+        held[3][j] = get_or(a.next_weight, c, j, B(1));
+        held[4][j] = get_or(a.next_bias, c, j, B(0));
+    }
+    const auto parameter = [&](int which, const void* from, int j, B absent) {
+        if constexpr (kHeld) return held[which][j];
+        else return get_or(from, c, j, absent);
+    };
 
     const uint32_t first = p.shared ? id * p.rows_per_team : id, next = p.shared ? 1u : (uint32_t)p.teams,
                    last = p.shared ? min(first + p.rows_per_team, rows) : rows;
@@ -459,20 +457,21 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, int MODE, bool BRANCH, bool NEXT, bool BIG>
-__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG))
+__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG, sizeof(S) == 8))
     ring_backward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p,
                          const __grid_constant__ BackwardSlabs slabs) {
     using B = Br<S>;
     constexpr int T = ring_threads(BIG, sizeof(S) == 8);
-    using FS = Feed<S, LANES, V, MODE, T>;
-    using FB = Feed<B, LANES, V, MODE, T>;
-    using FQ = Feed<uint8_t, LANES, V, MODE, T>;
+    using C = Columns<LANES, V, MODE, MODE == kScalar ? 1 : 16 / (int)sizeof(B)>;
+    using FS = Feed<S, C, T>;
+    using FB = Feed<B, C, T>;
+    using FQ = Feed<uint8_t, C, T>;
     using At = BackwardStage<NEXT, BRANCH, V, T, MODE != kScalar, (int)sizeof(S), (int)sizeof(B)>;
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
     Team<B, LANES, BIG> team;
-    Columns<LANES, V, MODE> c;
-    const uint32_t id = set_up<LANES, V, MODE, BIG, B>(p, (int)a.width, &scratch, team, c);
+    C c;
+    const uint32_t id = set_up<BIG, B>(p, (int)a.width, &scratch, team, c);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const bool row_gate = BRANCH && (a.gate || a.gate_codes) && !p.shared;
@@ -482,16 +481,16 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
     const S *x = static_cast<const S*>(a.x) + c.col, *dout = static_cast<const S*>(a.dout) + c.col;
     const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col,
             *dh = static_cast<const B*>(a.dh) + c.col, *pb = static_cast<const B*>(a.post_bias) + c.col;
-    // parameters, chunk after chunk of the team's threads: teams of a block share them
+    // parameters: teams of a block share them
     const int per_team = blockDim.x / p.teams_per_block, in_team = threadIdx.x % per_team;
-    Four<B>* shelf = reinterpret_cast<Four<B>*>(ring + p.stages * p.stage_bytes);
-    Four<B> *const nw = shelf + in_team, *const pw = shelf + (NEXT ? V * per_team : 0) + in_team, *const scale = pw + V * per_team;
+    const int array = per_team * 4 * V * (int)sizeof(B);
+    char *const nw = ring + p.stages * p.stage_bytes + in_team * 16, *const pw = nw + (NEXT ? array : 0), *const scale = pw + array;
     if ((int)threadIdx.x < per_team)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (NEXT) nw[j * per_team] = get_or(a.next_weight, c, j, B(1));
-            if (BRANCH) pw[j * per_team] = get_or(a.post_weight, c, j, B(1));
-            if (BRANCH) scale[j * per_team] = get_or(a.scale, c, j, B(1));
+            if (NEXT) to_shelf(nw, per_team, j, get_or(a.next_weight, c, j, B(1)));
+            if (BRANCH) to_shelf(pw, per_team, j, get_or(a.post_weight, c, j, B(1)));
+            if (BRANCH) to_shelf(scale, per_team, j, get_or(a.scale, c, j, B(1)));
         }
     __syncthreads();
     Four<B> sum_scale[V], sum_pw[V], sum_pb[V], sum_nw[V], sum_nb[V], sum_gate[V];
@@ -511,7 +510,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                 copy_async<sizeof(B)>(at + 4 * V * T + (clique * V + team.lane) * (uint32_t)sizeof(B),
                                       static_cast<const B*>(scales) + (uint64_t)row * (uint32_t)groups + team.group + team.lane);
         } else {
-            Feed<E, LANES, V, MODE, T>::issue(at, row_at(values, row, stride), c);
+            Feed<E, C, T>::issue(at, row_at(values, row, stride), c);
         }
     };
     const auto take_kept = [&](const char* at, const void* codes, auto* values, int64_t stride, uint32_t row, int j) {
@@ -519,9 +518,9 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
         if (codes) {
             const Quad<uint8_t> q = FQ::take(at, static_cast<const uint8_t*>(codes) + (uint64_t)row * (uint32_t)D + (uint32_t)c.col, c, j);
             const B s = reinterpret_cast<const B*>(at + 4 * V * T)[clique * V + j / kTogether];
-            return decode4<B>(a.checkpoint, *reinterpret_cast<const uint32_t*>(&q), s);
+            return decode4<B>(a.checkpoint, word_of(q), s);
         }
-        return widen4<E>(Feed<E, LANES, V, MODE, T>::take(at, row_at(values, row, stride), c, j));
+        return widen4<E>(Feed<E, C, T>::take(at, row_at(values, row, stride), c, j));
     };
     const auto issue_stats = [&](uint32_t at, const void* stats, uint32_t row) {
         if (team.lane == 0)
@@ -583,7 +582,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                     v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);          // the normalised row
                     sum_nw[j] = fma4(d[j], v[j], sum_nw[j]);
                     sum_nb[j] = sum_nb[j] + d[j];
-                    d[j] = d[j] * from_shelf(nw + j * per_team);
+                    d[j] = d[j] * from_shelf<B>(nw, per_team, j);
                     s0 = s0 + d[j];
                     s1 = fma4(d[j], v[j], s1);
                 }
@@ -619,7 +618,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                 for (int j = 0; j < V; ++j) {
                     v[j] = take_kept(at + At::y, a.y_codes, y, a.y_stride, row, j);
                     if (a.post_norm != kNormNone) v[j] = centre<B>(c, j, v[j], mean) * four<B>(rstd);
-                    const Four<B> w = from_shelf(pw + j * per_team), sc = from_shelf(scale + j * per_team);
+                    const Four<B> w = from_shelf<B>(pw, per_team, j), sc = from_shelf<B>(scale, per_team, j);
                     Four<B> z = v[j] * w;
                     if (a.post_bias) z = z + get(pb, c, j);
                     if (p.shared || row_gate) {
@@ -675,7 +674,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
 
     // one slab row per block: the teams' sums, added in the order of the teams
     const uint32_t block = BIG && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
-    shelf = reinterpret_cast<Four<B>*>(ring);
+    Four<B>* shelf = reinterpret_cast<Four<B>*>(ring);
     const auto leave = [&](int which, Four<B> (&v)[V]) {
         if (!slabs.column[which]) return;
         B* row = static_cast<B*>(slabs.column[which]) + (uint64_t)block * (uint32_t)D + c.col;
@@ -686,7 +685,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                 shelf[threadIdx.x] = v[j];
                 __syncthreads();
                 if ((int)threadIdx.x >= per_team) continue;
-                for (int i = 1; i < p.teams_per_block; ++i) v[j] = v[j] + from_shelf(shelf + i * per_team + threadIdx.x);
+                for (int i = 1; i < p.teams_per_block; ++i) v[j] = v[j] + shelf[i * per_team + threadIdx.x];
             }
             put(row, c, j, v[j]);
         }
@@ -733,21 +732,22 @@ cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...)
 template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_forward_as(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
-    constexpr int few = ring_chunks(false, f64), many = ring_chunks(true, f64);
+    constexpr int few = ring_chunks(false, BIG, f64), many = ring_chunks(true, BIG, f64);
     if (!a.y) return ring_launch(p, st, ring_forward_kernel<S, LANES, many, MODE, false, BIG>, a, p);
     if constexpr (LANES == 32)
         if (BIG || p.many) return ring_launch(p, st, ring_forward_kernel<S, LANES, many, MODE, true, BIG>, a, p);
-    return ring_launch(p, st, ring_forward_kernel<S, LANES, few, MODE, true, false>, a, p);
+    if constexpr (BIG) return cudaErrorInvalidValue;         // not reached
+    else return ring_launch(p, st, ring_forward_kernel<S, LANES, few, MODE, true, false>, a, p);
 }
 template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_backward_as(const kanb200_block_args& a, const RingPlan& p, const BackwardSlabs& slabs, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
     if (!a.has_branch)
-        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, f64), MODE, false, true, BIG>,
+        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, BIG, f64), MODE, false, true, BIG>,
                            a, p, slabs);
-    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, f64), MODE, true, true, BIG>,
+    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, BIG, f64), MODE, true, true, BIG>,
                               a, p, slabs)
-                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, f64), MODE, true, false, BIG>,
+                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, BIG, f64), MODE, true, false, BIG>,
                               a, p, slabs);
 }
 
