@@ -367,20 +367,17 @@ Team team_for(const kanb200_block_args& a, bool backward) {
     Team t{};
     t.many = !branch;
     const auto cover = [&] {
-        t.chunks = ring_chunks(t.many, t.big, f64);
+        t.chunks = ring_chunks(t.many, f64);
         t.warps = (int)div_up(a.width, kPackGroup * t.chunks);
     };
     cover();
-    if (t.warps > 8 && !backward && !t.many) {
+    if (t.warps > 8 && !backward && !t.many && !f64) {
         t.many = true;
         cover();
     }
-    if (t.warps > 8) {
-        t.big = true;
-        cover();
-    }
+    t.big = t.warps > 8 && !f64;
     t.cluster = 1;
-    const int all = t.warps, most = ring_threads(t.big, f64) / 32;
+    const int all = t.warps, most = ring_threads(t.big) / 32;
     while (div_up(all, t.cluster) > most) t.cluster *= 2;
     t.warps = (int)div_up(all, t.cluster);
     return t;
@@ -404,14 +401,14 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.warps = team.warps;
     p.big = team.big;
     p.many = team.many;
-    p.teams_per_block = p.big ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
+    p.teams_per_block = p.big || p.cluster > 1 ? 1 : p.lanes == 32 ? 8 / p.warps : 256 / p.lanes;
     p.threads = p.lanes == 32 ? 32 * p.warps * p.teams_per_block : 256;
     const int T = p.threads;
     const bool vec = four_at_once(a);
     p.mode = !vec ? kScalar : p.lanes * 4 * V * (p.lanes == 32 ? p.warps * p.cluster : 1) == a.width ? kFull : kVector;
 
     // a stage of the ring: BackwardStage, or x, y and a gate per row
-    const int most = ring_threads(p.big, B == 8);
+    const int most = ring_threads(p.big);
     const bool row_gate = branch && (a.gate || a.gate_codes) && !(a.gate && a.gate_rows > 1);
     if (backward) {
         const auto take = [&](bool there, int bytes) { p.stage_bytes += there ? bytes : 0; };
@@ -429,7 +426,7 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.parameter_bytes = backward ? ((a.dh ? 1 : 0) + (branch ? 2 : 0)) * (p.threads / p.teams_per_block) * 4 * V * B : 0;
 
     // blocks to an SM by registers (the kernels' launch bounds) and shared memory, then up to four stages while there is room
-    const int registers = 65536 / (ring_threads(p.big, false) * ring_blocks(p.big, B == 8));
+    const int registers = 65536 / (ring_threads(p.big) * ring_blocks(p.big, B == 8));
     int per_sm = std::max(1, 65536 / (registers * T));
     const auto fits = [&](int stages) { return stages * p.stage_bytes + p.parameter_bytes <= 228 * 1024 / per_sm - 228 * 1024 + kSharedBytes; };
     while (per_sm > 1 && !fits(2)) --per_sm;

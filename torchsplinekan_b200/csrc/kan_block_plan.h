@@ -48,10 +48,11 @@ struct RingPlan : RowSplit {
 //   * The backward behind a branch holds the sums that are parameter gradients (20 V values): few chunks always (with many the
 //     8-bit gated backward of 16384 x 2048 spilled and took 278 us instead of 243).
 //   * A norm alone takes many.
-constexpr int ring_chunks(bool many, bool big, bool f64) { return f64 ? (big ? (many ? 2 : 1) : 2) : many ? 4 : 2; }
-// Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.  (Float64: 384,
-// the backward's ring and parameters have to fit an SM's shared memory.)
-constexpr int ring_threads(bool big, bool f64) { return !big ? 256 : f64 ? 384 : 512; }
+constexpr int ring_chunks(bool many, bool f64) { return many && !f64 ? 4 : 2; }
+// Threads of a block and blocks to an SM, which bound the registers: 512 threads to an SM may use 128 each.  (Float64: one
+// block of 256, whose threads may use 255; wide rows take a cluster of those, as a larger block's ring and parameters would
+// not fit an SM's shared memory.)
+constexpr int ring_threads(bool big) { return big ? 512 : 256; }
 constexpr int ring_blocks(bool big, bool f64) { return big || f64 ? 1 : 2; }
 
 // Bytes of one tensor in a stage of the ring: elements of less than 4 bytes that cannot be copied four at a time are not

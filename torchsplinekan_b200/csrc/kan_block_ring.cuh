@@ -169,7 +169,7 @@ struct TeamScratch {                       // per block, in shared memory
 
 static_assert(sizeof(TeamScratch) == 768, "kSharedBytes");
 
-template <typename B, int LANES, bool BIG> struct Team {
+template <typename B, int LANES, bool CLUSTERED> struct Team {
     TeamScratch* scratch;
     int warps, team, warp, lane;           // warps of this block in a row's team; team and warp within the team
     int group;                             // of 128 columns, the warp's first
@@ -181,7 +181,7 @@ template <typename B, int LANES, bool BIG> struct Team {
         for (int o = LANES / 2; o > 0; o >>= 1)
 #pragma unroll
             for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-        if (LANES < 32 || (warps == 1 && (!BIG || cluster == 1))) return;
+        if (LANES < 32 || (warps == 1 && (!CLUSTERED || cluster == 1))) return;
         // alternating buffers: a warp can only be one sum ahead of the others, so one barrier per sum is enough
         phase ^= 1;
         B* mine = reinterpret_cast<B*>(scratch->warp[phase]) + team * warps * K;
@@ -194,7 +194,7 @@ template <typename B, int LANES, bool BIG> struct Team {
         for (int w = 1; w < warps; ++w)
 #pragma unroll
             for (int k = 0; k < K; ++k) v[k] += mine[w * K + k];
-        if (BIG && cluster > 1) {
+        if (CLUSTERED && cluster > 1) {
             namespace cg = cooperative_groups;
             cg::cluster_group all = cg::this_cluster();
             if (warp == 0 && lane < cluster) {
@@ -219,14 +219,15 @@ template <typename T> __device__ __forceinline__ T* row_at(T* base, uint32_t row
 }
 
 // The team's place: its first column, and its first row.
-template <bool BIG, typename B, typename C>
-__device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, C::LANES, BIG>& team, C& c) {
+template <typename B, typename C, bool CLUSTERED>
+__device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScratch* scratch, Team<B, C::LANES, CLUSTERED>& team,
+                                           C& c) {
     constexpr int LANES = C::LANES, V = C::V;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     team.scratch = scratch;
-    team.cluster = BIG ? p.cluster : 1;
-    team.rank = BIG && p.cluster > 1 ? (int)(blockIdx.x % p.cluster) : 0;
-    const uint32_t group = BIG && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
+    team.cluster = CLUSTERED ? p.cluster : 1;
+    team.rank = CLUSTERED && p.cluster > 1 ? (int)(blockIdx.x % p.cluster) : 0;
+    const uint32_t group = CLUSTERED && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
     uint32_t id;
     if (LANES == 32) {
         team.warps = p.warps;
@@ -245,7 +246,7 @@ __device__ __forceinline__ uint32_t set_up(const RingPlan& p, int width, TeamScr
     }
     c.width = width;
     team.group = (c.col - C::SIDE * team.lane) / kPackGroup;
-    if (BIG && p.cluster > 1) cooperative_groups::this_cluster().sync();      // every block's scratch exists
+    if (CLUSTERED && p.cluster > 1) cooperative_groups::this_cluster().sync();      // every block's scratch exists
     return id;
 }
 
@@ -284,10 +285,10 @@ __device__ __forceinline__ void put_codes(int format, const Four<B> (&v)[C::V], 
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, int MODE, bool BRANCH, bool BIG>
-__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG, sizeof(S) == 8))
+__global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(BIG, sizeof(S) == 8))
     ring_forward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p) {
     using B = Br<S>;
-    constexpr int T = ring_threads(BIG, sizeof(S) == 8);
+    constexpr int T = ring_threads(BIG);
     using C = Columns<LANES, V, MODE, MODE == kScalar ? 1 : 16 / (int)sizeof(B)>;
     using FS = Feed<S, C, T>;
     using FB = Feed<B, C, T>;
@@ -295,9 +296,10 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
                   at_gate = at_y + ring_bytes((int)sizeof(B), MODE != kScalar, V, T);
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
-    Team<B, LANES, BIG> team;
+    constexpr bool CLUSTERED = LANES == 32 && (BIG || sizeof(S) == 8);
+    Team<B, LANES, CLUSTERED> team;
     C c;
-    const uint32_t id = set_up<BIG, B>(p, (int)a.width, &scratch, team, c);
+    const uint32_t id = set_up(p, (int)a.width, &scratch, team, c);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const bool row_gate = BRANCH && a.gate && !p.shared;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
     const S* x = static_cast<const S*>(a.x) + c.col;
     const B *y = static_cast<const B*>(a.y) + c.col, *gate = static_cast<const B*>(a.gate) + c.col;
     // parameters in registers, or with many chunks behind a branch in memory
-    constexpr bool kHeld = !BRANCH || (sizeof(S) == 8 ? !BIG : V == 2);
+    constexpr bool kHeld = !BRANCH || V == 2;
     Four<B> held[5][kHeld ? V : 1];
 #pragma unroll
     for (int j = 0; j < (kHeld ? V : 1); ++j) {
@@ -457,11 +459,11 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 template <typename S, int LANES, int V, int MODE, bool BRANCH, bool NEXT, bool BIG>
-__global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks(BIG, sizeof(S) == 8))
+__global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(BIG, sizeof(S) == 8))
     ring_backward_kernel(const __grid_constant__ kanb200_block_args a, const __grid_constant__ RingPlan p,
                          const __grid_constant__ BackwardSlabs slabs) {
     using B = Br<S>;
-    constexpr int T = ring_threads(BIG, sizeof(S) == 8);
+    constexpr int T = ring_threads(BIG);
     using C = Columns<LANES, V, MODE, MODE == kScalar ? 1 : 16 / (int)sizeof(B)>;
     using FS = Feed<S, C, T>;
     using FB = Feed<B, C, T>;
@@ -469,9 +471,10 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
     using At = BackwardStage<NEXT, BRANCH, V, T, MODE != kScalar, (int)sizeof(S), (int)sizeof(B)>;
     extern __shared__ __align__(16) char ring[];
     __shared__ TeamScratch scratch;
-    Team<B, LANES, BIG> team;
+    constexpr bool CLUSTERED = LANES == 32 && (BIG || sizeof(S) == 8);
+    Team<B, LANES, CLUSTERED> team;
     C c;
-    const uint32_t id = set_up<BIG, B>(p, (int)a.width, &scratch, team, c);
+    const uint32_t id = set_up(p, (int)a.width, &scratch, team, c);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), rows = (uint32_t)a.rows;
     const int D = (int)a.width, groups = (D + kPackGroup - 1) / kPackGroup;
     const bool row_gate = BRANCH && (a.gate || a.gate_codes) && !p.shared;
@@ -673,7 +676,7 @@ __global__ void __launch_bounds__(ring_threads(BIG, sizeof(S) == 8), ring_blocks
     copies_wait<0>();
 
     // one slab row per block: the teams' sums, added in the order of the teams
-    const uint32_t block = BIG && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
+    const uint32_t block = CLUSTERED && p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
     Four<B>* shelf = reinterpret_cast<Four<B>*>(ring);
     const auto leave = [&](int which, Four<B> (&v)[V]) {
         if (!slabs.column[which]) return;
@@ -732,7 +735,7 @@ cudaError_t ring_launch(const RingPlan& p, cudaStream_t st, void (*kernel)(P...)
 template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_forward_as(const kanb200_block_args& a, const RingPlan& p, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
-    constexpr int few = ring_chunks(false, BIG, f64), many = ring_chunks(true, BIG, f64);
+    constexpr int few = ring_chunks(false, f64), many = ring_chunks(true, f64);
     if (!a.y) return ring_launch(p, st, ring_forward_kernel<S, LANES, many, MODE, false, BIG>, a, p);
     if constexpr (LANES == 32)
         if (BIG || p.many) return ring_launch(p, st, ring_forward_kernel<S, LANES, many, MODE, true, BIG>, a, p);
@@ -743,11 +746,11 @@ template <typename S, int LANES, int MODE, bool BIG>
 cudaError_t ring_backward_as(const kanb200_block_args& a, const RingPlan& p, const BackwardSlabs& slabs, cudaStream_t st) {
     constexpr bool f64 = sizeof(S) == 8;
     if (!a.has_branch)
-        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, BIG, f64), MODE, false, true, BIG>,
+        return ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(true, f64), MODE, false, true, BIG>,
                            a, p, slabs);
-    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, BIG, f64), MODE, true, true, BIG>,
+    return a.dh ? ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, f64), MODE, true, true, BIG>,
                               a, p, slabs)
-                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, BIG, f64), MODE, true, false, BIG>,
+                : ring_launch(p, st, ring_backward_kernel<S, LANES, ring_chunks(false, f64), MODE, true, false, BIG>,
                               a, p, slabs);
 }
 
@@ -759,7 +762,9 @@ cudaError_t ring_backward_as(const kanb200_block_args& a, const RingPlan& p, con
         default: return name<S, lanes, kScalar, big>(__VA_ARGS__);                            \
     }
 #define KANB200_RING_DISPATCH(name, ...)                                                      \
-    if (p.big) KANB200_RING_MODE(name, 32, true, __VA_ARGS__)                                 \
+    if constexpr (sizeof(S) < 8) {                                                            \
+        if (p.big) KANB200_RING_MODE(name, 32, true, __VA_ARGS__)                             \
+    }                                                                                         \
     switch (p.lanes) {                                                                        \
         case 32: KANB200_RING_MODE(name, 32, false, __VA_ARGS__)                              \
         case 16: KANB200_RING_MODE(name, 16, false, __VA_ARGS__)                              \
