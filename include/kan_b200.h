@@ -356,7 +356,8 @@ KANB200_API int kanb200_allreduce_sum_f32_ranges(const void* const* peer_bases, 
  *   of the forward.  NULL output = not needed.  dgate [rows / gate_rows, width] is summed over the rows that share a
  *   gate row.  The sums over rows go through slabs in the workspace that a second kernel adds in a fixed order: no
  *   atomics, the same bits on every run.
- * Row strides are in elements; a row's columns are contiguous.  out, h, dx, codes and scales are dense. */
+ * Row strides are in elements; a row's columns are contiguous.  out, h, dx, codes and scales are dense; the statistics
+ * are aligned to two of their elements. */
 #define KANB200_F16  2   /* stream types of these operators only */
 #define KANB200_BF16 3
 

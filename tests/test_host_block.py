@@ -116,6 +116,7 @@ def test_c_abi_refuses_before_any_launch():
     refused("per row", y=p, out=p, gate=p, gate_rows=2, gate_codes=p, gate_scales=p, checkpoint=1)
     refused("together", x_codes=p, checkpoint=1)
     refused("format", x_codes=p, x_scales=p)
+    refused("aligned", next_stats=p + 4)
     refused("dout or dh", backward=True)
     refused("statistics", backward=True, dh=p)
     refused("need dh", backward=True, dout=p, has_branch=1, y=p, dnext_weight=p)

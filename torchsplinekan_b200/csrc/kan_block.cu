@@ -433,7 +433,10 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     p.stages = 2;
     if (backward || !branch || !p.many)                  // (parameters in memory need L1)
         while (p.stages < 4 && fits(p.stages + 1)) ++p.stages;
-    static_cast<RowSplit&>(p) = split_rows(a, (int64_t)kSms * per_sm / p.cluster * p.teams_per_block);
+    // A handful of rows: one block leaves the parameters' gradients in place, which saves the launch that adds slabs (6 rows per
+    // team take about 8 us, as long as that launch and the two kernels' starts).
+    const bool one_block = backward && a.rows <= (int64_t)6 * p.teams_per_block;
+    static_cast<RowSplit&>(p) = split_rows(a, one_block ? p.teams_per_block : (int64_t)kSms * per_sm / p.cluster * p.teams_per_block);
     p.blocks = (int)div_up(p.teams, p.teams_per_block) * p.cluster;
     if (!p.shared) {                     // rows in turn: over every team that is launched
         p.teams = (int64_t)p.blocks / p.cluster * p.teams_per_block;

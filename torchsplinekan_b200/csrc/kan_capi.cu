@@ -118,6 +118,9 @@ int check_block(const kanb200_block_args* a, bool backward) {
         return fail(KANB200_EINVAL, "%s: codes and scales come together", what);
     if (a->checkpoint == KANB200_PACK_NONE && (a->x_codes || a->y_codes || a->gate_codes))
         return fail(KANB200_EINVAL, "%s: codes need a checkpoint format", what);
+    const uintptr_t pair = a->dtype == KANB200_F64 ? 16 : 8;       // a row's two statistics are read at once
+    if (reinterpret_cast<uintptr_t>(a->post_stats) % pair || reinterpret_cast<uintptr_t>(a->next_stats) % pair)
+        return fail(KANB200_EINVAL, "%s: the statistics must be aligned to two of their elements", what);
     if (a->rows == 0) return KANB200_OK;
     if (!backward) {
         if (!a->x) return fail(KANB200_EINVAL, "%s: x must not be NULL", what);
