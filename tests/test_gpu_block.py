@@ -203,7 +203,8 @@ def test_gated_options(gate, post, next, form):
 
 @pytest.mark.parametrize("lead,width,gate", [((1, 1), 64, "sequence"), ((1, 2000), 40, "sequence"), ((7, 311), 96, "sequence"),
                                              ((1500, 2), 33, "sequence"), ((2, 3, 70), 260, "sequence"), ((2500,), 24, "all"),
-                                             ((2, 900), 1030, "all"), ((3, 1), 48, "sequence"), ((400, 5), 1, "sequence")])
+                                             ((2, 900), 1030, "all"), ((3, 1), 48, "sequence"), ((400, 5), 1, "sequence"),
+                                             ((2, 3), 33001, "sequence"), ((2, 45), 9000, "sequence"), ((3, 200), 2052, "all")])
 def test_shared_gate_gradients(lead, width, gate):
     for act in (None, "silu"):
         check_gated(make_gated(lead, width, torch.float32, gate, act, form="int8"))
@@ -335,6 +336,22 @@ def test_rows_of_zeros_and_constants():
     for kind in ("rms", "layer"):
         check_norm(torch.zeros(4, 130, device="cuda"), randn(130, dtype=torch.float32), None, kind, "int8",
                    randn(4, 130, dtype=torch.float32, seed=5))
+
+
+def test_squares_that_overflow():
+    """r = 0 for a row whose squares overflow: finite elements become 0, forward and backward."""
+    for width in (24, 500, 40000):
+        x = torch.full((3, width), 1e30, device="cuda")
+        x[1] = randn(width, dtype=torch.float32)
+        x[2, ::2] = -1e30
+        for kind in ("rms", "layer"):
+            t = x.clone().requires_grad_()
+            h = sk.block_norm(t, kind=kind)
+            (dx,) = torch.autograd.grad(h, t, torch.ones_like(h))
+            assert bool((h[2] == 0).all()) and bool((dx[2] == 0).all()) and bool(torch.isfinite(h).all()) and bool(torch.isfinite(dx).all())
+            if kind == "rms":
+                assert bool((h[0] == 0).all())
+            assert float(h[1].abs().max()) > 0.5
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])

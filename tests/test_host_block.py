@@ -48,6 +48,7 @@ def test_refusals():
             (lambda: sk.block_norm(x.half(), w.half()), "weight must be"),
             (lambda: sk.block_norm(x, eps=0.0), "eps"),
             (lambda: sk.block_norm(x, eps=float("nan")), "eps"),
+            (lambda: sk.block_norm(x, eps=1e-45), "eps"),
             (lambda: sk.block_norm(x, checkpoint="int8"), "CUDA"),
             (lambda: sk.gated_residual(x, y[:, :2]), "y must have shape"),
             (lambda: sk.gated_residual(x, y.double()), "y must be"),
@@ -102,6 +103,7 @@ def test_c_abi_refuses_before_any_launch():
     refused("sizes", rows=-1)
     refused("too large", rows=1 << 60)
     refused("eps", eps=0.0)
+    refused("eps", eps=1e-40)
     refused("norm", next_norm=5)
     refused("activation", gate_act=7)
     refused("checkpoint", checkpoint=3)
@@ -156,6 +158,11 @@ def test_networks_of_blocks_on_the_dense_backend():
     assert torch.allclose(y, net(x)) and torch.allclose(reg, net.regularization_loss(x=x))
     plain = sk.KAN([6, 8, 2])
     assert sorted(k for k, _ in plain.named_parameters()) == sorted(k for k, _ in sk.KAN.from_layers(list(plain.layers)).named_parameters())
+    state = plain.__getstate__()
+    state.pop("norms"), state.pop("connections")
+    old = sk.KAN.__new__(sk.KAN)
+    old.__setstate__(state)                                   # pickled before the blocks existed
+    assert torch.equal(old(x.detach().float()), plain(x.detach().float()))
     for bad, words in ((dict(norm="batch"), "norm"), (dict(gate="silu"), "residual"), (dict(gate="relu", residual=True), "gate"),
                        (dict(residual=True), "equal widths"), (dict(activation_checkpoint="int4"), "activation_checkpoint")):
         with pytest.raises(ValueError, match=words):

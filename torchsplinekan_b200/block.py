@@ -39,7 +39,7 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """``(x - m) r * weight + bias`` over the last dimension, in the branch's type: the norm in front of a layer.
 
     ``kind``: "rms" (``m = 0``, ``r = (mean(x^2) + eps)^-1/2``) or "layer" (``m = mean(x)``,
-    ``r = (mean((x - m)^2) + eps)^-1/2``).
+    ``r = (mean((x - m)^2) + eps)^-1/2``).  Rows whose squares overflow the branch's type have ``r = 0``.
 
     ``checkpoint``: None keeps ``x`` for the backward; "int8" / "e4m3" keep 8-bit codes of it instead (see
     :func:`pack_activation`), written by the same kernel.  The result is the same; the gradients are those of the

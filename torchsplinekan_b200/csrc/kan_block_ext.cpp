@@ -62,8 +62,10 @@ void check_vector(const Tensor& t, const char* what, const char* name, int64_t w
     TORCH_CHECK(t.device() == x.device(), what, ": ", name, " must be on x's device");
 }
 
-void check_settings(const char* what, double eps, int64_t checkpoint) {
-    TORCH_CHECK(eps > 0.0 && std::isfinite(eps), what, ": eps must be positive, got ", eps);
+void check_settings(const char* what, const Tensor& x, double eps, int64_t checkpoint) {
+    const double least = branch_type(x) == at::kDouble ? 2.2250738585072014e-308 : 1.17549435e-38;
+    TORCH_CHECK(eps >= least && std::isfinite(eps), what, ": eps must be a positive normal number of the branch's type, got ",
+                eps);
     TORCH_CHECK(checkpoint >= KANB200_PACK_NONE && checkpoint <= KANB200_PACK_E4M3, what, ": unknown checkpoint format");
 }
 
@@ -131,7 +133,7 @@ void check_norm(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind,
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must have at least one column, got ", x.sizes());
     stream_code(x, what);
     TORCH_CHECK(kind == KANB200_NORM_RMS || kind == KANB200_NORM_LAYER, what, ": unknown norm");
-    check_settings(what, eps, checkpoint);
+    check_settings(what, x, eps, checkpoint);
     check_vector(w, what, "weight", x.size(-1), branch_type(x), x);
     check_vector(b, what, "bias", x.size(-1), branch_type(x), x);
 }
@@ -198,6 +200,7 @@ struct SavedNode : public torch::autograd::Node {
     }
     bool need(size_t i) const { return i < num_outputs() && task_should_compute_output(i); }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         released = true;
         for (SavedVariable& v : saved) v.reset_data();
     }
@@ -305,7 +308,7 @@ void check_gated(Gated& g) {
     const Tensor &x = g.x, &y = g.y;
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must have at least one column, got ", x.sizes());
     stream_code(x, what);
-    check_settings(what, g.eps, g.checkpoint);
+    check_settings(what, x, g.eps, g.checkpoint);
     TORCH_CHECK(g.act >= KANB200_ACT_NONE && g.act <= KANB200_ACT_SILU, what, ": unknown gate activation");
     for (int64_t n : {g.post, g.next})
         TORCH_CHECK(n >= KANB200_NORM_NONE && n <= KANB200_NORM_LAYER, what, ": unknown norm");

@@ -156,10 +156,11 @@ __device__ __forceinline__ void clear_ring(char* ring, int bytes) {
     __syncthreads();
 }
 
-// 1 / sqrt: the float approximation (2 ulp) and a Newton step, instead of a correctly rounded root and division
+// 1 / sqrt: the float approximation (2 ulp) and a Newton step, instead of a correctly rounded root and division.  0 for
+// infinity (squares that overflow), where the step would give NaN.
 __device__ __forceinline__ float rsqrt_newton(float v) {
     const float r = rsqrtf(v);
-    return r * fmaf(-0.5f * v * r, r, 1.5f);
+    return r == 0.0f ? 0.0f : r * fmaf(-0.5f * v * r, r, 1.5f);
 }
 __device__ __forceinline__ double rsqrt_newton(double v) { return 1.0 / sqrt(v); }
 

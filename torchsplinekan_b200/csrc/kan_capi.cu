@@ -103,7 +103,8 @@ int check_block(const kanb200_block_args* a, bool backward) {
         return fail(KANB200_EINVAL, "%s: unknown gate activation %d", what, a->gate_act);
     if (a->checkpoint < KANB200_PACK_NONE || a->checkpoint > KANB200_PACK_E4M3)
         return fail(KANB200_EINVAL, "%s: unknown checkpoint format %d", what, a->checkpoint);
-    if (!(a->eps > 0.0) || !std::isfinite(a->eps)) return fail(KANB200_EINVAL, "%s: eps must be positive", what);
+    if (!(a->eps >= (a->dtype == KANB200_F64 ? 2.2250738585072014e-308 : 1.17549435e-38)) || !std::isfinite(a->eps))
+        return fail(KANB200_EINVAL, "%s: eps must be a positive normal number of the branch's type", what);
     if (a->x_stride < 0 || a->y_stride < 0 || a->gate_stride < 0 || a->dout_stride < 0 || a->dh_stride < 0)
         return fail(KANB200_EINVAL, "%s: row strides must not be negative", what);
     if ((a->post_norm == KANB200_NORM_NONE && (a->post_weight || a->post_bias)) ||

@@ -57,6 +57,12 @@ class KAN(nn.Module):
             str(i): GatedResidual(a, gate, norm, scale_init, checkpoint=activation_checkpoint)
             for i, (a, b) in enumerate(pairs) if a == b}) if residual else None
 
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        for part in ("norms", "connections"):                # of networks pickled before the blocks existed
+            if part not in self.__dict__ and part not in self._modules:
+                setattr(self, part, None)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self._walk(x, lambda layer, h: layer(h))
 

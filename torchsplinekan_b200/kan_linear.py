@@ -54,6 +54,8 @@ class KANLinear(nn.Module):
     it), so it does not either.
     """
 
+    activation_checkpoint: Optional[str] = None      # also of layers pickled before the option existed
+
     def __init__(self, in_features: int, out_features: int, grid_size: int = 5, spline_order: int = 3,
                  scale_noise: float = 0.1, scale_base: float = 1.0, scale_spline: float = 1.0,
                  enable_standalone_scale_spline: bool = True, base_activation=nn.SiLU, grid_eps: float = 0.02,
