@@ -28,6 +28,8 @@ PACK_GROUP = int(_C.PACK_GROUP)
 
 
 def _code(table: dict, name: str, value) -> int:
+    if value is None:
+        return 0
     try:
         return table[value]
     except (KeyError, TypeError):
@@ -44,11 +46,9 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``checkpoint``: None keeps ``x`` for the backward; "int8" / "e4m3" keep 8-bit codes of it instead (see
     :func:`pack_activation`), written by the same kernel.  The result is the same; the gradients are those of the
     formulas with the restored ``x`` next to the exact ``m`` and ``r``."""
-    kind_code = _code(NORMS, "kind", kind)
-    if kind_code == 0:
+    if kind is None:
         raise ValueError("kind must be 'rms' or 'layer', got None")
-    return _C.block_norm(x, weight, bias, kind_code, eps, 0 if checkpoint is None else
-                         _code(CHECKPOINTS, "checkpoint", checkpoint))
+    return _C.block_norm(x, weight, bias, _code(NORMS, "kind", kind), eps, _code(CHECKPOINTS, "checkpoint", checkpoint))
 
 
 def gated_residual(x: torch.Tensor, y: torch.Tensor, *, gate: Union[torch.Tensor, str, None] = None,
@@ -86,10 +86,9 @@ def pack_activation(x: torch.Tensor, format: str = "int8") -> Tuple[torch.Tensor
     ``codes = round(x / scale)``, int8 or float8_e4m3fn.  "int8" has the smaller error on inputs of about one size
     (at most ``A / 254``), "e4m3" keeps relative precision (``2^-4``) over a wide range.  A group that holds a NaN or an
     infinity comes back as NaN, so an overflow stays visible.  CUDA tensors only; no gradient flows through it."""
-    code = _code(CHECKPOINTS, "format", format)
-    if code == 0:
+    if format is None:
         raise ValueError("format must be 'int8' or 'e4m3', got None")
-    return _C.pack_activation(x, code)
+    return _C.pack_activation(x, _code(CHECKPOINTS, "format", format))
 
 
 def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -102,8 +101,9 @@ class BlockNorm(nn.Module):
 
     def __init__(self, width: int, kind: str = "rms", eps: float = 1e-6, checkpoint: Optional[str] = None) -> None:
         super().__init__()
-        if _code(NORMS, "kind", kind) == 0:
+        if kind is None:
             raise ValueError("kind must be 'rms' or 'layer', got None")
+        _code(NORMS, "kind", kind)
         _code(CHECKPOINTS, "checkpoint", checkpoint)
         self.kind, self.eps, self.checkpoint = kind, eps, checkpoint
         self.weight = nn.Parameter(torch.ones(width))
