@@ -432,9 +432,14 @@ RingPlan plan_ring(const kanb200_block_args& a, bool backward) {
     int per_sm = std::max(1, 65536 / (registers * T));
     const auto fits = [&](int stages) { return stages * p.stage_bytes + p.parameter_bytes <= 228 * 1024 / per_sm - 228 * 1024 + kSharedBytes; };
     while (per_sm > 1 && !fits(2)) --per_sm;
+    // Stages: two, more only where two leave less than 40 KB (a norm alone: 32) on their way to an SM.  Deeper rings are slower
+    // (forward / backward in us, two against four stages: 16384 x 1024 connection 54 / 94 against 61 / 99, 8192 x 2048 53 / 88
+    // against 60 / 94), too little as well (10922 x 1536, 36 KB: forward 56 with two, 52 with three).  Parameters read from
+    // memory need the rest for L1.
+    const int enough = (branch ? 40 : 32) * 1024, moving = (int)((int64_t)p.stage_bytes * T / most) * per_sm;
     p.stages = 2;
-    if (backward || !branch || !p.many)                  // (parameters in memory need L1)
-        while (p.stages < 4 && fits(p.stages + 1)) ++p.stages;
+    if (backward || !branch || !p.many)
+        while (p.stages < 4 && (p.stages - 1) * moving < enough && fits(p.stages + 1)) ++p.stages;
     // A handful of rows: one block leaves the parameters' gradients in place, which saves the launch that adds slabs (6 rows per
     // team take about 8 us, as long as that launch and the two kernels' starts).
     const bool one_block = backward && a.rows <= (int64_t)6 * p.teams_per_block;

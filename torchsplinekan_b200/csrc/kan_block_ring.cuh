@@ -193,11 +193,15 @@ template <typename B, int LANES, bool CLUSTERED> struct Team {
 #pragma unroll
             for (int k = 0; k < K; ++k) mine[warp * K + k] = v[k];
         asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(warps * 32) : "memory");
+        // a lane takes one warp's sums (the low bits of its number say whose), and the lanes add them up in pairs
+        const int low = warps > 8 ? 15 : warps > 4 ? 7 : warps > 2 ? 3 : 1, whose = lane & low;
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = mine[k];
-        for (int w = 1; w < warps; ++w)
+        for (int k = 0; k < K; ++k) v[k] = whose < warps ? mine[whose * K + k] : B(0);
 #pragma unroll
-            for (int k = 0; k < K; ++k) v[k] += mine[w * K + k];
+        for (int o = 8; o > 0; o >>= 1)
+            if (o <= low)
+#pragma unroll
+                for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
         if (CLUSTERED && cluster > 1) {
             namespace cg = cooperative_groups;
             cg::cluster_group all = cg::this_cluster();
@@ -500,9 +504,11 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(BIG, sizeof(S) 
             if (BRANCH) to_shelf(scale, per_team, j, get_or(a.scale, c, j, B(1)));
         }
     __syncthreads();
-    Four<B> sum_scale[V], sum_pw[V], sum_pb[V], sum_nw[V], sum_nb[V], sum_gate[V];
+    // sums over rows: of g a yhat and of g a behind a branch (its three parameters' gradients are multiples of those, see the
+    // end), of dh xhat and dh at a norm, of dgate
+    Four<B> sum_gay[V], sum_ga[V], sum_nw[V], sum_nb[V], sum_gate[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum_scale[j] = sum_pw[j] = sum_pb[j] = sum_nw[j] = sum_nb[j] = sum_gate[j] = zero;
+    for (int j = 0; j < V; ++j) sum_gay[j] = sum_ga[j] = sum_nw[j] = sum_nb[j] = sum_gate[j] = zero;
 
     // What a warp's lanes read in common (statistics, scales) one lane copies: a copy of one address by 32 lanes to 32 places
     // takes 32 passes of the shared memory.  The lanes meet in a __syncwarp before they read it.
@@ -633,19 +639,14 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(BIG, sizeof(S) 
                         const Four<B> gv = p.shared ? get(row_at(gate, span, a.gate_stride), c, j)
                                                     : take_kept(at + At::gate, a.gate_codes, gate, a.gate_stride, row, j);
                         gate4_grad<B>(a.gate_act, gv, act, dact);
-                        const Four<B> gz = g[j] * z;
-                        sum_scale[j] = fma4(gz, act, sum_scale[j]);
-                        const Four<B> dg = gz * (dact * sc);
+                        const Four<B> dg = g[j] * z * (dact * sc);
                         if (p.shared) sum_gate[j] = sum_gate[j] + dg;
                         else if (a.dgate) put(row_at(static_cast<B*>(a.dgate) + c.col, row, a.dgate_stride), c, j, dg);
-                        g[j] = g[j] * (act * sc);
-                    } else {
-                        sum_scale[j] = fma4(g[j], z, sum_scale[j]);
-                        g[j] = g[j] * sc;
+                        g[j] = g[j] * act;
                     }
-                    sum_pw[j] = fma4(g[j], v[j], sum_pw[j]);
-                    sum_pb[j] = sum_pb[j] + g[j];
-                    g[j] = g[j] * w;
+                    sum_gay[j] = fma4(g[j], v[j], sum_gay[j]);
+                    sum_ga[j] = sum_ga[j] + g[j];
+                    g[j] = g[j] * (sc * w);
                     s0 = s0 + g[j];
                     s1 = fma4(g[j], v[j], s1);
                 }
@@ -698,9 +699,18 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(BIG, sizeof(S) 
         }
     };
     if (BRANCH) {
-        leave(kSumScale, sum_scale);
-        leave(kSumPostWeight, sum_pw);
-        leave(kSumPostBias, sum_pb);
+        // z = yhat w + b:  dscale = sum g a z = w sum g a yhat + b sum g a,  dw = scale sum g a yhat,  db = scale sum g a
+        Four<B> share[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            share[j] = fma4(sum_gay[j], get_or(a.post_weight, c, j, B(1)), sum_ga[j] * get_or(a.post_bias, c, j, B(0)));
+        leave(kSumScale, share);
+#pragma unroll
+        for (int j = 0; j < V; ++j) share[j] = sum_gay[j] * get_or(a.scale, c, j, B(1));
+        leave(kSumPostWeight, share);
+#pragma unroll
+        for (int j = 0; j < V; ++j) share[j] = sum_ga[j] * get_or(a.scale, c, j, B(1));
+        leave(kSumPostBias, share);
     }
     if (NEXT) {
         leave(kSumNextWeight, sum_nw);
