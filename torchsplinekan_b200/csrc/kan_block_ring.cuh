@@ -47,9 +47,11 @@ __device__ __forceinline__ void copies_wait_oldest(int stages) {
 
 // Which columns a thread owns.  A warp covers V chunks of 4 LANES columns, one after the other.  A thread has four of each:
 // runs of SIDE columns, 16 bytes of the branch's type (kFull, kVector: rows, strides and pointers allow four elements at
-// once; float64: two runs, so that the lanes' accesses stay side by side) or single ones (kScalar).  kFull: the team's
-// columns are exactly the row's, so nothing is masked (a third of the instructions of the gated backward were predicates,
-// selects and zeros).  Distances between a thread's elements are constants, so a row costs one address per tensor.
+// once; float64: two runs, so that the lanes' accesses stay side by side) or single ones (kScalar: connection of
+// 16384 x 1024 that way forward 70 us instead of 54, backward 130 instead of 93).  kFull: the team's columns are exactly the
+// row's, so nothing is masked (against kVector: forward of 4096 x 4096 60 us instead of 77, 8-bit half-precision pass of
+// 16384 x 2048 211 instead of 222; no difference at 16384 x 1024).  Distances between a thread's elements are constants, so a
+// row costs one address per tensor.
 template <int LANES_, int V_, int MODE_, int SIDE_> struct Columns {
     static constexpr int LANES = LANES_, V = V_, MODE = MODE_, SIDE = SIDE_;
     int col, width;
