@@ -7,6 +7,7 @@
 // composite formulas serve CPU tensors and backward passes that are themselves recorded (create_graph=True).
 #include <ATen/TensorUtils.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -75,16 +76,55 @@ int64_t row_count(const Tensor& x) {
     return n;
 }
 
-Packed new_codes(int64_t rows, int64_t width, int format, const Tensor& like, at::ScalarType scale_type) {
-    const int64_t groups = (width + KANB200_PACK_GROUP - 1) / KANB200_PACK_GROUP;
-    return {at::empty({rows, width}, like.options().dtype(format == KANB200_PACK_INT8 ? at::kChar : at::kFloat8_e4m3fn)),
-            at::empty({rows, groups}, like.options().dtype(scale_type))};
+// New memory from the caching allocator, past the dispatcher (a third of the time of at::empty; a training call of a few
+// rows makes about ten).
+Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
 }
+
+int64_t group_count(int64_t width) { return (width + KANB200_PACK_GROUP - 1) / KANB200_PACK_GROUP; }
+
+// What the forward leaves for the backward besides its inputs, in one piece of memory: the norms' statistics, and the codes and
+// scales of y, of a gate per row and of the last norm's input.
+struct Record {
+    bool post = false, next = false, y = false, gate = false, x = false;
+
+    // its size; with `base`, the places of its parts
+    int64_t lay(kanb200_block_args& a, char* base) const {
+        const int64_t value = a.dtype == KANB200_F64 ? 8 : 4;
+        int64_t at = 0;
+        const auto take = [&](bool there, int64_t bytes, void*& to) {
+            if (!there) return;
+            if (base) to = base + at;
+            at += (bytes + 255) / 256 * 256;
+        };
+        take(post, 2 * a.rows * value, a.post_stats);
+        take(next, 2 * a.rows * value, a.next_stats);
+        const auto codes = [&](bool there, void*& c, void*& s) {
+            take(there, a.rows * a.width, c);
+            take(there, a.rows * group_count(a.width) * value, s);
+        };
+        codes(y, a.y_codes, a.y_scales);
+        codes(gate, a.gate_codes, a.gate_scales);
+        codes(x, a.x_codes, a.x_scales);
+        return at;
+    }
+    Tensor make(kanb200_block_args& a, const Tensor& like) const {
+        const int64_t bytes = lay(a, nullptr);
+        if (bytes == 0) return Tensor();
+        Tensor t = fresh({bytes}, at::kByte, like);
+        lay(a, static_cast<char*>(t.data_ptr()));
+        return t;
+    }
+    void find(kanb200_block_args& a, const Tensor& t) const {
+        if (t.defined()) lay(a, static_cast<char*>(t.data_ptr()));
+    }
+};
 
 void run_backward(kanb200_block_args& a, const Tensor& like, cudaStream_t st) {
     const size_t bytes = kanb200_block_backward_workspace_bytes(&a);
     Tensor ws;
-    if (bytes) ws = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    if (bytes) ws = fresh({(int64_t)bytes}, at::kByte, like);
     check_rc(kanb200_block_backward(&a, mptr(ws), bytes, st));
 }
 
@@ -138,33 +178,28 @@ void check_norm(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind,
     check_vector(b, what, "bias", x.size(-1), branch_type(x), x);
 }
 
-struct NormSaved {
-    Tensor stats;
-    Packed packed;
-};
-
+Record norm_record(int64_t checkpoint) {
+    Record r;
+    r.next = true;
+    r.x = checkpoint != KANB200_PACK_NONE;
+    return r;
+}
+// `record`: where what the backward needs goes (NULL: no backward)
 Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind, double eps, int64_t checkpoint,
-                    NormSaved* saved) {
+                    Tensor* record) {
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
-    const at::ScalarType type = branch_type(x);
-    Tensor h = at::empty(x.sizes(), x.options().dtype(type));
+    Tensor h = fresh(x.sizes(), branch_type(x), x);
     kanb200_block_args a{};
     a.dtype = stream_code(x, "block_norm");
     a.rows = row_count(x);
     a.width = x.size(-1);
     a.next_norm = (int)kind;
     a.eps = eps;
-    if (saved) {
-        saved->stats = at::empty({a.rows, 2}, h.options());
-        a.next_stats = mptr(saved->stats);
-        if (checkpoint != KANB200_PACK_NONE) {
-            saved->packed = new_codes(a.rows, a.width, (int)checkpoint, x, type);
-            a.checkpoint = (int)checkpoint;
-            a.x_codes = mptr(saved->packed.codes);
-            a.x_scales = mptr(saved->packed.scales);
-        }
+    if (record) {
+        a.checkpoint = (int)checkpoint;
+        *record = norm_record(checkpoint).make(a, x);
     }
     const Rows xr = as_rows(x, a.rows, a.width);
     const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
@@ -231,7 +266,7 @@ struct BlockNormNode : public SavedNode {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list result(3);
         if (!grads[0].defined()) return result;
-        const Tensor x = kept(0), w = kept(1), stats = kept(2), codes = kept(3), scales = kept(4);
+        const Tensor x = kept(0), w = kept(1), record = kept(2);
         if (at::GradMode::is_enabled()) {
             TORCH_CHECK(checkpoint == KANB200_PACK_NONE,
                         "block_norm: create_graph=True needs the input itself, not its 8-bit checkpoint");
@@ -239,16 +274,18 @@ struct BlockNormNode : public SavedNode {
             result[0] = result[0].to(type);
             return result;
         }
-        c10::cuda::CUDAGuard guard(stats.device());
+        const Tensor& like = grads[0];
+        c10::cuda::CUDAGuard guard(like.device());
         const cudaStream_t st = at::cuda::getCurrentCUDAStream();
+        const at::ScalarType branch = type == at::kDouble ? at::kDouble : at::kFloat;
         kanb200_block_args a{};
-        a.width = shape.back();
-        a.rows = stats.size(0);
-        const Rows xr = as_rows(x, a.rows, a.width), dr = as_rows(grads[0], a.rows, a.width);
-        if (need(0)) result[0] = at::empty(shape, stats.options().dtype(type));
-        if (need(1)) result[1] = at::empty({a.width}, stats.options());
-        if (need(2)) result[2] = at::empty({a.width}, stats.options());
         a.dtype = type_code(type);
+        a.width = shape.back();
+        a.rows = grads[0].numel() / a.width;
+        const Rows xr = as_rows(x, a.rows, a.width), dr = as_rows(grads[0], a.rows, a.width);
+        if (need(0)) result[0] = fresh(shape, type, like);
+        if (need(1)) result[1] = fresh({a.width}, branch, like);
+        if (need(2)) result[2] = fresh({a.width}, branch, like);
         a.next_norm = (int)kind;
         a.checkpoint = (int)checkpoint;
         a.eps = eps;
@@ -256,15 +293,13 @@ struct BlockNormNode : public SavedNode {
         a.x_stride = xr.stride;
         const Tensor wc = w.defined() ? w.contiguous() : w;
         a.next_weight = cptr(wc);
-        a.next_stats = const_cast<void*>(cptr(stats));
-        a.x_codes = const_cast<void*>(cptr(codes));
-        a.x_scales = const_cast<void*>(cptr(scales));
+        norm_record(checkpoint).find(a, record);
         a.dh = dr.ptr();
         a.dh_stride = dr.stride;
         a.dx = mptr(result[0]);
         a.dnext_weight = mptr(result[1]);
         a.dnext_bias = mptr(result[2]);
-        run_backward(a, stats, st);
+        run_backward(a, like, st);
         return result;
     }
 };
@@ -276,16 +311,16 @@ Tensor block_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     TORCH_CHECK(x.is_cuda() || checkpoint == KANB200_PACK_NONE, "block_norm: 8-bit checkpoints need CUDA tensors");
     if (!x.is_cuda() || x.numel() == 0) return norm_composite(x, w, b, kind, eps);
     if (!wants_grad({x, w, b}, "block_norm")) return norm_forward(x, w, b, kind, eps, checkpoint, nullptr);
-    NormSaved s;
-    Tensor h = norm_forward(x, w, b, kind, eps, checkpoint, &s);
+    Tensor record;
+    Tensor h = norm_forward(x, w, b, kind, eps, checkpoint, &record);
     auto node = new_node<BlockNormNode>({x, w, b});
     node->kind = kind;
     node->eps = eps;
     node->checkpoint = checkpoint;
     node->type = x.scalar_type();
     node->shape = x.sizes().vec();
-    for (const Tensor& t : {checkpoint != KANB200_PACK_NONE ? Tensor() : x, w, s.stats, s.packed.codes, s.packed.scales})
-        node->keep(t);
+    node->saved.reserve(3);
+    for (const Tensor& t : {checkpoint != KANB200_PACK_NONE ? Tensor() : x, w, record}) node->keep(t);
     torch::autograd::set_history(h, node);
     return h;
 }
@@ -299,6 +334,7 @@ struct Gated {
     int64_t act = 0, post = 0, next = 0, checkpoint = 0;
     double eps = 0;
     int64_t rows = 0, width = 0, gate_rows = 1;
+    bool row_gate = false;             // a gate of its own for every row
 
     bool gated() const { return packed || gate.defined(); }
 };
@@ -340,6 +376,7 @@ void check_gated(Gated& g) {
                     t.sizes());
         g.gate_rows = own > 0 ? std::max<int64_t>(g.rows / own, 1) : 1;
     }
+    g.row_gate = g.gated() && g.gate_rows == 1;
     check_vector(g.scale, what, "scale", g.width, type, x);
     check_vector(g.pw, what, "post_weight", g.width, type, x);
     check_vector(g.pb, what, "post_bias", g.width, type, x);
@@ -367,19 +404,14 @@ variable_list gated_composite(const Gated& g) {
     return {out, norm_composite(out, g.nw, g.nb, g.next, g.eps)};
 }
 
-struct GatedSaved {
-    Tensor stats;                                            // [norms, rows, 2], the post norm's first
-    Packed y, gate, out;
-};
-// the two norms' parts of it
-void stats_of(kanb200_block_args& a, const Tensor& stats, int64_t post, int64_t next) {
-    if (!stats.defined()) return;
-    char* at = static_cast<char*>(const_cast<void*>(cptr(stats)));
-    if (post != KANB200_NORM_NONE) {
-        a.post_stats = at;
-        at += a.rows * 2 * stats.element_size();
-    }
-    if (next != KANB200_NORM_NONE) a.next_stats = at;
+Record gated_record(const Gated& g) {
+    Record r;
+    r.post = g.post != KANB200_NORM_NONE;
+    r.next = g.next != KANB200_NORM_NONE;
+    r.y = g.checkpoint != KANB200_PACK_NONE;
+    r.gate = r.y && g.row_gate;
+    r.x = r.y && r.next;
+    return r;
 }
 
 void fill(kanb200_block_args& a, const Gated& g) {
@@ -405,37 +437,18 @@ void branch_rows(const Gated& g, Rows& y, const void*& gate, int64_t& gate_strid
     }
 }
 
-variable_list gated_forward(const Gated& g, GatedSaved* saved) {
+variable_list gated_forward(const Gated& g, Tensor* record) {
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(g.x.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
-    const at::ScalarType type = branch_type(g.x);
-    const auto branch = g.x.options().dtype(type);
-    Tensor out = at::empty(g.x.sizes(), g.x.options()), h;
-    if (g.next != KANB200_NORM_NONE) h = at::empty(g.x.sizes(), branch);
+    Tensor out = fresh(g.x.sizes(), g.x.scalar_type(), g.x), h;
+    if (g.next != KANB200_NORM_NONE) h = fresh(g.x.sizes(), branch_type(g.x), g.x);
     kanb200_block_args a{};
-    fill(a, g);
     a.dtype = stream_code(g.x, "gated_residual");
-    if (saved) {
-        const int64_t norms = (g.post != KANB200_NORM_NONE) + (g.next != KANB200_NORM_NONE);
-        if (norms) saved->stats = at::empty({norms, g.rows, 2}, branch);
-        stats_of(a, saved->stats, g.post, g.next);
-        if (g.checkpoint != KANB200_PACK_NONE) {
-            a.checkpoint = (int)g.checkpoint;
-            saved->y = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
-            a.y_codes = mptr(saved->y.codes);
-            a.y_scales = mptr(saved->y.scales);
-            if (g.gated() && g.gate_rows == 1) {
-                saved->gate = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
-                a.gate_codes = mptr(saved->gate.codes);
-                a.gate_scales = mptr(saved->gate.scales);
-            }
-            if (h.defined()) {
-                saved->out = new_codes(g.rows, g.width, a.checkpoint, g.x, type);
-                a.x_codes = mptr(saved->out.codes);
-                a.x_scales = mptr(saved->out.scales);
-            }
-        }
+    fill(a, g);
+    if (record) {
+        a.checkpoint = (int)g.checkpoint;
+        *record = gated_record(g).make(a, g.x);
     }
     const Rows xr = as_rows(g.x, g.rows, g.width);
     Rows yr, gr;
@@ -472,7 +485,7 @@ struct GatedResidualNode : public SavedNode {
         variable_list result(kGatedInputs);
         const Tensor dout = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
         if (!dout.defined() && !dh.defined()) return result;
-        std::array<Tensor, 14> v;
+        std::array<Tensor, 8> v;
         for (size_t i = 0; i < v.size(); ++i) v[i] = kept(i);
         Gated g = settings;
         g.y = v[1];
@@ -490,7 +503,7 @@ struct GatedResidualNode : public SavedNode {
         const Tensor& like = dout.defined() ? dout : dh;
         c10::cuda::CUDAGuard guard(like.device());
         const cudaStream_t st = at::cuda::getCurrentCUDAStream();
-        const auto branch = like.options().dtype(type == at::kDouble ? at::kDouble : at::kFloat);
+        const at::ScalarType branch = type == at::kDouble ? at::kDouble : at::kFloat;
         kanb200_block_args a{};
         fill(a, g);
         if (!dh.defined()) a.next_norm = KANB200_NORM_NONE;
@@ -500,19 +513,19 @@ struct GatedResidualNode : public SavedNode {
         Tensor dx, dy, dgate;
         if (need(kX)) {
             // without a norm behind, the stream's gradient passes through unchanged
-            if (dh.defined()) dx = at::empty(shape, like.options().dtype(type));
+            if (dh.defined()) dx = fresh(shape, type, like);
             else result[kX] = dout;
         }
         const bool want_gate = g.packed ? need(kY) : need(kGate);
         if (need(kY)) {
             auto s = shape;
             if (g.packed) s.back() *= 2;
-            dy = at::empty(s, branch);
+            dy = fresh(s, branch, like);
             a.dy_stride = s.back();
         }
-        if (want_gate && !g.packed) dgate = at::empty(gate_shape, branch);
+        if (want_gate && !g.packed) dgate = fresh(gate_shape, branch, like);
         const auto vec = [&](int i) {
-            if (need(i)) result[i] = at::empty({g.width}, branch);
+            if (need(i)) result[i] = fresh({g.width}, branch, like);
             return mptr(result[i]);
         };
         a.dscale = vec(kScale);
@@ -541,15 +554,8 @@ struct GatedResidualNode : public SavedNode {
         a.post_weight = cptr(pw);
         a.post_bias = cptr(pb);
         if (dh.defined()) a.next_weight = cptr(nw);
-        stats_of(a, v[7], g.post, g.next);
-        if (dh.defined()) {
-            a.x_codes = const_cast<void*>(cptr(v[8]));
-            a.x_scales = const_cast<void*>(cptr(v[9]));
-        }
-        a.y_codes = const_cast<void*>(cptr(v[10]));
-        a.y_scales = const_cast<void*>(cptr(v[11]));
-        a.gate_codes = const_cast<void*>(cptr(v[12]));
-        a.gate_scales = const_cast<void*>(cptr(v[13]));
+        gated_record(g).find(a, v[7]);
+        if (!dh.defined()) a.x_codes = a.x_scales = nullptr;
         a.dout = dor.ptr();
         a.dout_stride = dor.stride;
         a.dh = dhr.ptr();
@@ -617,8 +623,8 @@ py::object gated_residual(const Tensor& x, const Tensor& y, const std::optional<
     } else if (!wants_grad({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb}, "gated_residual")) {
         outs = gated_forward(g, nullptr);
     } else {
-        GatedSaved saved;
-        outs = gated_forward(g, &saved);
+        Tensor record;
+        outs = gated_forward(g, &record);
         auto node = new_node<GatedResidualNode>({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb});
         node->settings = g;
         for (Tensor Gated::*t : {&Gated::x, &Gated::y, &Gated::gate, &Gated::scale, &Gated::pw, &Gated::pb, &Gated::nw, &Gated::nb})
@@ -628,11 +634,9 @@ py::object gated_residual(const Tensor& x, const Tensor& y, const std::optional<
         if (g.gate.defined()) node->gate_shape = g.gate.sizes().vec();
         for (Tensor& t : outs) torch::autograd::set_history(t, node);
         const bool codes = checkpoint != KANB200_PACK_NONE, keep_gate = !codes || g.gate_rows > 1;
-        node->saved.reserve(14);
+        node->saved.reserve(8);
         node->keep(next != KANB200_NORM_NONE && !codes ? outs[0] : Tensor(), true);
-        for (const Tensor& t : {codes ? Tensor() : g.y, keep_gate ? g.gate : Tensor(), g.scale, g.pw, g.pb, g.nw, saved.stats,
-                                saved.out.codes, saved.out.scales, saved.y.codes, saved.y.scales, saved.gate.codes,
-                                saved.gate.scales})
+        for (const Tensor& t : {codes ? Tensor() : g.y, keep_gate ? g.gate : Tensor(), g.scale, g.pw, g.pb, g.nw, record})
             node->keep(t);
     }
     if (outs.size() == 1) return py::cast(outs[0]);
@@ -653,7 +657,8 @@ Packed pack_rows(const Tensor& x, int format) {
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     const int64_t rows = row_count(x), width = x.size(-1);
     auto shape = x.sizes().vec();
-    Packed p = new_codes(rows, width, format, x, branch_type(x));
+    Packed p{fresh({rows, width}, format == KANB200_PACK_INT8 ? at::kChar : at::kFloat8_e4m3fn, x),
+             fresh({rows, group_count(width)}, branch_type(x), x)};
     const Rows xr = as_rows(x, rows, width);
     check_rc(kanb200_pack_activation(code, format, xr.ptr(), xr.stride, mptr(p.codes), mptr(p.scales), rows, width, st));
     if (x.dim() != 2) {
@@ -683,7 +688,7 @@ Tensor unpack_rows(const Tensor& codes, const Tensor& scales, at::ScalarType dty
     c10::cuda::CUDAGuard guard(codes.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     const Tensor cc = codes.contiguous(), sc = scales.contiguous();
-    Tensor x = at::empty(codes.sizes(), codes.options().dtype(dtype));
+    Tensor x = fresh(codes.sizes(), dtype, codes);
     check_rc(kanb200_unpack_activation(stream_code(x, what),
                                        codes.scalar_type() == at::kChar ? KANB200_PACK_INT8 : KANB200_PACK_E4M3, cptr(cc),
                                        cptr(sc), mptr(x), row_count(codes), codes.size(-1), st));
