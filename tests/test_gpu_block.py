@@ -201,6 +201,17 @@ def test_gated_options(gate, post, next, form):
         check_gated(make_gated((3, 5), 132, dtype, gate, act, scale, post, next, form))
 
 
+@pytest.mark.parametrize("rows,width,dtype", [(9, 5, torch.float32), (3, 40, torch.float64), (5, 270, torch.float32),
+                                              (5, 592, torch.bfloat16), (3, 2060, torch.float32), (2, 8195, torch.float32)])
+@pytest.mark.parametrize("absent", [("scale", "pw", "pb", "nw", "nb"), ("scale", "pw"), ("scale",), ("pw",), ("pb", "nb"), ("nw",)])
+def test_absent_parameters(rows, width, dtype, absent):
+    """Widths that leave threads without a column, and the parameters whose place a constant takes."""
+    for post, next, gate in itertools.product(["rms", "layer"], ["rms", "layer"], ["row", None, "all"]):
+        c = make_gated(rows, width, dtype, gate, post=post, next=next)
+        c.update((name, None) for name in absent)
+        check_gated(c)
+
+
 @pytest.mark.parametrize("lead,width,gate", [((1, 1), 64, "sequence"), ((1, 2000), 40, "sequence"), ((7, 311), 96, "sequence"),
                                              ((1500, 2), 33, "sequence"), ((2, 3, 70), 260, "sequence"), ((2500,), 24, "all"),
                                              ((2, 900), 1030, "all"), ((3, 1), 48, "sequence"), ((400, 5), 1, "sequence"),

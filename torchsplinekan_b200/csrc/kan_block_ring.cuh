@@ -123,8 +123,17 @@ template <typename B, typename C> __device__ __forceinline__ Four<B> get(const B
         if (c.ok(j, r)) move<C::SIDE * (int)sizeof(B)>(q.v + r, row + C::apart(j, r));
     return widen4<B>(q);
 }
+// ... or `absent` where there is no such parameter, 0 beyond the row as well: what a mean-subtracting norm's backward leaves
+// in the columns beyond the row (its mean) has to stay out of the sums behind it.
 template <typename B, typename C> __device__ __forceinline__ Four<B> get_or(const void* p, const C& c, int j, B absent) {
-    return p ? get(static_cast<const B*>(p) + c.col, c, j) : four<B>(absent);
+    Four<B> ones = four<B>(absent);
+    if constexpr (C::MODE != kFull) {
+        Quad<B> q;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q.v[r] = c.ok(j, r / C::SIDE * C::SIDE) ? absent : B(0);
+        ones = widen4<B>(q);
+    }
+    return p ? get(static_cast<const B*>(p) + c.col, c, j) : ones;
 }
 // x - mean for the row's own columns; 0 beyond them, where x is 0
 template <typename B, typename C> __device__ __forceinline__ Four<B> centre(const C& c, int j, const Four<B>& x, B mean) {
