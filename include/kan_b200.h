@@ -357,7 +357,7 @@ KANB200_API int kanb200_allreduce_sum_f32_ranges(const void* const* peer_bases, 
  *   gate row.  The sums over rows go through slabs in the workspace that a second kernel adds in a fixed order: no
  *   atomics, the same bits on every run.
  * Row strides are in elements; a row's columns are contiguous.  out, h, dx, codes and scales are dense; the statistics
- * are aligned to two of their elements. */
+ * are aligned to two of their elements, everything else (parameters and their gradients too) to its own element. */
 #define KANB200_F16  2   /* stream types of these operators only */
 #define KANB200_BF16 3
 
@@ -401,6 +401,11 @@ typedef struct kanb200_block_args {
     void* dscale;       void* dpost_weight;  void* dpost_bias;  void* dnext_weight;  void* dnext_bias;   /* [width] */
 } kanb200_block_args;
 
+/* Columns that this call's kernels move at once: 4 where width, row strides and every pointer (parameters included) allow
+ * 16-byte accesses of the branch's type, 1 otherwise (any alignment of the elements' own size will do, at a lower rate) and
+ * for rows too wide for registers.  backward = 1: as kanb200_block_backward, else as kanb200_block_forward.  Negative: the
+ * call would be refused. */
+KANB200_API int kanb200_block_columns_at_once(const kanb200_block_args* args, int backward);
 KANB200_API int kanb200_block_forward(const kanb200_block_args* args, void* stream);
 /* scratch of kanb200_block_backward for these arguments (plain scratch, no status header; 0 = none) */
 KANB200_API size_t kanb200_block_backward_workspace_bytes(const kanb200_block_args* args);

@@ -289,6 +289,48 @@ def test_layouts(how, dtype):
         assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [64, 1024, 8192])
+def test_parameters_that_are_views_into_a_flat_buffer(width, dtype):
+    """Every parameter one element behind a 16-byte boundary, each alone and all of them, forward and backward."""
+    bt = branch_type(dtype)
+    w, b, dh = randn(width, dtype=bt, seed=2), randn(width, dtype=bt, seed=3), randn(9, width, dtype=bt, seed=4)
+    for shifted in (("w",), ("b",), ("w", "b")):
+        check_norm(stream(9, width, dtype), strided(w, "shifted") if "w" in shifted else w,
+                   strided(b, "shifted") if "b" in shifted else b, "layer", "int8" if width == 64 else None, dh)
+    names = ("scale", "pw", "pb", "nw", "nb")
+    for gate, shifted in (("row", names), ("sequence", names), *((None, (n,)) for n in names)):
+        c = make_gated((3, 4), width, dtype, gate, None if gate is None else "silu", post="layer", next="layer")
+        for n in shifted:
+            c[n] = strided(c[n], "shifted")
+            assert c[n].is_contiguous() and c[n].data_ptr() % 16 != 0
+        check_gated(c)
+
+
+def test_column_sums_at_any_address():
+    """The C entry point with parameter gradients that 16-byte stores cannot reach, from one block and from many."""
+    import ctypes
+    from torchsplinekan_b200 import _native
+    for rows, width in ((3, 64), (900, 64), (3, 1024), (700, 1024)):
+        x, w = stream(rows, width, torch.float32), randn(width, dtype=torch.float32, seed=2)
+        dh = randn(rows, width, dtype=torch.float32, seed=4)
+        leaves = [w.clone().requires_grad_(), torch.zeros(width, device="cuda", requires_grad=True)]
+        want = torch.autograd.grad(sk.block_norm(x, *leaves, kind="layer", eps=EPS), leaves, dh)
+        h, stats = torch.empty_like(x), torch.empty(rows, 2, device="cuda")
+        flat = torch.full((2, width + 2), float("nan"), device="cuda")
+        a = _native.BlockArgs(dtype=_native.F32, next_norm=_native.NORM_LAYER, eps=EPS, rows=rows, width=width,
+                              x=x.data_ptr(), x_stride=width, next_weight=w.data_ptr(), next_stats=stats.data_ptr(),
+                              h=h.data_ptr(), dh=dh.data_ptr(), dh_stride=width, dnext_weight=flat.data_ptr() + 4,
+                              dnext_bias=flat.data_ptr() + 4 * (width + 3))
+        lib, st = _native.lib(), torch.cuda.current_stream().cuda_stream
+        assert lib.kanb200_block_forward(ctypes.byref(a), st) == 0
+        need = lib.kanb200_block_backward_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        assert need > 0 and lib.kanb200_block_backward(ctypes.byref(a), ws.data_ptr(), need, st) == 0
+        for row, v in zip(flat, want):
+            assert torch.equal(row[1:-1], v) and bool(torch.isnan(row[[0, -1]]).all())
+
+
 def test_broadcast_rows_and_gradients():
     """Rows of stride 0 in the inputs and in the incoming gradients."""
     one = randn(1, 96, dtype=torch.float32).expand(50, 96)

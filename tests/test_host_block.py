@@ -171,3 +171,48 @@ def test_networks_of_blocks_on_the_dense_backend():
         sk.GatedResidual(8)(torch.zeros(2, 8), torch.zeros(2, 8), sk.BlockNorm(8, eps=1e-3))
     with pytest.raises(ValueError, match="chains"):
         sk.KAN([4, 4, 4], residual=True).prune(torch.zeros(3, 4))
+
+
+PARAMETERS = ("scale", "post_weight", "post_bias", "next_weight", "next_bias")
+
+
+def block_call(width, dtype, backward, rows=700, **kw):
+    """Arguments of a connection with everything, all pointers aligned (nothing here is launched)."""
+    p = 1 << 20
+    a = dict(dtype=dtype, post_norm=_native.NORM_LAYER, next_norm=_native.NORM_LAYER, eps=1e-6, rows=rows, width=width, x=p,
+             x_stride=width, y=p, y_stride=width, gate=p, gate_stride=width, gate_rows=1, post_stats=p, next_stats=p,
+             **{n: p for n in PARAMETERS})
+    if backward:
+        a.update(has_branch=1, dout=p, dout_stride=width, dh=p, dh_stride=width, dx=p, dy=p, dy_stride=width, dgate=p,
+                 dgate_stride=width, **{"d" + n: p for n in PARAMETERS})
+    else:
+        a.update(out=p, h=p)
+    return _native.BlockArgs(**{**a, **kw})
+
+
+@pytest.mark.parametrize("dtype", [_native.F32, _native.F64, _native.F16, _native.BF16])
+@pytest.mark.parametrize("width", [64, 1024, 8192])
+@pytest.mark.parametrize("backward", [0, 1])
+def test_parameters_of_any_alignment_are_not_read_16_bytes_at_a_time(dtype, width, backward):
+    lib, element, p = _native.lib(), 8 if dtype == _native.F64 else 4, 1 << 20
+    at_once = lambda **kw: lib.kanb200_block_columns_at_once(ctypes.byref(block_call(width, dtype, backward, **kw)), backward)
+    assert at_once() == 4
+    for name in PARAMETERS:
+        assert at_once(**{name: p + element}) == 1, name
+    assert at_once(rows=-1) == _native.EINVAL
+    # parameters of a norm alone
+    alone = dict(y=None, gate=None, scale=None, post_norm=0, post_weight=None, post_bias=None)
+    if backward:
+        alone.update(has_branch=0, dy=None, dgate=None, dscale=None, dpost_weight=None, dpost_bias=None)
+    assert at_once(**alone) == 4 and at_once(**alone, next_weight=p + element) == 1
+
+
+@pytest.mark.parametrize("dtype", [_native.F32, _native.F64, _native.F16, _native.BF16])
+def test_column_sums_of_any_alignment_leave_through_a_slab(dtype):
+    """A handful of rows runs in one block that stores the parameters' gradients itself, 16 bytes at a time; a result that
+    such stores cannot reach goes through scratch and the kernel that adds slabs element by element."""
+    lib, element, p = _native.lib(), 8 if dtype == _native.F64 else 4, 1 << 20
+    need = lambda **kw: lib.kanb200_block_backward_workspace_bytes(ctypes.byref(block_call(1024, dtype, 1, rows=3, **kw)))
+    assert need() == 0
+    for name in PARAMETERS:
+        assert need(**{"d" + name: p + element}) >= 1024 * element, name

@@ -96,6 +96,7 @@ SIGNATURES = {
     "kanb200_backward_param_rows": (_c_int, [_c_int] + [_c_void_p] * 9 + [_c_i64, _c_i64, _c_i64, _c_int, _c_int,
                                                                           _c_i64, _c_i64, _c_void_p, _c_size,
                                                                           _c_void_p]),
+    "kanb200_block_columns_at_once": (_c_int, [_c_void_p, _c_int]),
     "kanb200_block_forward": (_c_int, [_c_void_p, _c_void_p]),
     "kanb200_block_backward_workspace_bytes": (_c_size, [_c_void_p]),
     "kanb200_block_backward": (_c_int, [_c_void_p, _c_void_p, _c_size, _c_void_p]),

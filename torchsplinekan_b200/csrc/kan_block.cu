@@ -354,6 +354,9 @@ bool four_at_once(const kanb200_block_args& a) {
         if (!aligned(p, s)) return false;
     for (const void* p : {a.y, a.gate, (const void*)a.h, a.dh, (const void*)a.dy, (const void*)a.dgate})
         if (!aligned(p, b)) return false;
+    // a parameter may be a view into a flat buffer, anywhere an element may be
+    for (const void* p : {a.scale, a.post_weight, a.post_bias, a.next_weight, a.next_bias})
+        if (!aligned(p, b)) return false;
     for (const void* p : {a.x_codes, a.y_codes, a.gate_codes})
         if (!aligned(p, 4)) return false;
     return true;
@@ -470,7 +473,8 @@ struct BackwardPlan {
     size_t bytes;
 };
 
-// slabs of the column sums first, then those of a shared gate
+// Slabs of the column sums first, then those of a shared gate.  A single slab row is the result itself, where the kernel's
+// 16-byte stores can reach that.
 BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
     BackwardPlan p{};
     p.use_ring = ring_fits(a, true);
@@ -491,7 +495,7 @@ BackwardPlan plan_backward(const kanb200_block_args& a, void* ws) {
     void* outs[kColumnSums];
     column_outputs(a, outs);
     for (int k = 0; k < kColumnSums; ++k)
-        p.slabs.column[k] = !outs[k] ? nullptr : p.slab_rows == 1 ? outs[k] : take(row * p.slab_rows);
+        p.slabs.column[k] = !outs[k] ? nullptr : p.slab_rows == 1 && aligned(outs[k], 16) ? outs[k] : take(row * p.slab_rows);
     if (a.dgate && p.split.shared) p.slabs.gate = take(row * (p.split.teams + a.rows / a.gate_rows));
     return p;
 }
@@ -553,6 +557,10 @@ cudaError_t allow_shared_memory(const void* kernel) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (e == cudaSuccess) allowed.insert({kernel, device});
     return e;
+}
+
+int block_columns_at_once(const kanb200_block_args& a, bool backward) {
+    return a.rows > 0 && ring_fits(a, backward) && plan_ring(a, backward).mode != kScalar ? 4 : 1;
 }
 
 cudaError_t block_forward(const kanb200_block_args& a, cudaStream_t st) {

@@ -14,6 +14,7 @@ constexpr int kNormNone = KANB200_NORM_NONE, kNormRms = KANB200_NORM_RMS, kNormL
 constexpr int kPackNone = KANB200_PACK_NONE, kPackInt8 = KANB200_PACK_INT8, kPackE4m3 = KANB200_PACK_E4M3;
 constexpr int kPackGroup = KANB200_PACK_GROUP;
 
+int block_columns_at_once(const kanb200_block_args& a, bool backward);
 cudaError_t block_forward(const kanb200_block_args& a, cudaStream_t st);
 size_t block_backward_workspace(const kanb200_block_args& a);
 cudaError_t block_backward(const kanb200_block_args& a, void* ws, size_t ws_bytes, cudaStream_t st);

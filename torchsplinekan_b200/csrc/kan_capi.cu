@@ -783,6 +783,11 @@ KANB200_API int kanb200_allreduce_sum_f32(const void* const* peer_bases, void* m
                                             rank, world, local_ranks, blocks, 512, scale, status, stream);
 }
 
+KANB200_API int kanb200_block_columns_at_once(const kanb200_block_args* args, int backward) {
+    const int rc = check_block(args, backward != 0);
+    return rc != KANB200_OK ? rc : block_columns_at_once(*args, backward != 0);
+}
+
 KANB200_API int kanb200_block_forward(const kanb200_block_args* args, void* stream) {
     const int rc = check_block(args, false);
     if (rc != KANB200_OK || args->rows == 0) return rc;
