@@ -407,7 +407,7 @@ typedef struct kanb200_block_args {
  * call would be refused. */
 KANB200_API int kanb200_block_columns_at_once(const kanb200_block_args* args, int backward);
 KANB200_API int kanb200_block_forward(const kanb200_block_args* args, void* stream);
-/* scratch of kanb200_block_backward for these arguments (plain scratch, no status header; 0 = none) */
+/* scratch of kanb200_block_backward for these arguments (plain scratch, no status header, aligned to 16 bytes; 0 = none) */
 KANB200_API size_t kanb200_block_backward_workspace_bytes(const kanb200_block_args* args);
 KANB200_API int kanb200_block_backward(const kanb200_block_args* args, void* workspace, size_t workspace_bytes,
                                        void* stream);

@@ -216,3 +216,13 @@ def test_column_sums_of_any_alignment_leave_through_a_slab(dtype):
     assert need() == 0
     for name in PARAMETERS:
         assert need(**{"d" + name: p + element}) >= 1024 * element, name
+
+
+def test_scratch_that_16_byte_stores_cannot_reach_is_refused():
+    lib = _native.lib()
+    a = block_call(1024, _native.F32, 1)
+    need = lib.kanb200_block_backward_workspace_bytes(ctypes.byref(a))
+    assert need > 0
+    for off in (4, 8):
+        assert lib.kanb200_block_backward(ctypes.byref(a), (1 << 20) + off, need, None) == _native.EINVAL
+        assert "workspace" in _native.last_error()

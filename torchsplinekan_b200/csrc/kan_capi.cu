@@ -813,6 +813,8 @@ KANB200_API int kanb200_block_backward(const kanb200_block_args* args, void* wor
         }
         return KANB200_OK;
     }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16)
+        return fail(KANB200_EINVAL, "block_backward: the workspace must be aligned to 16 bytes");
     const cudaError_t e = block_backward(*args, workspace, workspace ? workspace_bytes : 0, st);
     return e == cudaSuccess ? KANB200_OK : cuda_fail(e, "block_backward");
 }
