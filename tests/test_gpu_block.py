@@ -230,6 +230,17 @@ def test_many_rows(rows, width, dtype):
     check_gated(make_gated(rows, width, dtype))
 
 
+@pytest.mark.parametrize("rows,width", [(60000, 24), (40000, 60), (20000, 132), (5000, 1030), (1200, 4100)])
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_many_rows_without_a_sum_over_the_row(rows, width, form):
+    """Scales and statistics that one lane brings for all, row after row, where nothing else keeps the lanes together: no
+    post norm behind its codes, or one whose input needs no gradient.  Gradients per row, so a scale of another row shows."""
+    for gate in ("row", "packed"):
+        check_gated(make_gated(rows, width, torch.float32, gate, post=None, next=None, form=form))
+    check_gated(make_gated(rows, width, torch.bfloat16, "row", post="layer", next=None, form=form), only=("x", "gate", "scale"))
+    check_gated(make_gated(rows, width, torch.float32, "row", post="rms", next="rms", form=form), only=("gate",))
+
+
 def test_only_one_result_used():
     c = make_gated(40, 200, torch.float32)
     check_gated(c, use_h=False)

@@ -7,7 +7,8 @@
 //     forward 99 us against 91).
 //   * Memory -> registers goes through a ring of 2 to 4 rows in shared memory, filled by cp.async.  A thread copies
 //     exactly what it reads back itself, so the ring needs no barrier: only its own cp.async group to have landed.  The
-//     bytes in flight then do not depend on registers or on how many warps wait in a barrier.
+//     bytes in flight then do not depend on registers or on how many warps wait in a barrier.  (Statistics and scales in the
+//     backward are one lane's copies for its team's lanes: a __syncwarp on either side of them.)
 //   * Parameters stay on chip: in registers in the forward, in shared memory in the backward, where the registers hold the
 //     sums over rows that are their gradients (one slab row per block leaves the kernel at its end).  Read from L1 for every
 //     row they came from L2 whenever the ring took most of the SM's memory, a few hundred cycles at a time (gated forward of
@@ -581,9 +582,12 @@ __global__ void __launch_bounds__(ring_threads(BIG), ring_blocks(BIG, sizeof(S) 
     for (int s = 0; s + 1 < p.stages; ++s, ahead += next) issue(ahead, s);
     int stage = 0;
     for (uint32_t step = 0, row = first; step < p.rows_per_team; ++step, row += next, ahead += next) {
+        // The slot that is filled now is the one the step before has read, statistics and scales by all lanes but copied by one:
+        // that lane waits for the others (a sum over the row may be the last thing that kept them together, or there was none).
+        __syncwarp();
         issue(ahead, stage == 0 ? p.stages - 1 : stage - 1);
         copies_wait_oldest(p.stages);
-        __syncwarp();
+        __syncwarp();                                       // ... and the others for its copies
         const bool live = row < last;
         if (LANES == 32 && !live) break;
         const char* at = ring + stage * p.stage_bytes;
