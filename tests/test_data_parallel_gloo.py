@@ -95,3 +95,37 @@ def test_global_batch_regulariser_equals_unsharded(tmp_path):
     world = 2
     mp.spawn(_reg_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True)
     assert all((tmp_path / f"ok{r}.pt").exists() for r in range(world))
+
+
+def _block_worker(rank, world, port, result_dir):
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    import torchsplinekan_b200 as sk
+    make = lambda: sk.KAN([6, 8, 8, 8, 3], norm="layer", residual=True, gate="silu", backend="reference").double()
+    torch.manual_seed(0)
+    net, full = make(), make()
+    full.load_state_dict(net.state_dict())
+    x = torch.randn(37, 6, dtype=torch.float64, generator=torch.Generator().manual_seed(1))
+    full(x).square().sum().backward()
+    assert [type(m).__name__ for m in net.parameter_modules()] == [
+        "BlockNorm", "KANLinear", "BlockNorm", "KANLinear", "GatedResidual", "BlockNorm", "KANLinear", "GatedResidual",
+        "BlockNorm", "KANLinear"]
+    bucket = sk.GradientBucket(net)
+    assert bucket.bucket_bytes() == sum(p.numel() for p in net.parameters()) * 8
+    a, b = sk.shard_rows(x.shape[0], world, rank)
+    for step in range(2):
+        bucket.zero_grad()
+        net(x[a:b]).square().sum().backward()
+        bucket.finish()
+        for (n, p), q in zip(net.named_parameters(), full.parameters()):
+            assert torch.allclose(p.grad, q.grad, rtol=1e-9, atol=1e-11), (rank, step, n)
+    torch.save(torch.tensor(1), os.path.join(result_dir, f"ok{rank}.pt"))
+    dist.destroy_process_group()
+
+
+def test_networks_of_blocks_reduce_every_parameter(tmp_path):
+    """Norms and residual connections own parameters of their own: all of them get the whole batch's gradients."""
+    world = 2
+    mp.spawn(_block_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True)
+    assert all((tmp_path / f"ok{r}.pt").exists() for r in range(world))

@@ -19,7 +19,7 @@ and the reduction is this library's own kernel (``kanb200_allreduce_sum_f32``: i
 from __future__ import annotations
 
 import os
-from typing import Iterable, List, Optional, Tuple
+from typing import Iterable, List, Optional, Tuple, Union
 
 import torch
 import torch.distributed as dist
@@ -103,8 +103,10 @@ def _layer_params(layer: nn.Module) -> List[nn.Parameter]:
 class GradientBucket:
     """Flat per-layer gradient buckets with an overlapped all-reduce.
 
-    ``layers``: modules in forward order (each gets one bucket).  Call
-    :meth:`finish` after ``loss.backward()`` and before the optimiser step.
+    ``layers``: modules in forward order (each gets one bucket), or a :class:`KAN`, which stands for all
+    modules that own its parameters (:meth:`KAN.parameter_modules`).  A list has to name every one of
+    them: ``net.layers`` of a network with norms or connections leaves theirs out, and the gradients of
+    what is left out stay this process's own.  Call :meth:`finish` after ``loss.backward()`` and before the optimiser step.
     ``average=True`` divides by the world size (for mean-type losses); sum-type
     losses keep the plain sum.
 
@@ -125,10 +127,12 @@ class GradientBucket:
     micro-batches): the gradients of a step overwrite the bucket.
     """
 
-    def __init__(self, layers: Iterable[nn.Module], process_group: Optional[dist.ProcessGroup] = None,
+    def __init__(self, layers: Union[nn.Module, Iterable[nn.Module]], process_group: Optional[dist.ProcessGroup] = None,
                  average: bool = False, transport: str = "auto", direct: bool = False, chunks: int = 1) -> None:
         if transport not in ("auto", "nccl", "nvlink"):
             raise ValueError(f"transport must be 'auto', 'nccl' or 'nvlink', got {transport!r}")
+        if hasattr(layers, "parameter_modules"):
+            layers = layers.parameter_modules()
         self.group = process_group
         self.average = average
         self.world = dist.get_world_size(process_group) if dist.is_initialized() else 1

@@ -153,6 +153,18 @@ class KAN(nn.Module):
         net.norms = net.connections = None
         return net
 
+    def parameter_modules(self) -> List[nn.Module]:
+        """The modules that own the parameters, in forward order: every layer with its norm in front of it and its
+        connection behind it (what :class:`GradientBucket` reduces for this network)."""
+        modules: List[nn.Module] = []
+        for i, layer in enumerate(self.layers):
+            if self.norms is not None:
+                modules.append(self.norms[i])
+            modules.append(layer)
+            if self.connections is not None and str(i) in self.connections:
+                modules.append(self.connections[str(i)])
+        return modules
+
     @property
     def widths(self) -> List[int]:
         """Widths of the stream (a gated connection halves its layer's outputs)."""
