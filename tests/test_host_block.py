@@ -226,3 +226,13 @@ def test_scratch_that_16_byte_stores_cannot_reach_is_refused():
     for off in (4, 8):
         assert lib.kanb200_block_backward(ctypes.byref(a), (1 << 20) + off, need, None) == _native.EINVAL
         assert "workspace" in _native.last_error()
+
+
+@pytest.mark.parametrize("config", [dict(norm="rms"), dict(residual=True), dict(norm="layer", residual=True, gate="silu")])
+def test_node_scores_of_networks_of_blocks_are_refused(config):
+    """Walking the layers as a plain chain would score them on inputs that they never see."""
+    from torchsplinekan_b200.pruning import node_scores
+    with pytest.raises(ValueError, match="node_scores works on plain chains"):
+        node_scores(sk.KAN([4, 4, 4], **config), torch.zeros(3, 4))
+    incoming, outgoing = node_scores(sk.KAN([4, 4, 4]), torch.zeros(3, 4))
+    assert len(incoming) == len(outgoing) == 1

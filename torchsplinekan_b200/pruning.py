@@ -39,10 +39,17 @@ class PruneResult:
         return {n: getattr(self, n) for n in names}
 
 
+def _refuse_blocks(model: KAN, what: str) -> None:
+    if model.norms is not None or model.connections is not None:
+        raise ValueError(f"{what} works on plain chains of layers: norms and residual connections tie the widths "
+                         "of their layers together")
+
+
 @torch.no_grad()
 def node_scores(model: KAN, x: torch.Tensor):
     """``(incoming, outgoing)``: per hidden layer one ``[width]`` tensor each
     (spline_kan/pruning.py:55-69)."""
+    _refuse_blocks(model, "node_scores")
     strengths, h = [], x
     for layer in model.layers:
         strengths.append(layer.edge_l1(h))              # [O, I] on this layer's own inputs
@@ -72,9 +79,7 @@ def prune_nodes(model: KAN, x_calib: Optional[torch.Tensor] = None, threshold: f
     ``threshold``; ``model`` is left untouched.  ``keep`` lists the surviving indices per hidden
     layer explicitly (no scoring then); ``min_keep`` nodes per hidden layer always survive, chosen
     by the larger ``min(incoming, outgoing)`` (spline_kan/pruning.py:86-156)."""
-    if model.norms is not None or model.connections is not None:
-        raise ValueError("prune_nodes works on plain chains of layers: norms and residual connections tie the widths "
-                         "of their layers together")
+    _refuse_blocks(model, "prune_nodes")
     hidden = len(model.layers) - 1
     scores_in: List[torch.Tensor] = []
     scores_out: List[torch.Tensor] = []
