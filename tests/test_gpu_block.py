@@ -442,6 +442,32 @@ def test_saturated_gates():
     check_gated(c)
 
 
+@pytest.mark.parametrize("width", [8, 1000, 4096, 40000])
+def test_gates_are_accurate_far_from_zero(width):
+    """The activation alone (a branch of ones next to a stream of zeros leaves its value as it is), over all gates whose
+    sigmoid is a normal number.  Roundings, in units of 2^-24: 2^t 4 and 1 / a 2 (the instructions' bounds), the sum in front of
+    it 1, the remainder of t's rounding 1; SiLU's product 1 more."""
+    rows = 1 << 17 if width <= 8 else 64
+    g = torch.linspace(-87.3, 40.0, rows * width, device="cuda", dtype=torch.float64).float().view(rows, width)
+    x, y = torch.zeros(rows, width, device="cuda"), torch.ones(rows, width, device="cuda")
+    s = torch.sigmoid(g.double())
+    worst = {}
+    for act, want, units in (("sigmoid", s, 8), ("silu", g.double() * s, 9)):
+        got = sk.gated_residual(x, y, gate=g, gate_activation=act).double()
+        worst[act] = float(((got - want).abs() / want.abs().clamp_min(1e-300)).max()) * 2 ** 24
+        assert worst[act] <= units, worst
+    # derivatives: of the magnitudes s and |g| s (1 - s), where 1 - s carries the error of s
+    for act, want, mag in (("sigmoid", s * (1 - s), s), ("silu", s * (1 + g.double() * (1 - s)), s * (1 + g.double().abs()))):
+        leaf = g.clone().requires_grad_()
+        (got,) = torch.autograd.grad(sk.gated_residual(x, y, gate=leaf, gate_activation=act), leaf, torch.ones_like(x))
+        assert float(((got.double() - want).abs() / mag).max()) * 2 ** 24 <= 24
+    ends = torch.tensor([-float("inf"), -1e30, -200.0, 200.0, 1e30, float("inf"), float("nan"), 0.0], device="cuda")
+    at = torch.zeros(rows, width, device="cuda")
+    at[:, :8] = ends
+    got = sk.gated_residual(x, y, gate=at, gate_activation="sigmoid")[0, :8]
+    assert got.isnan().tolist() == [False] * 6 + [True, False] and got[[0, 1, 2, 3, 4, 5, 7]].tolist() == [0, 0, 0, 1, 1, 1, 0.5]
+
+
 # ---- checkpoints -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("rows,width", SIZES)
 @pytest.mark.parametrize("dtype", DTYPES)
