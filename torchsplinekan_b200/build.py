@@ -8,6 +8,8 @@ loaded with ctypes.  nvcc cross-compiles without a GPU.
 from __future__ import annotations
 
 import concurrent.futures
+import functools
+import importlib.metadata
 import os
 import re
 import shutil
@@ -30,13 +32,30 @@ HEADERS = ["kan_block.h", "kan_block.cuh", "kan_block_plan.h", "kan_block_ring.c
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=hidden"]
+CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+
+
+def _nvcc_path() -> str:
+    return shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 
 
 def _nvcc() -> str:
-    cand = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    cand = _nvcc_path()
     if not os.path.exists(cand):
         raise RuntimeError("nvcc not found; the KAN B200 library cannot be built")
     return cand
+
+
+def _cxx() -> str:
+    # The system compiler, whatever $CXX says: the extension must use the same libstdc++ as the
+    # interpreter's other extension modules (a toolchain that links its own copy statically breaks
+    # stream formatting inside the module).
+    return shutil.which("g++", path="/usr/bin:/usr/local/bin:/bin") or shutil.which("g++") or "g++"
+
+
+@functools.lru_cache(maxsize=None)
+def _version(compiler: str) -> str:
+    return subprocess.run([compiler, "--version"], capture_output=True, text=True).stdout
 
 
 def _older_than(target: str, deps) -> bool:
@@ -44,6 +63,42 @@ def _older_than(target: str, deps) -> bool:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+# What a built file was made with besides its sources (compiler and its version, flags, torch where its headers are used) is
+# kept beside the objects: files made with anything else are out of date, whatever their age.
+def _stamp_path(target: str) -> str:
+    return os.path.join(PKG, "build", os.path.basename(target) + ".stamp")
+
+
+def _made_with(target: str):
+    """The stamp of ``target``, None where there is none (built elsewhere)."""
+    try:
+        with open(_stamp_path(target)) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _make(cmd, target: str, what: str, stamp: str) -> str:
+    """Runs ``cmd -o target`` and returns its messages.  ``target`` appears when it is complete, and its stamp after it."""
+    os.makedirs(os.path.dirname(_stamp_path(target)), exist_ok=True)
+    r = subprocess.run([*cmd, "-o", target + ".tmp"], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed for {what}:\n{r.stdout}\n{r.stderr[-6000:]}")
+    os.replace(target + ".tmp", target)
+    with open(_stamp_path(target) + ".tmp", "w") as f:
+        f.write(stamp)
+    os.replace(_stamp_path(target) + ".tmp", _stamp_path(target))
+    return r.stderr
+
+
+def _library_stamp() -> str:
+    return "\n".join([_version(_nvcc()), *ARCH_FLAGS, *NVCC_FLAGS])
+
+
+def _extension_stamp() -> str:
+    return "\n".join([_version(_cxx()), importlib.metadata.version("torch"), sys.version, *CXX_FLAGS])
 
 
 def _includes(src: str) -> set:
@@ -61,7 +116,10 @@ def _includes(src: str) -> set:
 
 
 def _stale() -> bool:
-    return _older_than(LIB_PATH, [os.path.join(CSRC, s) for s in SOURCES + HEADERS])
+    if _older_than(LIB_PATH, [os.path.join(CSRC, s) for s in SOURCES + HEADERS]):
+        return True
+    made = _made_with(LIB_PATH)                     # without a compiler here its version says nothing
+    return made is not None and shutil.which(_nvcc_path()) is not None and made != _library_stamp()
 
 
 def ext_path() -> str:
@@ -89,7 +147,8 @@ def build_extension(force: bool = False) -> str:
     import sysconfig
     target = ext_path()
     deps = [os.path.join(CSRC, s) for s in EXT_SOURCES + EXT_HEADERS]
-    if not force and not _older_than(target, deps + [LIB_PATH]):
+    stamp = _extension_stamp() if shutil.which(_cxx()) else None
+    if not force and not _older_than(target, deps + [LIB_PATH]) and (stamp is None or _made_with(target) in (None, stamp)):
         return target
     import torch
     from torch.utils import cpp_extension as ce
@@ -98,35 +157,23 @@ def build_extension(force: bool = False) -> str:
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cudart = ["-L" + cudart_dir, "-l:libcudart.so.12", "-Wl,-rpath," + os.path.abspath(cudart_dir)] \
         if os.path.exists(os.path.join(cudart_dir, "libcudart.so.12")) else ["-L" + os.path.join(cuda_home, "lib64"), "-lcudart"]
-    # The system compiler, whatever $CXX says: the extension must use the same libstdc++ as the
-    # interpreter's other extension modules (a toolchain that links its own copy statically breaks
-    # stream formatting inside the module).
-    cxx = shutil.which("g++", path="/usr/bin:/usr/local/bin:/bin") or shutil.which("g++") or "g++"
-    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
-             "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+    cxx = _cxx()
+    flags = [*CXX_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
              *["-I" + p for p in ce.include_paths()], "-I" + sysconfig.get_paths()["include"],
              "-I" + os.path.join(cuda_home, "include")]
-    obj_dir = os.path.join(PKG, "build")
-    os.makedirs(obj_dir, exist_ok=True)
-
-    def run(cmd, what: str) -> None:
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"g++ failed for {what}:\n{r.stdout}\n{r.stderr[-6000:]}")
 
     def compile_one(src: str) -> str:
-        obj = os.path.join(obj_dir, src.replace(".cpp", ".ext.o"))
-        if force or _older_than(obj, [os.path.join(CSRC, src), *_includes(src)]):
-            run([cxx, *flags, "-c", os.path.join(CSRC, src), "-o", obj], src)
+        obj = os.path.join(PKG, "build", src.replace(".cpp", ".ext.o"))
+        if force or _older_than(obj, [os.path.join(CSRC, src), *_includes(src)]) or _made_with(obj) != stamp:
+            _make([cxx, *flags, "-c", os.path.join(CSRC, src)], obj, src, stamp)
         return obj
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=len(EXT_SOURCES)) as ex:
         objs = list(ex.map(compile_one, EXT_SOURCES))
-    run([cxx, "-shared", *objs, "-o", target + ".tmp",
-         "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
-         "-L" + LIB_DIR, "-lkan_b200", "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib, *cudart], "the operator layer")
-    os.replace(target + ".tmp", target)
+    _make([cxx, "-shared", *objs,
+           "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+           "-L" + LIB_DIR, "-lkan_b200", "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib, *cudart], target,
+          "the operator layer", stamp)
     return target
 
 
@@ -143,33 +190,22 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    obj_dir = os.path.join(PKG, "build")
-    os.makedirs(obj_dir, exist_ok=True)
-    nvcc = _nvcc()
+    nvcc, stamp = _nvcc(), _library_stamp()
 
     def compile_one(src: str) -> str:
-        obj = os.path.join(obj_dir, src.replace(".cu", ".o"))
-        if not force and not verbose and not _older_than(obj, [os.path.join(CSRC, src), *_includes(src)]):
+        obj = os.path.join(PKG, "build", src.replace(".cu", ".o"))
+        if not force and not verbose and not _older_than(obj, [os.path.join(CSRC, src), *_includes(src)]) \
+                and _made_with(obj) == stamp:
             return obj
-        cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
+        messages = _make([nvcc, *(["-Xptxas", "-v"] if verbose else []), *ARCH_FLAGS, *NVCC_FLAGS, "-c", os.path.join(CSRC, src)],
+                         obj, src, stamp)
         if verbose:
-            cmd.insert(1, "-Xptxas")
-            cmd.insert(2, "-v")
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-        if verbose:
-            sys.stderr.write(r.stderr)
+            sys.stderr.write(messages)
         return obj
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
         objs = list(ex.map(compile_one, SOURCES))
-    tmp = LIB_PATH + ".tmp"
-    cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", tmp, *objs]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, LIB_PATH)
+    _make([nvcc, *ARCH_FLAGS, "-shared", *objs], LIB_PATH, "the library", stamp)
     return LIB_PATH
 
 
