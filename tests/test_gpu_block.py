@@ -547,6 +547,16 @@ def test_refusals_on_the_device():
         torch.autograd.grad(out.sum(), t, create_graph=True)
 
 
+def test_function_transforms_are_refused():
+    x = torch.ones(3, 4, 8, device="cuda")
+    for call in (lambda: torch.vmap(lambda t: sk.block_norm(t))(x), lambda: torch.func.grad(lambda t: sk.block_norm(t).sum())(x),
+                 lambda: torch.vmap(lambda t: sk.gated_residual(t, t))(x), lambda: torch.vmap(lambda t: sk.pack_activation(t))(x)):
+        with pytest.raises(RuntimeError, match="torch.func"):
+            call()
+    got = sk.block_norm(torch.nn.Parameter(x), torch.nn.Parameter(torch.ones(8, device="cuda")))
+    assert got.requires_grad and torch.allclose(got, x)
+
+
 def test_graph_is_used_once_and_inputs_stay():
     """A second backward without retain_graph, and an input changed in between, are errors; forward mode is refused."""
     x = stream(5, 64, torch.float32).requires_grad_()

@@ -236,3 +236,18 @@ def test_node_scores_of_networks_of_blocks_are_refused(config):
         node_scores(sk.KAN([4, 4, 4], **config), torch.zeros(3, 4))
     incoming, outgoing = node_scores(sk.KAN([4, 4, 4]), torch.zeros(3, 4))
     assert len(incoming) == len(outgoing) == 1
+
+
+def test_tensors_without_memory_are_refused_by_name():
+    """Fake CUDA tensors need no device: the refusal comes before anything touches one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w = torch.empty(4, 8, device="cuda"), torch.ones(8, device="cuda", requires_grad=True)
+        codes, scales = torch.empty(4, 8, dtype=torch.int8, device="cuda"), torch.empty(4, 1, device="cuda")
+        for name, call in (("block_norm", lambda: sk.block_norm(x, w)),
+                           ("gated_residual", lambda: sk.gated_residual(x, x, scale=w, next_norm="rms")),
+                           ("pack_activation", lambda: sk.pack_activation(x)),
+                           ("unpack_activation", lambda: sk.unpack_activation(codes, scales))):
+            with pytest.raises(RuntimeError, match=name + ": fake tensors"):
+                call()
+        assert sk.block_norm(torch.empty(4, 8)).shape == (4, 8)          # the dense formulas trace

@@ -70,6 +70,15 @@ void check_settings(const char* what, const Tensor& x, double eps, int64_t check
     TORCH_CHECK(checkpoint >= KANB200_PACK_NONE && checkpoint <= KANB200_PACK_E4M3, what, ": unknown checkpoint format");
 }
 
+// The native path reads memory: no tensors that stand for others (fake tensors, torch.func transforms, vmap, subclasses).
+void check_memory(const char* what, std::initializer_list<Tensor> ts) {
+    const c10::DispatchKeySet stands_in({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                         c10::DispatchKey::FuncTorchGradWrapper});
+    for (const Tensor& t : ts)
+        TORCH_CHECK(!t.defined() || !t.key_set().has_any(stands_in), what,
+                    ": fake tensors, tensor subclasses and torch.func transforms are not available on CUDA");
+}
+
 int64_t row_count(const Tensor& x) {
     int64_t n = 1;
     for (int64_t d = 0; d + 1 < x.dim(); ++d) n *= x.size(d);
@@ -310,6 +319,7 @@ Tensor block_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     check_norm(x, w, b, kind, eps, checkpoint);
     TORCH_CHECK(x.is_cuda() || checkpoint == KANB200_PACK_NONE, "block_norm: 8-bit checkpoints need CUDA tensors");
     if (!x.is_cuda() || x.numel() == 0) return norm_composite(x, w, b, kind, eps);
+    check_memory("block_norm", {x, w, b});
     if (!wants_grad({x, w, b}, "block_norm")) return norm_forward(x, w, b, kind, eps, checkpoint, nullptr);
     Tensor record;
     Tensor h = norm_forward(x, w, b, kind, eps, checkpoint, &record);
@@ -618,6 +628,7 @@ py::object gated_residual(const Tensor& x, const Tensor& y, const std::optional<
     check_gated(g);
     TORCH_CHECK(x.is_cuda() || checkpoint == KANB200_PACK_NONE, "gated_residual: 8-bit checkpoints need CUDA tensors");
     variable_list outs;
+    if (x.is_cuda() && x.numel() > 0) check_memory("gated_residual", {g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb});
     if (!x.is_cuda() || x.numel() == 0) {
         outs = gated_composite(g);
     } else if (!wants_grad({g.x, g.y, g.gate, g.scale, g.pw, g.pb, g.nw, g.nb}, "gated_residual")) {
@@ -653,6 +664,7 @@ Packed pack_rows(const Tensor& x, int format) {
     const int code = stream_code(x, what);
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must have at least one column, got ", x.sizes());
     TORCH_CHECK(x.is_cuda(), what, ": x must be a CUDA tensor (this backend has no CPU kernels)");
+    check_memory(what, {x});
     c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     const int64_t rows = row_count(x), width = x.size(-1);
@@ -685,6 +697,7 @@ Tensor unpack_rows(const Tensor& codes, const Tensor& scales, at::ScalarType dty
                 scales.scalar_type());
     TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(), what,
                 ": codes and scales must be CUDA tensors on one device");
+    check_memory(what, {codes, scales});
     c10::cuda::CUDAGuard guard(codes.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
     const Tensor cc = codes.contiguous(), sc = scales.contiguous();
