@@ -241,6 +241,32 @@ def test_many_rows_without_a_sum_over_the_row(rows, width, form):
     check_gated(make_gated(rows, width, torch.float32, "row", post="rms", next="rms", form=form), only=("gate",))
 
 
+@pytest.mark.parametrize("rows,width", [(1, 8), (7, 64), (4097, 20), (5000, 333), (3001, 1024), (1001, 5000), (37, 33001)])
+def test_sums_over_rows_hold_every_row_once(rows, width):
+    """Sums of small whole numbers have no rounding, in whatever order they are formed: a row that is left out or counted twice
+    shows, however many there are."""
+    whole = lambda *shape, seed: torch.randint(-8, 9, shape, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).float()
+    x, y, dout = whole(rows, width, seed=1), whole(rows, width, seed=2), whole(rows, width, seed=3)
+    scale, gate = whole(width, seed=4).requires_grad_(), whole(width, seed=5).requires_grad_()
+    for g, factor in ((None, 1.0), (gate, gate.detach())):
+        out = sk.gated_residual(x, y, gate=g, scale=scale)
+        got = torch.autograd.grad(out, [scale] if g is None else [scale, gate], dout)
+        assert torch.equal(got[0], (dout.double() * y.double()).sum(0).float() * factor)
+        if g is not None:
+            assert torch.equal(got[1], (dout.double() * y.double()).sum(0).float() * scale.detach())
+    b = torch.zeros(width, device="cuda", requires_grad=True)
+    (got,) = torch.autograd.grad(sk.block_norm(x, None, b, kind="layer"), b, dout)
+    assert torch.equal(got, dout.sum(0))
+    out = sk.gated_residual(x, y, post_norm="rms", post_bias=b)
+    (got,) = torch.autograd.grad(out, b, dout)
+    assert torch.equal(got, dout.sum(0))
+    for batch in (d for d in (3, 7, 11) if rows % d == 0):
+        per = whole(batch, 1, width, seed=6).requires_grad_()
+        view = lambda t: t.view(batch, -1, width)
+        (got,) = torch.autograd.grad(sk.gated_residual(view(x), view(y), gate=per), per, view(dout))
+        assert torch.equal(got, view(dout * y).sum(1, keepdim=True))
+
+
 def test_only_one_result_used():
     c = make_gated(40, 200, torch.float32)
     check_gated(c, use_h=False)
