@@ -368,6 +368,28 @@ def test_column_sums_at_any_address():
             assert torch.equal(row[1:-1], v) and bool(torch.isnan(row[[0, -1]]).all())
 
 
+def test_views_that_negate_lazily():
+    """The imaginary part of a conjugate negates when it is read; its memory holds the other sign."""
+    z = torch.complex(randn(40, 1, dtype=torch.float32), randn(40, 1, dtype=torch.float32, seed=1))
+    lazy, w = z.conj().imag, torch.full((1,), 2.0, device="cuda")
+    assert lazy.is_neg()
+    plain = lazy.clone()
+    minus = lambda t: torch._neg_view(-t)
+    x, v = randn(9, 64, dtype=torch.float32, seed=2), randn(64, dtype=torch.float32, seed=3)
+    for got, want in ((sk.block_norm(lazy, w), sk.block_norm(plain, w)),
+                      (sk.gated_residual(lazy, lazy), 2 * plain), (sk.block_norm(minus(x), minus(v)), sk.block_norm(x, v)),
+                      (sk.gated_residual(x, minus(x), scale=minus(v)), sk.gated_residual(x, x, scale=v)),
+                      (sk.unpack_activation(*sk.pack_activation(lazy)), sk.unpack_activation(*sk.pack_activation(plain)))):
+        assert torch.equal(got, want)
+    grads = []
+    for f in (minus, lambda t: t):
+        leaf, wl = x.clone().requires_grad_(), v.clone().requires_grad_()
+        grads.append(torch.autograd.grad(sk.gated_residual(f(leaf), f(leaf), scale=f(wl), post_norm="rms", next_norm="layer"),
+                                         [leaf, wl], (f(x), f(x))))
+    for p, q in zip(*grads):
+        assert torch.equal(p, q)
+
+
 def test_broadcast_rows_and_gradients():
     """Rows of stride 0 in the inputs and in the incoming gradients."""
     one = randn(1, 96, dtype=torch.float32).expand(50, 96)

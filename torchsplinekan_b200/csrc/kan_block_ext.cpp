@@ -46,8 +46,12 @@ struct Rows {
     int64_t stride = 0;
     const void* ptr() const { return keep.defined() ? keep.data_ptr() : nullptr; }
 };
-Rows as_rows(const Tensor& t, int64_t rows, int64_t width) {
-    if (!t.defined()) return {};
+// A dense copy of a vector where it is not its own memory already.  (Memory says nothing of a view that negates lazily, such
+// as the imaginary part of a conjugate.)
+Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+Rows as_rows(const Tensor& given, int64_t rows, int64_t width) {
+    if (!given.defined()) return {};
+    const Tensor t = given.resolve_neg();
     const int64_t shape[2] = {rows, width};
     const auto strides = at::detail::computeStride(t.sizes(), t.strides(), at::IntArrayRef(shape, 2));
     if (strides && ((*strides)[1] == 1 || width == 1) && ((*strides)[0] >= 0)) return {t, (*strides)[0]};
@@ -211,7 +215,7 @@ Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t k
         *record = norm_record(checkpoint).make(a, x);
     }
     const Rows xr = as_rows(x, a.rows, a.width);
-    const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+    const Tensor wc = dense(w), bc = dense(b);
     a.x = xr.ptr();
     a.x_stride = xr.stride;
     a.next_weight = cptr(wc);
@@ -300,7 +304,7 @@ struct BlockNormNode : public SavedNode {
         a.eps = eps;
         a.x = xr.ptr();
         a.x_stride = xr.stride;
-        const Tensor wc = w.defined() ? w.contiguous() : w;
+        const Tensor wc = dense(w);
         a.next_weight = cptr(wc);
         norm_record(checkpoint).find(a, record);
         a.dh = dr.ptr();
@@ -463,8 +467,7 @@ variable_list gated_forward(const Gated& g, Tensor* record) {
     const Rows xr = as_rows(g.x, g.rows, g.width);
     Rows yr, gr;
     branch_rows(g, yr, a.gate, a.gate_stride, gr);
-    const auto vec = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
-    const Tensor scale = vec(g.scale), pw = vec(g.pw), pb = vec(g.pb), nw = vec(g.nw), nb = vec(g.nb);
+    const Tensor scale = dense(g.scale), pw = dense(g.pw), pb = dense(g.pb), nw = dense(g.nw), nb = dense(g.nb);
     a.x = xr.ptr();
     a.x_stride = xr.stride;
     a.y = yr.ptr();
@@ -554,7 +557,6 @@ struct GatedResidualNode : public SavedNode {
             a.gate = gr.ptr();
             a.gate_stride = gr.stride;
         }
-        const auto dense = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
         const Tensor scale = dense(g.scale), pw = dense(g.pw), pb = dense(g.pb), nw = dense(g.nw);
         a.x = xr.ptr();
         a.x_stride = xr.stride;
@@ -700,7 +702,7 @@ Tensor unpack_rows(const Tensor& codes, const Tensor& scales, at::ScalarType dty
     check_memory(what, {codes, scales});
     c10::cuda::CUDAGuard guard(codes.device());
     const cudaStream_t st = at::cuda::getCurrentCUDAStream();
-    const Tensor cc = codes.contiguous(), sc = scales.contiguous();
+    const Tensor cc = codes.contiguous(), sc = dense(scales);
     Tensor x = fresh(codes.sizes(), dtype, codes);
     check_rc(kanb200_unpack_activation(stream_code(x, what),
                                        codes.scalar_type() == at::kChar ? KANB200_PACK_INT8 : KANB200_PACK_E4M3, cptr(cc),
