@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <new>
 #include <set>
 #include <utility>
 
@@ -555,7 +556,10 @@ cudaError_t allow_shared_memory(const void* kernel) {
     std::lock_guard<std::mutex> lock(mutex);
     if (allowed.count({kernel, device})) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
-    if (e == cudaSuccess) allowed.insert({kernel, device});
+    try {
+        if (e == cudaSuccess) allowed.insert({kernel, device});
+    } catch (const std::bad_alloc&) {                        // not remembered, set again by the next call
+    }
     return e;
 }
 
