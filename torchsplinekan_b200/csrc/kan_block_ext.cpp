@@ -15,6 +15,7 @@
 
 #include <array>
 #include <cmath>
+#include <functional>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -48,10 +49,11 @@ struct Rows {
 };
 // A dense copy of a vector where it is not its own memory already.  (Memory says nothing of a view that negates lazily, such
 // as the imaginary part of a conjugate.)
-Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+Tensor own_sign(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return t.defined() ? own_sign(t).contiguous() : t; }
 Rows as_rows(const Tensor& given, int64_t rows, int64_t width) {
     if (!given.defined()) return {};
-    const Tensor t = given.resolve_neg();
+    const Tensor t = own_sign(given);
     const int64_t shape[2] = {rows, width};
     const auto strides = at::detail::computeStride(t.sizes(), t.strides(), at::IntArrayRef(shape, 2));
     if (strides && ((*strides)[1] == 1 || width == 1) && ((*strides)[0] >= 0)) return {t, (*strides)[0]};
@@ -75,7 +77,7 @@ void check_settings(const char* what, const Tensor& x, double eps, int64_t check
 }
 
 // The native path reads memory: no tensors that stand for others (fake tensors, torch.func transforms, vmap, subclasses).
-void check_memory(const char* what, std::initializer_list<Tensor> ts) {
+void check_memory(const char* what, std::initializer_list<std::reference_wrapper<const Tensor>> ts) {
     const c10::DispatchKeySet stands_in({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                          c10::DispatchKey::FuncTorchGradWrapper});
     for (const Tensor& t : ts)
