@@ -107,6 +107,29 @@ def test_layer_checkpoint_and_gradient_sink():
         bucket.remove()
 
 
+def test_network_of_blocks_and_gradient_buckets():
+    """Buckets over a whole network: the layers' gradients from their sinks, those of norms and connections from autograd."""
+    make = lambda: seeded(lambda: sk.KAN([64, 128, 128, 128], norm="layer", residual=True, gate="silu", activation_checkpoint="int8",
+                                         backend="cuda")).cuda()
+    net, plain = make(), make()
+    plain.load_state_dict(net.state_dict())
+    x = torch.randn(30000, 64, device="cuda")
+    bucket = sk.GradientBucket(net, direct=True)
+    try:
+        assert len(bucket.buckets) == len(net.parameter_modules()) == 8 and len(bucket._sinks) == 3
+        for _ in range(2):
+            bucket.zero_grad()
+            net(x).square().mean().backward()
+            bucket.finish()
+        plain(x).square().mean().backward()
+        held = {b.data_ptr(): b.data_ptr() + 4 * b.numel() for b in bucket.buckets}
+        for (n, p), q in zip(net.named_parameters(), plain.parameters()):
+            assert rel(p.grad, q.grad) < 1e-6, n
+            assert any(lo <= p.grad.data_ptr() < hi for lo, hi in held.items()), n
+    finally:
+        bucket.remove()
+
+
 # ---- networks of blocks --------------------------------------------------------------------------------------------------
 CONFIGS = [dict(norm="rms"), dict(norm="layer", residual=True), dict(norm="rms", residual=True, gate="silu", scale_init=0.3),
            dict(residual=True), dict(norm="layer", residual=True, gate="sigmoid")]

@@ -9,8 +9,9 @@ be float32, float64, bfloat16 or float16; the *branch* (``y``, gates, parameters
 :class:`KANLinear` computes in: float64 next to a float64 stream, float32 otherwise.
 
 CUDA tensors run on the native kernels (one kernel forward; backward one kernel plus the fixed-order sum of the
-parameter gradients), CPU tensors on dense PyTorch formulas.  ``create_graph=True`` is exact without a checkpoint and
-raises with one.
+parameter gradients), CPU tensors on dense PyTorch formulas.  Any strides and alignments are taken; widths that are a
+multiple of four with rows and parameters on 16-byte boundaries run fastest.  ``create_graph=True`` is exact without a
+checkpoint and raises with one.  Fake tensors and ``torch.func`` transforms are refused on CUDA.
 """
 from __future__ import annotations
 
@@ -41,7 +42,8 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """``(x - m) r * weight + bias`` over the last dimension, in the branch's type: the norm in front of a layer.
 
     ``kind``: "rms" (``m = 0``, ``r = (mean(x^2) + eps)^-1/2``) or "layer" (``m = mean(x)``,
-    ``r = (mean((x - m)^2) + eps)^-1/2``).  Rows whose squares overflow the branch's type have ``r = 0``.
+    ``r = (mean((x - m)^2) + eps)^-1/2``).  Rows whose sum of squares overflows the branch's type have ``r = 0``;
+    rows whose sum overflows as well come back as NaN from "layer".
 
     ``checkpoint``: None keeps ``x`` for the backward; "int8" / "e4m3" keep 8-bit codes of it instead (see
     :func:`pack_activation`), written by the same kernel.  The result is the same; the gradients are those of the

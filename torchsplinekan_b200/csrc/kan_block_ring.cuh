@@ -15,9 +15,15 @@
 //     16777 x 1000: 85 us, most of the stalls).
 //   * Sums over a row: lanes by shuffles, warps through shared memory with a barrier of the team alone, blocks of a
 //     cluster through each other's shared memory; every thread gets the same bits.
-//   * Issue slots bound these kernels before bandwidth does, so: what a row costs besides its elements (sums, barriers,
-//     addresses) is shared by 4 V elements; distances between a thread's elements are constants; float arithmetic works
-//     on pairs (one instruction for two elements).
+//   * Four warps per scheduler is what the registers of sums and parameters allow, so besides bandwidth the number of
+//     instructions and their latencies count: what a row costs besides its elements (sums, barriers, addresses) is shared by
+//     4 V elements; distances between a thread's elements are constants; float arithmetic works on pairs (one instruction for
+//     two elements).
+//
+// What bounds them, by counters: the norm alone memory (DRAM 74 to 80 % of nominal, a copy reaches
+// 85 %; issue slots 26 to 33 %); the float32 connection memory and latencies together (71 %, issue slots 52 to 54 %); with 8-bit
+// codes instructions and latencies (issue slots 62 to 64 %, DRAM 37 to 65 %); rows whose width is not a multiple of four their
+// element-wise copies and loads (DRAM 21 to 36 %).
 //
 // Measured, float32: norm of 65536 x 1024 forward 89 us (6.0 TB/s), backward 137 us (5.9 TB/s); connection of 16384 x 1024
 // with a gate per row and both norms forward 54 us (6.2 TB/s), backward 93 us (5.8 TB/s); a copy runs at 6.55 TB/s.

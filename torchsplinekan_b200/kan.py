@@ -23,7 +23,10 @@ class KAN(nn.Module):
     the norm of the next layer is fused into that connection.  ``gate``: "sigmoid" or "silu": such a
     layer has twice the outputs, value and gate, and the connection multiplies by ``act(gate)``.
     ``scale_init``: the residual scales' first value.  ``activation_checkpoint``: "int8" or "e4m3": layers,
-    norms and connections keep what their backward reads as 8-bit codes (CUDA inputs)."""
+    norms and connections keep what their backward reads as 8-bit codes (CUDA inputs).
+
+    A float16 or bfloat16 input is a stream of that type through the connections and needs ``norm``: the layers
+    compute in the type of their parameters, which is what a norm returns, and refuse another one."""
 
     def __init__(self, layers_hidden: List[int], grid_size: int = 5, spline_order: int = 3,
                  scale_noise: float = 0.1, scale_base: float = 1.0, scale_spline: float = 1.0,
