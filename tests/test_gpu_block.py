@@ -466,6 +466,17 @@ def test_squares_that_overflow():
             assert float(h[1].abs().max()) > 0.5
 
 
+def test_sums_that_overflow():
+    """Beyond that the mean itself overflows: NaN from the mean-subtracting norm, still 0 from RMS, and only in that row."""
+    for width in (24, 512, 40000):
+        x = torch.full((3, width), 3e38, device="cuda")
+        x[1] = randn(width, dtype=torch.float32)
+        assert bool((sk.block_norm(x)[[0, 2]] == 0).all())
+        h = sk.block_norm(x, kind="layer")
+        assert h.isnan().all(1).tolist() == [True, False, True] and bool(torch.isfinite(h[1]).all())
+        assert bool(sk.block_norm(x.cpu(), kind="layer")[0].isnan().all())
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_a_bad_row_stays_alone(bad):
     """NaN and infinities make their own row NaN, in both directions, and no other."""
